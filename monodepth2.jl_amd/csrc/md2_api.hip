@@ -5,6 +5,7 @@
 // (the reference gets them from Zygote).  A step is enqueued on the caller's stream plus internal side streams (weight gradients,
 // pose branch, RCCL buckets) forked and joined by events; no allocation or host synchronisation happens inside a step.
 #include "md2_internal.h"
+#include "muon.h"
 #include "../../include/md2hip.h"
 #include <vector>
 #include <string>
@@ -12,6 +13,7 @@
 #include <cmath>
 #include <algorithm>
 #include <cstdlib>
+#include <exception>
 #include <dlfcn.h>
 #include <rccl/rccl.h>        // types only: the RCCL entry points are resolved with dlsym at md2_comm_init (no link-time dependency)
 
@@ -1472,6 +1474,99 @@ int32_t md2_adam_raw(float* p, const float* g, float* m, float* v, int64_t n, in
     if (n <= 0 || step < 1) return 2;
     launch_adam(p, g, m, v, (long)n, (float)(1.0 - std::pow(0.9, step)), (float)(1.0 - std::pow(0.999, step)), (float)lr, grad_scale, (hipStream_t)stream);
     return hipGetLastError() != hipSuccess;
+}
+
+
+// ---- Muon (muon.hip) ---------------------------------------------------------------------------------------------------
+// (no exception crosses the ABI: the weight lists are std::vectors)
+#define NS_ENTRY(...) try { __VA_ARGS__ } catch (const std::exception& e) { g_create_err = e.what(); return 3; }
+static int ns_fail(const char* what, const char* why) { g_create_err = std::string(what) + ": " + why; return 2; }
+static int ns_finish(const char* what) {
+    const hipError_t e = hipGetLastError();
+    if (e == hipSuccess) return 0;
+    g_create_err = std::string(what) + ": kernel launch: " + hipGetErrorString(e); return 1;
+}
+static int ns_options(NsOptions& o, int32_t steps, const double* co, double eps, const char* what) {
+    if (!co) return ns_fail(what, "null coefficients");
+    o.steps = steps; o.eps = eps; for (int i = 0; i < 3; ++i) o.coef[i] = co[i];
+    return 0;
+}
+int64_t md2_newton_schulz_workspace(int64_t batch, int64_t rows, int64_t cols, int32_t steps, int32_t pullback) {
+    try { NsMatrices q; q.batch = batch; q.rows = rows; q.cols = cols; return ns_workspace(pullback ? NS_BACKWARD : NS_FORWARD, steps, &q, 1); } catch (const std::exception&) { return -1; }
+}
+static int ns_call(const char* what, int kind, const void* x, const void* d, void* y, int64_t batch, int64_t rows, int64_t cols, const int64_t* xs, const int64_t* ds, int32_t dtype, int32_t steps,
+                   const double* co, double eps, void* ws, int64_t ws_bytes, void* stream) {
+    NsOptions o; if (int r = ns_options(o, steps, co, eps, what)) return r;
+    if (!xs || (kind == NS_BACKWARD && !ds)) return ns_fail(what, "null strides");
+    if (dtype < NS_F32 || dtype > NS_F16) return ns_fail(what, "dtype must be 0 (fp32), 1 (bf16) or 2 (fp16)");
+    NsMatrices q; q.x = x; q.d = d; q.y = y; q.batch = batch; q.rows = rows; q.cols = cols;
+    for (int i = 0; i < 3; ++i) { q.xs[i] = xs[i]; q.ds[i] = ds ? ds[i] : 0; }
+    const char* why = "";
+    if (int r = ns_run(kind, dtype, &q, 1, o, ws, ws_bytes, (hipStream_t)stream, &why)) { ns_fail(what, why); return r; }
+    return ns_finish(what);
+}
+int32_t md2_newton_schulz(const void* x, void* y, int64_t batch, int64_t rows, int64_t cols, const int64_t* xs, int32_t dtype, int32_t steps, const double* co, double eps, void* ws,
+                          int64_t ws_bytes, void* stream) {
+    NS_ENTRY(return ns_call("newton_schulz", NS_FORWARD, x, nullptr, y, batch, rows, cols, xs, nullptr, dtype, steps, co, eps, ws, ws_bytes, stream);)
+}
+int32_t md2_newton_schulz_bwd(const void* x, const void* dout, void* dx, int64_t batch, int64_t rows, int64_t cols, const int64_t* xs, const int64_t* ds, int32_t dtype, int32_t steps,
+                              const double* co, double eps, void* ws, int64_t ws_bytes, void* stream) {
+    NS_ENTRY(return ns_call("newton_schulz_bwd", NS_BACKWARD, x, dout, dx, batch, rows, cols, xs, ds, dtype, steps, co, eps, ws, ws_bytes, stream);)
+}
+int64_t md2_muon_workspace(const int64_t* rows, const int64_t* cols, int32_t count, int32_t steps) {
+    try {
+        if (!rows || !cols || count < 1) return -1;
+        std::vector<NsMatrices> q((size_t)count);
+        for (int i = 0; i < count; ++i) { q[i].rows = rows[i]; q[i].cols = cols[i]; }
+        return ns_workspace(NS_MUON, steps, q.data(), count);
+    } catch (const std::exception&) { return -1; }
+}
+// what md2_muon_raw and md2_muon_step share: the hyperparameters' checks and the list
+struct MuonHyper { double lr, momentum; int32_t nesterov; double weight_decay; int32_t adjust; float grad_scale; int32_t steps; const double* co; double eps; };
+static const char* muon_check(const MuonHyper& y) {
+    if (!(y.lr >= 0) || !std::isfinite(y.lr)) return "lr must be finite and not negative";
+    if (!(y.momentum >= 0 && y.momentum < 1)) return "momentum must be in [0, 1)";
+    if (!(y.weight_decay >= 0) || !std::isfinite(y.weight_decay)) return "weight_decay must be finite and not negative";
+    if (y.adjust != 0 && y.adjust != 1) return "adjust must be 0 (spectral) or 1 (rms)";
+    if (!std::isfinite(y.grad_scale)) return "grad_scale must be finite";
+    return nullptr;
+}
+static NsMatrices muon_matrix(float* p, const float* g, float* m, int64_t rows, int64_t cols, const MuonHyper& y) {
+    NsMatrices q; q.x = m; q.d = g; q.y = p; q.rows = rows; q.cols = cols;
+    q.xs[1] = q.ds[1] = cols; q.xs[2] = q.ds[2] = 1;
+    const double s = y.adjust ? 0.2 * std::sqrt((double)std::max(rows, cols)) : std::sqrt(std::max(1.0, (double)rows / (double)cols));
+    q.alpha = (float)(y.lr * s);
+    return q;
+}
+static int muon_run(const char* what, const std::vector<NsMatrices>& q, const MuonHyper& y, void* ws, int64_t ws_bytes, hipStream_t s, const char** why) {
+    if ((*why = muon_check(y))) return 2;
+    NsOptions o; if (ns_options(o, y.steps, y.co, y.eps, what)) { *why = "null coefficients"; return 2; }
+    o.lr = y.lr; o.momentum = y.momentum; o.nesterov = y.nesterov != 0; o.weight_decay = y.weight_decay; o.grad_scale = y.grad_scale;
+    return ns_run(NS_MUON, NS_F32, q.data(), (int)q.size(), o, ws, ws_bytes, s, why);
+}
+int32_t md2_muon_raw(float* const* p, const float* const* g, float* const* m, const int64_t* rows, const int64_t* cols, int32_t count, double lr, double momentum, int32_t nesterov,
+                     double weight_decay, int32_t adjust, float grad_scale, int32_t steps, const double* co, double eps, void* ws, int64_t ws_bytes, void* stream) {
+    NS_ENTRY(
+        if (!p || !g || !m || !rows || !cols || count < 1) return ns_fail("muon_raw", "null list, or no weights");
+        const MuonHyper y{lr, momentum, nesterov, weight_decay, adjust, grad_scale, steps, co, eps};
+        std::vector<NsMatrices> q; struct Span { uintptr_t lo, hi; bool write; }; std::vector<Span> spans;
+        for (int i = 0; i < count; ++i) {
+            if (rows[i] < 1 || cols[i] < 1 || rows[i] > (1 << 20) || cols[i] > (1 << 20)) return ns_fail("muon_raw", "sizes must be positive, a side at most 2^20");
+            q.push_back(muon_matrix(p[i], g[i], m[i], rows[i], cols[i], y));
+            const uintptr_t n = (uintptr_t)(rows[i] * cols[i]) * 4;
+            spans.push_back({(uintptr_t)p[i], (uintptr_t)p[i] + n, true}); spans.push_back({(uintptr_t)m[i], (uintptr_t)m[i] + n, true}); spans.push_back({(uintptr_t)g[i], (uintptr_t)g[i] + n, false});
+        }
+        // nothing that the step writes may overlap anything else of the call: the weights are updated at the same time
+        std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.lo < b.lo; });
+        uintptr_t end_any = 0; uintptr_t end_write = 0;
+        for (const Span& a : spans) {
+            if (a.lo < end_write || (a.write && a.lo < end_any)) return ns_fail("muon_raw", "a weight or momentum overlaps another tensor of the call");
+            end_any = std::max(end_any, a.hi); if (a.write) end_write = std::max(end_write, a.hi);
+        }
+        const char* why = "";
+        if (int r = muon_run("muon_raw", q, y, ws, ws_bytes, (hipStream_t)stream, &why)) { ns_fail("muon_raw", why); return r; }
+        return ns_finish("muon_raw");
+    )
 }
 
 

@@ -1,0 +1,563 @@
+// muon.hip -- orthogonalisation of matrices by Newton-Schulz products, its pullback, and the Muon update that is built on it.
+//
+// The mathematics.  X0 = X / max(|X|_F, eps), taken with its short side first (m rows, n >= m columns), and `steps` times
+//     A = X X^T,   B = b A + c A A,   X <- a X + B X          (an odd quintic in the singular values of X; nothing else of X changes).
+// The pullback walks the iterates back, G = dL/dX_{k+1} -> dL/dX_k, with the symmetric S = G X^T + X G^T:
+//     dL/dX_k = a G + B G + V X,   V = b S + c (S A + A S),
+// and goes through the normalisation: dX = (G - X0 <X0, G>) / |X|_F   (G / eps where the norm was clamped).
+// Every product is one of two forms: a symmetric result L R^T whose K axis is contiguous in both operands, of which the tiles on and above the diagonal are computed and the
+// others mirrored; or (symmetric) x (m x n), whose right operand is read transposed out of LDS.  Both take a sum of two products, so S, V and the pullback's last line are one launch.
+//
+// Numbers.  A singular value grows by up to a per step, so what is rounded in an early step is amplified by up to a^steps (485 with the default coefficients): operands of 8 or
+// 11 bits leave errors of 1e-3 .. 4e-3 relative to the result.  Every operand is therefore a PAIR of f16, x = hi + lo with 22 significant bits, and a product three
+// v_mfma_f32_32x32x16_f16 (hi hi + hi lo + lo hi) with fp32 sums: 1.0 - 1.2x the error of plain fp32 products against 64 bits, at a third of the f16 rate instead of the fp32 MFMA's
+// sixteenth.  The pairs are scaled by powers of two that come from bounds of the iterates' norms (ns_plan), so that no hi overflows and the lo of a typical entry is a normal number.
+// a X is added in fp32 in the epilogue: inside B (B + a I) its rounding would be the largest error of all.  Norms are sums in 64 bits.
+//
+// Layout.  A pair matrix is row-major in blocks of 32 columns, 128 bytes each: 32 hi, then 32 lo -- one cache line holds what an MFMA K-step reads of a row.  Rows are padded to 128,
+// columns of X to 128, with zeros that every step keeps (rows of B beyond m are 0), so the products need no bounds checks.
+#include "md2_internal.h"
+#include "muon.h"
+#include <cmath>
+#include <algorithm>
+#include <vector>
+
+namespace md2 {
+
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+namespace {
+
+constexpr int TILE = 128;                 // rows and columns of a product tile; 4 waves of 64 x 64
+constexpr int PK_ROWS = 64, PK_COLS = 128;   // tile of the norm / pack kernels
+
+// what the host passes per weight (or per batch of equal matrices), by value
+struct Desc {
+    const void* x; const void* d; void* y;                    // matrix | dout | result;  Muon: momentum | gradient | weight
+    int64_t xb, xs, xl, db, ds, dl, yb, ys, yl;               // strides in elements: batch, along the short side, along the long side
+    int64_t ws0, ws1;                                         // first matrix's buffers (bytes into the workspace), bytes per matrix
+    int32_t m, n, batch, first;                               // short side, long side, matrices, index of the first
+    int32_t sym0, nn0, pk0;                                   // first work items
+    float alpha;                                              // Muon: lr * shape factor
+};
+constexpr int DESCS = 16;                 // 16 * 168 bytes of kernel arguments
+struct DescPack { Desc d[DESCS]; };
+
+// the same per matrix, on the device
+struct Mat {
+    const char* x; const char* d; char* y;
+    int64_t xs, xl, ds, dl, ys, yl;
+    char* buf; int64_t xbytes, abytes;                        // pair buffers: nX of mp x np, then nA of mp x mp (4 bytes an entry)
+    int32_t m, n, mp, np, pk0, pkn, nn0, nnn;
+    float alpha;
+};
+struct Item { int32_t mat, ti, tj, pad; };
+
+struct Fac { float inv2; int q; };                             // a clamped matrix is carried 2^q larger (ns_pack_kernel): 2^-2q, q
+struct Ws { Mat* mats; Item *sym, *nn, *pk; Fac* fac; double* part; char* buf; };      // part: [3][pk items] sums of squares of x, of dout, and [nn items] of X0 G
+
+__global__ __launch_bounds__(256) void ns_setup_kernel(DescPack dp, int dt_bytes_x, int dt_bytes_y, Ws ws) {
+    const Desc& D = dp.d[blockIdx.y];
+    const int mt = (D.m + TILE - 1) / TILE, nt = (D.n + TILE - 1) / TILE;
+    const int nsym = mt * (mt + 1) / 2, nnn = mt * nt, npk = mt * (TILE / PK_ROWS) * nt * (TILE / PK_COLS);
+    for (int b = blockIdx.x; b < D.batch; b += gridDim.x) {
+        const int id = D.first + b;
+        if (threadIdx.x == 0) {
+            Mat M;
+            M.x = (const char*)D.x + D.xb * b * dt_bytes_x; M.d = (const char*)D.d + D.db * b * dt_bytes_x; M.y = (char*)D.y + D.yb * b * dt_bytes_y;
+            M.xs = D.xs; M.xl = D.xl; M.ds = D.ds; M.dl = D.dl; M.ys = D.ys; M.yl = D.yl;
+            M.buf = ws.buf + D.ws0 + D.ws1 * b;
+            M.m = D.m; M.n = D.n; M.mp = mt * TILE; M.np = nt * TILE;
+            M.xbytes = (int64_t)M.mp * M.np * 4; M.abytes = (int64_t)M.mp * M.mp * 4;
+            M.pk0 = D.pk0 + npk * b; M.pkn = npk; M.nn0 = D.nn0 + nnn * b; M.nnn = nnn; M.alpha = D.alpha;
+            ws.mats[id] = M;
+        }
+        for (int q = threadIdx.x; q < mt * mt; q += 256) {
+            const int i = q / mt, j = q % mt;
+            if (j >= i) ws.sym[D.sym0 + nsym * b + i * mt - i * (i - 1) / 2 + (j - i)] = Item{id, i, j, 0};
+        }
+        for (int q = threadIdx.x; q < nnn; q += 256) ws.nn[D.nn0 + nnn * b + q] = Item{id, q % mt, q / mt, 0};
+        const int pr = mt * (TILE / PK_ROWS);
+        for (int q = threadIdx.x; q < npk; q += 256) ws.pk[D.pk0 + npk * b + q] = Item{id, q % pr, q / pr, 0};
+    }
+}
+
+// ---- elements ---------------------------------------------------------------------------------------------------------
+template <int DT> __device__ inline float ld_el(const char* p, int64_t i) {
+    if constexpr (DT == NS_F32) return reinterpret_cast<const float*>(p)[i];
+    else if constexpr (DT == NS_F16) return (float)reinterpret_cast<const _Float16*>(p)[i];
+    else return __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(p)[i] << 16);
+}
+template <int DT> __device__ inline void st_el(char* p, int64_t i, float v) {
+    if constexpr (DT == NS_F32) reinterpret_cast<float*>(p)[i] = v;
+    else if constexpr (DT == NS_F16) reinterpret_cast<_Float16*>(p)[i] = (_Float16)v;
+    else { const uint32_t u = __float_as_uint(v); reinterpret_cast<uint16_t*>(p)[i] = v != v ? (uint16_t)((u >> 16) | 0x40) : (uint16_t)((u + 0x7fff + ((u >> 16) & 1)) >> 16); }
+}
+// (v is pinned: left to itself the compiler folds the multiplication that made it into the conversion to hi, but not into the difference, and where v lies next to a tie of f16 the
+// two then disagree about hi by one of its steps)
+__device__ inline void split4(const float v[4], f16x4& hi, f16x4& lo) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { float x = v[e]; asm("" : "+v"(x)); hi[e] = (_Float16)x; lo[e] = (_Float16)(x - (float)hi[e]); }
+}
+__device__ inline int64_t pair_off(int64_t row_bytes, int i, int j) { return i * row_bytes + (j >> 5) * 128 + (j & 31) * 2; }      // bytes of hi(i, j); lo is 64 behind it
+
+// sum over the block in a fixed order (256 threads); every thread gets it
+__device__ inline double block_sum(double v, double* red) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+struct MuonArgs { float beta, gscale; int nesterov; };
+enum { SRC_X = 0, SRC_DOUT = 1, SRC_MUON = 2 };
+
+// One 64 x 128 tile of the source, 8 values of each of the thread's four columns: v[p][e] = element (p * 8 + t / 32, (t % 32) * 4 + e).
+// A source whose short side is the contiguous one goes through LDS, so that either way neighbouring lanes read neighbouring addresses.
+template <int DT, int SRC, bool UPDATE> __device__ inline void load_tile(const Mat& M, const Item& it, const MuonArgs& mu, float v[8][4], float* lds) {
+    const int t = threadIdx.x, i0 = it.ti * PK_ROWS, j0 = it.tj * PK_COLS;
+    const char* src = SRC == SRC_DOUT ? M.d : M.x; const int64_t ss = SRC == SRC_DOUT ? M.ds : M.xs, sl = SRC == SRC_DOUT ? M.dl : M.xl;
+    auto get = [&](int i, int j) -> float {
+        if (i >= M.m || j >= M.n) return 0.f;
+        const int64_t o = i * ss + j * sl;
+        if constexpr (SRC != SRC_MUON) return ld_el<DT>(src, o);
+        else {
+            float* mom = reinterpret_cast<float*>(const_cast<char*>(M.x)); const float g = mu.gscale * reinterpret_cast<const float*>(M.d)[o];
+            float mm = mom[o];
+            if constexpr (UPDATE) { mm = mu.beta * mm + (1.f - mu.beta) * g; mom[o] = mm; }
+            return mu.nesterov ? mu.beta * mm + (1.f - mu.beta) * g : mm;
+        }
+    };
+    if (ss == 1 && sl != 1) {
+        for (int q = 0; q < PK_COLS / 4; ++q) { const int j = q * 4 + (t >> 6), i = t & 63; lds[i * (PK_COLS + 1) + j] = get(i0 + i, j0 + j); }
+        __syncthreads();
+#pragma unroll
+        for (int p = 0; p < 8; ++p)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[p][e] = lds[(p * 8 + (t >> 5)) * (PK_COLS + 1) + (t & 31) * 4 + e];
+        __syncthreads();
+    } else {
+#pragma unroll
+        for (int p = 0; p < 8; ++p)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[p][e] = get(i0 + p * 8 + (t >> 5), j0 + (t & 31) * 4 + e);
+    }
+}
+
+// sum of squares of every tile (Muon: after moving the momentum on)
+template <int DT, int SRC> __global__ __launch_bounds__(256) void ns_norm_kernel(Ws ws, double* part, MuonArgs mu) {
+    __shared__ float lds[PK_ROWS * (PK_COLS + 1)]; __shared__ double red[4];
+    const Item it = ws.pk[blockIdx.x]; const Mat M = ws.mats[it.mat];
+    float v[8][4]; load_tile<DT, SRC, true>(M, it, mu, v, lds);
+    double s = 0;
+#pragma unroll
+    for (int p = 0; p < 8; ++p)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s += (double)v[p][e] * (double)v[p][e];
+    s = block_sum(s, red);
+    if (threadIdx.x == 0) part[blockIdx.x] = s;
+}
+// |.|_F of a matrix from its tiles' sums, in a fixed order
+__device__ inline double norm_of(const Mat& M, const double* part, double* red) {
+    double s = 0;
+    for (int q = threadIdx.x; q < M.pkn; q += 256) s += part[M.pk0 + q];
+    return sqrt(block_sum(s, red));
+}
+// scale * source / max(norm, eps) as pairs.
+// Where the norm r = |X| / eps is clamped, X0 may be too small for f16: it is carried 2^q larger, 2^q r grow <= 4 (grow: by how much all steps can grow a singular value), so A, B, S and V
+// are 2^2q, 2^2q, 2^q and 2^q larger, and what has one factor of A too many (A A, S A, B X, V X) is multiplied by 2^-2q.  q = 0 for every other matrix.
+template <int DT, int SRC> __global__ __launch_bounds__(256) void ns_pack_kernel(Ws ws, const double* part, MuonArgs mu, int x_slot, double scale, double eps, double grow) {
+    __shared__ float lds[PK_ROWS * (PK_COLS + 1)]; __shared__ double red[4];
+    const Item it = ws.pk[blockIdx.x]; const Mat M = ws.mats[it.mat];
+    const double norm = norm_of(M, part, red);
+    if constexpr (SRC != SRC_DOUT) {
+        int q = 0;
+        if (norm <= eps && norm > 0) { const double room = 4.0 * eps / (norm * grow); if (room >= 2.0) q = ilogb(room); }
+        if (it.ti == 0 && it.tj == 0 && threadIdx.x == 0) ws.fac[it.mat] = Fac{(float)ldexp(1.0, -2 * q), q};
+        scale = ldexp(scale, q);
+    }
+    const double fd = norm <= eps ? (eps > 0 ? scale / eps : 0.0) : scale / norm;      // (a NaN norm stays one; eps = 0, dout: 0 for a zero dout)
+    int fe; const float f = (float)frexp(fd, &fe);               // mantissa and exponent apart: 1 / norm may lie outside fp32's range where the product does not
+    float v[8][4]; load_tile<DT, SRC, false>(M, it, mu, v, lds);
+    char* out = M.buf + x_slot * M.xbytes; const int64_t rb = (int64_t)M.np * 4;
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+        float w[4]; f16x4 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = ldexpf(v[p][e], fe) * f;
+        split4(w, hi, lo);
+        char* o = out + pair_off(rb, it.ti * PK_ROWS + p * 8 + (threadIdx.x >> 5), it.tj * PK_COLS + (threadIdx.x & 31) * 4);
+        *reinterpret_cast<f16x4*>(o) = hi; *reinterpret_cast<f16x4*>(o + 64) = lo;
+    }
+}
+
+// ---- products -------------------------------------------------------------------------------------------------------------
+struct Slot { int x, a; };                                                      // buffer = x * xbytes + a * abytes behind the matrix's first
+__device__ inline char* slot(const Mat& M, Slot s) { return M.buf + s.x * M.xbytes + s.a * M.abytes; }
+__device__ inline f32x16 mfma3(f16x8 ah, f16x8 al, f16x8 bh, f16x8 bl, f32x16 c) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl, c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, c, 0, 0, 0);
+}
+// 128 rows x 32 columns of a pair matrix, 16 KB of LDS: row r's eight 16-byte chunks (hi k 0..7, 8..15, 16..23, 24..31, then lo) are stored at chunk ^ (r & 7), so that eight
+// neighbouring rows' reads of one chunk meet eight different bank groups
+__device__ inline void stage_rows(char* lds, const char* src, int64_t rb) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int id = q * 256 + threadIdx.x, r = id >> 3, c = id & 7;
+        *reinterpret_cast<f32x4*>(lds + r * 128 + ((c ^ (r & 7)) << 4)) = *reinterpret_cast<const f32x4*>(src + r * rb + c * 16);
+    }
+}
+__device__ inline f16x8 frag_rows(const char* lds, int r, int c) { return *reinterpret_cast<const f16x8*>(lds + r * 128 + ((c ^ (r & 7)) << 4)); }
+// 32 rows (the K axis) x 128 columns, 16 KB: a row's sixteen 32-byte units are stored at unit ^ (k & 7), so that the four rows of a transposed read meet different banks
+__device__ inline void stage_cols(char* lds, const char* src, int64_t rb) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int id = q * 256 + threadIdx.x, k = id >> 5, c = id & 31;
+        *reinterpret_cast<f32x4*>(lds + k * 512 + (((c >> 1) ^ (k & 7)) << 5) + (c & 1) * 16) = *reinterpret_cast<const f32x4*>(src + k * rb + c * 16);
+    }
+}
+// The MFMA operand of 32 columns from c0 and 16 rows from k0 (lane: column lane % 32, rows (lane / 32) * 8 .. + 8).  ds_read_b64_tr_b16: within 16 lanes, lane s gives the
+// address of 4 columns of row s / 4 and receives the four rows of column s; so two reads of 4 rows make the operand.
+__device__ inline f16x8 frag_cols(const char* lds, int k0, int c0, int lo) {
+    const int l = threadIdx.x & 63, s = l & 15, g = l >> 4;
+    const int col = c0 + (g & 1) * 16 + (s & 3) * 4, unit = (col >> 5) * 4 + lo * 2 + ((col >> 4) & 1);
+    f16x8 r;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int k = k0 + (g >> 1) * 8 + h * 4 + (s >> 2);
+        const char* p = lds + k * 512 + ((unit ^ (k & 7)) << 5) + (col & 15) * 2;
+        const s16x4 q = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[h * 4 + e] = __builtin_bit_cast(_Float16, (short)q[e]);
+    }
+    return r;
+}
+
+struct SymArgs { Slot l[2], r[2], e, out; int nseg, k_is_n, have_e; float acc, ecoef; };      // out = acc * (sum of l r^T) + ecoef * e, in the buffers' own scales (with e: a factor A too many)
+// A tile on or above the diagonal of a symmetric result, and its mirror image
+__global__ __launch_bounds__(256, 2) void ns_sym_kernel(Ws ws, SymArgs a) {
+    __shared__ __attribute__((aligned(16))) char lds[2 * 16384];
+    const Item it = ws.sym[blockIdx.x]; const Mat M = ws.mats[it.mat];
+    const int t = threadIdx.x, lane = t & 63, wv = t >> 6, wi = (wv >> 1) * 64, wj = (wv & 1) * 64, lr = lane & 31, lk = lane >> 5;
+    const int64_t rb = (int64_t)(a.k_is_n ? M.np : M.mp) * 4; const int kb = ((a.k_is_n ? M.n : M.m) + 31) / 32;
+    f32x16 c[2][2] = {};
+    for (int sg = 0; sg < a.nseg; ++sg) {
+        const char* L = slot(M, a.l[sg]) + (int64_t)it.ti * TILE * rb; const char* R = slot(M, a.r[sg]) + (int64_t)it.tj * TILE * rb;
+        for (int k = 0; k < kb; ++k) {
+            __syncthreads();
+            stage_rows(lds, L + k * 128, rb); stage_rows(lds + 16384, R + k * 128, rb);
+            __syncthreads();
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                f16x8 ah[2], al[2], bh[2], bl[2];
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    ah[q] = frag_rows(lds, wi + q * 32 + lr, s * 2 + lk); al[q] = frag_rows(lds, wi + q * 32 + lr, s * 2 + lk + 4);
+                    bh[q] = frag_rows(lds + 16384, wj + q * 32 + lr, s * 2 + lk); bl[q] = frag_rows(lds + 16384, wj + q * 32 + lr, s * 2 + lk + 4);
+                }
+#pragma unroll
+                for (int p = 0; p < 2; ++p)
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) c[p][q] = mfma3(ah[p], al[p], bh[q], bl[q], c[p][q]);
+            }
+        }
+    }
+    // lane: column j, registers: rows i .. i + 3
+    const int64_t arb = (int64_t)M.mp * 4; char* out = slot(M, a.out); const char* E = slot(M, a.e); const float facc = a.have_e ? a.acc * ws.fac[it.mat].inv2 : a.acc;
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int i = it.ti * TILE + wi + p * 32 + g * 8 + lk * 4, j = it.tj * TILE + wj + q * 32 + lr;
+                const int64_t o = pair_off(arb, j, i);
+                float v[4]; f16x4 hi, lo;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = facc * c[p][q][g * 4 + e];
+                if (a.have_e) {
+                    const f16x4 eh = *reinterpret_cast<const f16x4*>(E + o), el = *reinterpret_cast<const f16x4*>(E + o + 64);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] += a.ecoef * ((float)eh[e] + (float)el[e]);
+                }
+                split4(v, hi, lo);
+                *reinterpret_cast<f16x4*>(out + o) = hi; *reinterpret_cast<f16x4*>(out + o + 64) = lo;
+                if (it.ti != it.tj)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) { char* w = out + pair_off(arb, i + e, j); *reinterpret_cast<_Float16*>(w) = hi[e]; *reinterpret_cast<_Float16*>(w + 64) = lo[e]; }
+            }
+}
+
+enum { OUT_PAIR = 0, OUT_Y = 1, OUT_MUON = 2, OUT_BACK = 3 };
+struct NnArgs { Slot l[2], r[2], e, out, x0; int nseg; float acc, ecoef, mid, decay; };      // value = acc * (mid * l0 r0 + l1 r1) + ecoef * e; one product: acc * l0 r0 + ecoef * e
+// A tile of (symmetric m x m) x (m x n)
+template <int DT, int OUT> __global__ __launch_bounds__(256, 2) void ns_nn_kernel(Ws ws, NnArgs a, double* dots) {
+    __shared__ __attribute__((aligned(16))) char lds[2 * 16384]; __shared__ double red[4];
+    const Item it = ws.nn[blockIdx.x]; const Mat M = ws.mats[it.mat];
+    const int t = threadIdx.x, lane = t & 63, wv = t >> 6, wi = (wv >> 1) * 64, wj = (wv & 1) * 64, lr = lane & 31, lk = lane >> 5;
+    const int64_t arb = (int64_t)M.mp * 4, xrb = (int64_t)M.np * 4; const int kb = (M.m + 31) / 32;
+    f32x16 c[2][2] = {};                                           // [j][i]: lane = row i, registers = four neighbouring columns j
+    for (int sg = 0; sg < a.nseg; ++sg) {
+        if (sg)                                                    // the second product's scale is another power of two
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+#pragma unroll
+                for (int q = 0; q < 2; ++q) c[p][q] *= a.mid;
+        const char* L = slot(M, a.l[sg]) + (int64_t)it.ti * TILE * arb; const char* R = slot(M, a.r[sg]) + (int64_t)it.tj * TILE * 4;
+        for (int k = 0; k < kb; ++k) {
+            __syncthreads();
+            stage_rows(lds, L + k * 128, arb); stage_cols(lds + 16384, R + (int64_t)k * 32 * xrb, xrb);
+            __syncthreads();
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                f16x8 ah[2], al[2], bh[2], bl[2];
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    ah[q] = frag_cols(lds + 16384, s * 16, wj + q * 32, 0); al[q] = frag_cols(lds + 16384, s * 16, wj + q * 32, 1);
+                    bh[q] = frag_rows(lds, wi + q * 32 + lr, s * 2 + lk); bl[q] = frag_rows(lds, wi + q * 32 + lr, s * 2 + lk + 4);
+                }
+#pragma unroll
+                for (int p = 0; p < 2; ++p)
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) c[p][q] = mfma3(ah[p], al[p], bh[q], bl[q], c[p][q]);
+            }
+        }
+    }
+    const char* E = slot(M, a.e); double dot = 0; const Fac fac = ws.fac[it.mat]; const float facc = a.acc * fac.inv2;
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int i = it.ti * TILE + wi + q * 32 + lr, j = it.tj * TILE + wj + p * 32 + g * 8 + lk * 4;
+                const int64_t o = pair_off(xrb, i, j);
+                const f16x4 eh = *reinterpret_cast<const f16x4*>(E + o), el = *reinterpret_cast<const f16x4*>(E + o + 64);
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = facc * c[p][q][g * 4 + e] + a.ecoef * ((float)eh[e] + (float)el[e]);
+                if constexpr (OUT == OUT_PAIR) {
+                    f16x4 hi, lo; split4(v, hi, lo);
+                    char* w = slot(M, a.out) + o;
+                    *reinterpret_cast<f16x4*>(w) = hi; *reinterpret_cast<f16x4*>(w + 64) = lo;
+                } else if constexpr (OUT == OUT_BACK) {              // G in fp32, and this tile's share of <X0, G>
+                    const char* X0 = slot(M, a.x0) + o; const f16x4 xh = *reinterpret_cast<const f16x4*>(X0), xl = *reinterpret_cast<const f16x4*>(X0 + 64);
+                    f32x4 w;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) { w[e] = v[e]; dot += (double)((float)xh[e] + (float)xl[e]) * (double)v[e]; }
+                    *reinterpret_cast<f32x4*>(slot(M, a.out) + i * xrb + (int64_t)j * 4) = w;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = ldexpf(v[e], -fac.q);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (i < M.m && j + e < M.n) {
+                            const int64_t yo = i * M.ys + (j + e) * M.yl;
+                            if constexpr (OUT == OUT_Y) st_el<DT>(M.y, yo, v[e]);
+                            else { float* P = reinterpret_cast<float*>(M.y) + yo; *P = a.decay * *P - M.alpha * v[e]; }
+                        }
+                }
+            }
+    if constexpr (OUT == OUT_BACK) {
+        dot = block_sum(dot, red);
+        if (t == 0) dots[blockIdx.x] = dot;
+    }
+}
+
+// dX = (G - X0 <X0, G>) / |X|_F, or G / eps where the norm was clamped; G carries gscale / |dout|_F
+template <int DT> __global__ __launch_bounds__(256) void ns_back_finish_kernel(Ws ws, const double* xpart, const double* dpart, const double* dots, Slot g, Slot x0, double gscale, double xscale, double eps) {
+    __shared__ float lds[PK_ROWS * (PK_COLS + 1)]; __shared__ double red[4];
+    const Item it = ws.pk[blockIdx.x]; const Mat M = ws.mats[it.mat];
+    const double norm = norm_of(M, xpart, red), dnorm = norm_of(M, dpart, red);
+    double along = 0;
+    for (int q = threadIdx.x; q < M.nnn; q += 256) along += dots[M.nn0 + q];
+    along = block_sum(along, red) / xscale;
+    const bool clamped = norm <= eps;
+    const float fg = (float)(dnorm / gscale / (clamped ? eps : norm)), fx = clamped ? 0.f : (float)(along * (dnorm / gscale) / norm / xscale);
+    const int64_t xrb = (int64_t)M.np * 4; const int t = threadIdx.x; const bool turn = M.ys == 1 && M.yl != 1;
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+        const int li = p * 8 + (t >> 5), lj = (t & 31) * 4, i = it.ti * PK_ROWS + li, j = it.tj * PK_COLS + lj;
+        const f32x4 G = *reinterpret_cast<const f32x4*>(slot(M, g) + i * xrb + (int64_t)j * 4);
+        const char* X0 = slot(M, x0) + pair_off(xrb, i, j); const f16x4 xh = *reinterpret_cast<const f16x4*>(X0), xl = *reinterpret_cast<const f16x4*>(X0 + 64);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float v = clamped ? G[e] * fg : G[e] * fg - ((float)xh[e] + (float)xl[e]) * fx;
+            if (turn) lds[li * (PK_COLS + 1) + lj + e] = v;
+            else if (i < M.m && j + e < M.n) st_el<DT>(M.y, i * M.ys + (j + e) * M.yl, v);
+        }
+    }
+    if (turn) {
+        __syncthreads();
+        for (int q = 0; q < PK_COLS / 4; ++q) {
+            const int j = it.tj * PK_COLS + q * 4 + (t >> 6), i = it.ti * PK_ROWS + (t & 63);
+            if (i < M.m && j < M.n) st_el<DT>(M.y, i * M.ys + j * M.yl, lds[(t & 63) * (PK_COLS + 1) + q * 4 + (t >> 6)]);
+        }
+    }
+}
+
+// ---- host -------------------------------------------------------------------------------------------------------------------
+// Bounds of what the iteration can meet, from the scalar polynomial on [0, s]: the iterates' singular values, B's, and by how much a step of the pullback can grow G
+struct Plan { bool ok = false; const char* why = ""; double grow = 1, growth[MD2_NS_MAX_STEPS + 1] = {}, s[MD2_NS_MAX_STEPS + 1] = {}, vgain[MD2_NS_MAX_STEPS] = {}; };
+Plan ns_bounds(int steps, const double* co, bool back) {
+    Plan P;
+    if (steps < 1 || steps > MD2_NS_MAX_STEPS) { P.why = "steps must be in 1..16"; return P; }
+    const double a = co[0], b = co[1], c = co[2];
+    if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) { P.why = "the coefficients must be finite"; return P; }
+    double lip[MD2_NS_MAX_STEPS]; P.s[0] = 1.0;
+    for (int k = 0; k < steps; ++k) {
+        double top = 0, bm = 0, L = 0, up = 0; const int N = 4096;
+        for (int i = 0; i <= N; ++i) {
+            const double s = P.s[k] * i / N, s2 = s * s, q = b * s2 + c * s2 * s2;
+            top = std::max(top, std::fabs(s * (a + q))); up = std::max(up, std::fabs(a + q)); bm = std::max(bm, std::fabs(q));
+            L = std::max(L, std::max(std::fabs(a + q), std::fabs(a + 3 * b * s2 + 5 * c * s2 * s2)));
+        }
+        P.s[k + 1] = top * 1.01; lip[k] = L * 1.01; P.vgain[k] = std::fabs(b) + 2 * std::fabs(c) * P.s[k] * P.s[k];
+        if (!(P.s[k + 1] <= 4.0) || !(bm <= 60.0)) { P.why = "these coefficients let a singular value grow past 4 (or b s^2 + c s^4 past 60)"; return P; }
+        P.grow *= std::max(up, 1.0) * 1.01;
+    }
+    P.growth[steps] = 1.0;
+    for (int k = steps - 1; k >= 0; --k) P.growth[k] = P.growth[k + 1] * std::max(lip[k], 1.0);
+    if (back && !(P.growth[0] <= 8192.0)) { P.why = "the pullback of this many steps can grow a gradient past 8192 times its norm"; return P; }
+    P.ok = true; return P;
+}
+double pow2_below(double v) { return std::exp2(std::floor(std::log2(v))); }
+constexpr double SX = 8192.0, SA = 2048.0, SB = 512.0;            // scales of X (norm <= 4), A (<= 16) and B (<= 60): below 2^15, and f16 ends at 65504
+
+int64_t up(int64_t v, int64_t q) { return (v + q - 1) / q * q; }
+struct Layout { int64_t mats, sym, nn, pk, fac, part, buf, total; int64_t n_mats, n_sym, n_nn, n_pk; };
+
+}  // namespace
+
+struct NsProblem { std::vector<Desc> d; int nX, nA; };
+
+static Layout ns_layout(NsProblem& p) {
+    Layout L{};
+    int64_t buf = 0;
+    for (Desc& d : p.d) {
+        const int64_t mt = (d.m + TILE - 1) / TILE, nt = (d.n + TILE - 1) / TILE;
+        d.first = (int)L.n_mats; d.sym0 = (int)L.n_sym; d.nn0 = (int)L.n_nn; d.pk0 = (int)L.n_pk;
+        d.ws0 = buf; d.ws1 = (p.nX * mt * nt + p.nA * mt * mt) * (int64_t)TILE * TILE * 4;
+        L.n_mats += d.batch; L.n_sym += mt * (mt + 1) / 2 * d.batch; L.n_nn += mt * nt * d.batch; L.n_pk += mt * (TILE / PK_ROWS) * nt * (TILE / PK_COLS) * d.batch;
+        buf += d.ws1 * d.batch;
+    }
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) { const int64_t r = at; at = up(at + bytes, 256); return r; };
+    L.mats = take(L.n_mats * sizeof(Mat)); L.sym = take(L.n_sym * sizeof(Item)); L.nn = take(L.n_nn * sizeof(Item)); L.pk = take(L.n_pk * sizeof(Item)); L.fac = take(L.n_mats * sizeof(Fac));
+    L.part = take((2 * L.n_pk + L.n_nn) * sizeof(double)); L.buf = take(buf); L.total = at;
+    return L;
+}
+static bool fits(int64_t batch, int64_t rows, int64_t cols) {      // sizes whose work items and element counts stay far inside 31 bits
+    return rows > 0 && cols > 0 && batch > 0 && rows <= (1 << 20) && cols <= (1 << 20) && rows * cols <= (1ll << 31) && batch <= (1 << 20);
+}
+static int64_t check_total(const Layout& L) { return (L.n_sym < (1ll << 30) && L.n_nn < (1ll << 30) && L.n_pk < (1ll << 30) && L.n_mats < (1ll << 24)) ? L.total : -1; }
+
+static Desc make_desc(const NsMatrices& q) {
+    Desc d{}; const bool tall = q.rows > q.cols;
+    d.x = q.x; d.d = q.d; d.y = q.y; d.m = (int)std::min(q.rows, q.cols); d.n = (int)std::max(q.rows, q.cols); d.batch = (int)q.batch;
+    d.xb = q.xs[0]; d.xs = q.xs[tall ? 2 : 1]; d.xl = q.xs[tall ? 1 : 2];
+    d.db = q.ds[0]; d.ds = q.ds[tall ? 2 : 1]; d.dl = q.ds[tall ? 1 : 2];
+    d.yb = q.rows * q.cols; d.ys = tall ? 1 : q.cols; d.yl = tall ? q.cols : 1;
+    d.alpha = q.alpha;
+    return d;
+}
+static void slots_of(int kind, int steps, int& nX, int& nA) {
+    if (kind == NS_BACKWARD) { nX = steps + 2; nA = 2 * steps + 2; }      // every iterate and two G | every A, every B, S, V
+    else { nX = 2; nA = 2; }                                             // X twice | A, B
+}
+int64_t ns_workspace(int kind, int steps, const NsMatrices* q, int count) {
+    if (steps < 1 || steps > MD2_NS_MAX_STEPS) return -1;
+    NsProblem p; slots_of(kind, steps, p.nX, p.nA);
+    for (int i = 0; i < count; ++i) { if (!fits(q[i].batch, q[i].rows, q[i].cols)) return -1; p.d.push_back(make_desc(q[i])); }
+    return check_total(ns_layout(p));
+}
+
+template <int DT> static void ns_launch(int kind, NsProblem& p, const Layout& L, char* base, const NsOptions& o, const Plan& P, hipStream_t s) {
+    Ws ws; ws.mats = (Mat*)(base + L.mats); ws.sym = (Item*)(base + L.sym); ws.nn = (Item*)(base + L.nn); ws.pk = (Item*)(base + L.pk); ws.fac = (Fac*)(base + L.fac); ws.part = (double*)(base + L.part); ws.buf = base + L.buf;
+    const int bytes = DT == NS_F32 ? 4 : 2, steps = o.steps;
+    for (size_t i = 0; i < p.d.size(); i += DESCS) {
+        DescPack dp; const int n = (int)std::min<size_t>(DESCS, p.d.size() - i); int most = 1;
+        for (int k = 0; k < n; ++k) { dp.d[k] = p.d[i + k]; most = std::max(most, dp.d[k].batch); }
+        hipLaunchKernelGGL(ns_setup_kernel, dim3(std::min(most, 256), n), dim3(256), 0, s, dp, bytes, bytes, ws);
+    }
+    const dim3 blk(256), pk((unsigned)L.n_pk), sym((unsigned)L.n_sym), nn((unsigned)L.n_nn);
+    const MuonArgs mu{(float)o.momentum, o.grad_scale, o.nesterov};
+    double *xpart = ws.part, *dpart = ws.part + L.n_pk, *dots = ws.part + 2 * L.n_pk;
+    if (kind == NS_MUON) {
+        hipLaunchKernelGGL((ns_norm_kernel<NS_F32, SRC_MUON>), pk, blk, 0, s, ws, xpart, mu);
+        hipLaunchKernelGGL((ns_pack_kernel<NS_F32, SRC_MUON>), pk, blk, 0, s, ws, xpart, mu, 0, SX, o.eps, P.grow);
+    } else {
+        hipLaunchKernelGGL((ns_norm_kernel<DT, SRC_X>), pk, blk, 0, s, ws, xpart, mu);
+        hipLaunchKernelGGL((ns_pack_kernel<DT, SRC_X>), pk, blk, 0, s, ws, xpart, mu, 0, SX, o.eps, P.grow);
+    }
+    const double a = o.coef[0], b = o.coef[1], c = o.coef[2];
+    const bool back = kind == NS_BACKWARD;
+    const int nX = p.nX;
+    auto X = [&](int k) { return Slot{back ? k : (k & 1), 0}; };
+    auto A = [&](int k) { return Slot{nX, back ? 2 * k : 0}; };
+    auto B = [&](int k) { return Slot{nX, back ? 2 * k + 1 : 1}; };
+    for (int k = 0; k < steps; ++k) {
+        SymArgs g{}; g.l[0] = g.r[0] = X(k); g.e = g.out = A(k); g.nseg = 1; g.k_is_n = 1; g.acc = (float)(SA / (SX * SX));
+        hipLaunchKernelGGL(ns_sym_kernel, sym, blk, 0, s, ws, g);
+        SymArgs q{}; q.l[0] = q.r[0] = q.e = A(k); q.out = B(k); q.nseg = 1; q.have_e = 1; q.acc = (float)(c * SB / (SA * SA)); q.ecoef = (float)(b * SB / SA);
+        hipLaunchKernelGGL(ns_sym_kernel, sym, blk, 0, s, ws, q);
+        if (back && k == steps - 1) break;
+        NnArgs f{}; f.l[0] = B(k); f.r[0] = f.e = X(k); f.out = X(k + 1); f.nseg = 1;
+        if (k < steps - 1) { f.acc = (float)(1.0 / SB); f.ecoef = (float)a; hipLaunchKernelGGL((ns_nn_kernel<NS_F32, OUT_PAIR>), nn, blk, 0, s, ws, f, dots); }
+        else {
+            f.acc = (float)(1.0 / (SB * SX)); f.ecoef = (float)(a / SX); f.decay = (float)(1.0 - o.lr * o.weight_decay);
+            if (kind == NS_MUON) hipLaunchKernelGGL((ns_nn_kernel<NS_F32, OUT_MUON>), nn, blk, 0, s, ws, f, dots);
+            else hipLaunchKernelGGL((ns_nn_kernel<DT, OUT_Y>), nn, blk, 0, s, ws, f, dots);
+        }
+    }
+    if (!back) return;
+    hipLaunchKernelGGL((ns_norm_kernel<DT, SRC_DOUT>), pk, blk, 0, s, ws, dpart, mu);
+    auto sg = [&](int k) { return pow2_below(16384.0 / P.growth[k]); };                 // scale of dL/dX_k (of dout / |dout|: at most growth[k])
+    const Slot G[2] = {Slot{steps, 0}, Slot{steps + 1, 0}}; const Slot S{nX, 2 * steps}, V{nX, 2 * steps + 1};
+    int cur = 0;
+    hipLaunchKernelGGL((ns_pack_kernel<DT, SRC_DOUT>), pk, blk, 0, s, ws, dpart, mu, G[cur].x, sg(steps), 0.0, 1.0);
+    for (int k = steps - 1; k >= 0; --k, cur ^= 1) {
+        const double gin = sg(k + 1), gout = sg(k), sbound = 2 * P.growth[k + 1] * P.s[k];
+        const double ss = pow2_below(16384.0 / sbound), sv = pow2_below(16384.0 / (sbound * P.vgain[k]));
+        SymArgs q{}; q.l[0] = G[cur]; q.r[0] = X(k); q.l[1] = X(k); q.r[1] = G[cur]; q.e = q.out = S; q.nseg = 2; q.k_is_n = 1; q.acc = (float)(ss / (gin * SX));
+        hipLaunchKernelGGL(ns_sym_kernel, sym, blk, 0, s, ws, q);
+        SymArgs v{}; v.l[0] = S; v.r[0] = A(k); v.l[1] = A(k); v.r[1] = S; v.e = S; v.out = V; v.nseg = 2; v.have_e = 1; v.acc = (float)(c * sv / (ss * SA)); v.ecoef = (float)(b * sv / ss);
+        hipLaunchKernelGGL(ns_sym_kernel, sym, blk, 0, s, ws, v);
+        NnArgs f{}; f.l[0] = B(k); f.r[0] = f.e = G[cur]; f.l[1] = V; f.r[1] = X(k); f.out = G[cur ^ 1]; f.x0 = X(0); f.nseg = 2;
+        f.mid = (float)(sv * SX / (SB * gin)); f.acc = (float)(gout / (sv * SX)); f.ecoef = (float)(a * gout / gin);
+        if (k > 0) hipLaunchKernelGGL((ns_nn_kernel<NS_F32, OUT_PAIR>), nn, blk, 0, s, ws, f, dots);
+        else hipLaunchKernelGGL((ns_nn_kernel<NS_F32, OUT_BACK>), nn, blk, 0, s, ws, f, dots);
+    }
+    hipLaunchKernelGGL((ns_back_finish_kernel<DT>), pk, blk, 0, s, ws, xpart, dpart, dots, G[cur], X(0), sg(0), SX, o.eps);
+}
+
+int ns_run(int kind, int dtype, const NsMatrices* q, int count, const NsOptions& o, void* wsp, int64_t ws_bytes, hipStream_t s, const char** why) {
+    if (!(o.eps > 0) || !std::isfinite(o.eps)) { *why = "eps must be positive"; return 2; }
+    const Plan P = ns_bounds(o.steps, o.coef, kind == NS_BACKWARD);
+    if (!P.ok) { *why = P.why; return 2; }
+    const int el = dtype == NS_F32 ? 4 : 2;
+    NsProblem p; slots_of(kind, o.steps, p.nX, p.nA);
+    for (int i = 0; i < count; ++i) {
+        const NsMatrices& m = q[i];
+        if (!m.x || !m.y || (kind != NS_FORWARD && !m.d)) { *why = "null pointer"; return 2; }
+        if (!fits(m.batch, m.rows, m.cols)) { *why = "sizes must be positive, a side at most 2^20, a matrix at most 2^31 elements, a batch at most 2^20"; return 2; }
+        if (((uintptr_t)m.x | (uintptr_t)m.d | (uintptr_t)m.y) % el) { *why = "a pointer is not aligned to its elements"; return 2; }
+        for (int k = 0; k < 3; ++k) if (m.xs[k] < 0 || m.ds[k] < 0) { *why = "negative stride"; return 2; }
+        p.d.push_back(make_desc(m));
+    }
+    const Layout L = ns_layout(p);
+    if (check_total(L) < 0) { *why = "too many matrices"; return 2; }
+    if (!wsp || (uintptr_t)wsp % 256 || ws_bytes < L.total) { *why = "the workspace is missing, too small or not aligned to 256 bytes"; return 2; }
+    if (dtype == NS_F32) ns_launch<NS_F32>(kind, p, L, (char*)wsp, o, P, s);
+    else if (dtype == NS_BF16) ns_launch<NS_BF16>(kind, p, L, (char*)wsp, o, P, s);
+    else ns_launch<NS_F16>(kind, p, L, (char*)wsp, o, P, s);
+    return 0;
+}
+
+}  // namespace md2

@@ -436,4 +436,26 @@ function ∇maxpool3s2(x::ROCArray{Float32,4}, Δ)
 end
 adam_raw!(p, g, m, v, step; lr=1e-4, grad_scale=1f0) = ok(md2_adam_raw(dptr(p), dptr(g), dptr(m), dptr(v), length(p), Int32(step), Float64(lr), Float32(grad_scale), NOSTREAM), "adam_raw")
 
+# Muon: a Julia matrix (cols, rows) is the library's row-major rows x cols; orthogonalisation does not depend on which side is called rows
+const NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+ns_dtype(::Type{Float32}) = Int32(0); ns_dtype(::Type{Float16}) = Int32(2)
+ns_strides(x) = Int64[size(x, 1) * size(x, 2), size(x, 1), 1]
+function newton_schulz(x::ROCArray{T,3}; steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7) where {T}
+    K, R, B = size(x); y = similar(x); n = md2_newton_schulz_workspace(Int64(B), Int64(R), Int64(K), Int32(steps), Int32(0)); ws = ROCArray{UInt8}(undef, max(n, 0)); co = collect(Float64, coefficients); st = ns_strides(x)
+    GC.@preserve co st ok(md2_newton_schulz(dptr(x), dptr(y), Int64(B), Int64(R), Int64(K), pointer(st), ns_dtype(T), Int32(steps), pointer(co), Float64(eps), dptr(ws), n, NOSTREAM), "newton_schulz"); y
+end
+function ∇newton_schulz(x::ROCArray{T,3}, Δ; steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7) where {T}
+    K, R, B = size(x); dx = similar(x); n = md2_newton_schulz_workspace(Int64(B), Int64(R), Int64(K), Int32(steps), Int32(1)); ws = ROCArray{UInt8}(undef, max(n, 0)); co = collect(Float64, coefficients); st = ns_strides(x)
+    GC.@preserve co st ok(md2_newton_schulz_bwd(dptr(x), dptr(Δ), dptr(dx), Int64(B), Int64(R), Int64(K), pointer(st), pointer(st), ns_dtype(T), Int32(steps), pointer(co), Float64(eps), dptr(ws), n, NOSTREAM), "newton_schulz_bwd"); dx
+end
+# ps, gs, ms: vectors of Float32 arrays whose LAST dimension is the output channels (Flux conv weights (kW,kH,Cin,Cout): rows = Cout)
+function muon_raw!(ps, gs, ms; lr=0.02, momentum=0.95, nesterov=true, weight_decay=0.0, adjust=:spectral, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, grad_scale=1f0)
+    rows = Int64[size(p, ndims(p)) for p in ps]; cols = Int64[length(p) ÷ size(p, ndims(p)) for p in ps]; co = collect(Float64, coefficients); P = dptr.(ps); G = dptr.(gs); M = dptr.(ms)
+    GC.@preserve rows cols co P G M begin
+        n = md2_muon_workspace(pointer(rows), pointer(cols), Int32(length(ps)), Int32(steps)); ws = ROCArray{UInt8}(undef, max(n, 0))
+        ok(md2_muon_raw(pointer(P), pointer(G), pointer(M), pointer(rows), pointer(cols), Int32(length(ps)), Float64(lr), Float64(momentum), Int32(nesterov), Float64(weight_decay), Int32(adjust === :rms),
+                        Float32(grad_scale), Int32(steps), pointer(co), Float64(eps), dptr(ws), n, NOSTREAM), "muon_raw")
+    end
+end
+
 end # module

@@ -778,6 +778,89 @@ def adam_raw(p, g, m, v, step, lr=1e-4, grad_scale=1.0):
     _check(_lib.lib().md2_adam_raw(_dev(p), _dev(g), _dev(m), _dev(v), p.numel(), int(step), float(lr), float(grad_scale), _stream()), None, "adam_raw")
 
 
+# -- Muon: updates orthogonalised by Newton-Schulz products, beside ADAM ---------------------------------------------------
+NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+_NS_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_MUON_ADJUST = {"spectral": 0, "rms": 1}
+
+
+def _ns_matrices(x, what):
+    """-> (x as (batch, rows, cols), a view where its strides allow one, dtype code)."""
+    if not (torch.is_tensor(x) and x.is_cuda and x.dtype in _NS_DTYPES and x.dim() >= 2):
+        raise ValueError("%s: expected a CUDA tensor (..., rows, cols) of float32, bfloat16 or float16 (the product path has no CPU fallback)" % what)
+    return x.detach().reshape((int(np.prod(x.shape[:-2], dtype=np.int64)),) + tuple(x.shape[-2:])), _NS_DTYPES[x.dtype]
+
+
+def _ns_workspace(nbytes, device, what):
+    if nbytes < 0:
+        raise ValueError("%s: sizes or steps out of range (a side at most 2^20, a matrix at most 2^31 elements, steps in 1..16)" % what)
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def _ns_args(steps, coefficients, eps):
+    co = tuple(float(c) for c in coefficients)
+    if len(co) != 3:
+        raise ValueError("coefficients: expected (a, b, c)")
+    return int(steps), (C.c_double * 3)(*co), float(eps)
+
+
+def newton_schulz(x, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7):
+    """The nearly orthogonal matrix with x's singular vectors: X0 = x / max(|x|_F, eps), then `steps` times X <- a X + (b X X^T + c (X X^T)^2) X, on the shorter side.  x (..., rows, cols),
+    float32 / bfloat16 / float16, any strides; a convolution is `w.flatten(1)`.  Products in fp32 accuracy.  -> contiguous, like x."""
+    x3, dt = _ns_matrices(x, "newton_schulz"); st, co, ep = _ns_args(steps, coefficients, eps); y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if y.numel() == 0:
+        return y
+    B, R, K = x3.shape; L = _lib.lib()
+    with torch.cuda.device(x.device):
+        ws = _ns_workspace(L.md2_newton_schulz_workspace(B, R, K, st, 0), x.device, "newton_schulz")
+        _check(L.md2_newton_schulz(x3.data_ptr(), y.data_ptr(), B, R, K, (C.c_int64 * 3)(*x3.stride()), dt, st, co, ep, ws.data_ptr(), ws.numel(), _stream()), None, "newton_schulz")
+    return y
+
+
+def newton_schulz_pullback(x, dout, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7):
+    """Pullback of newton_schulz: dout like its result -> dx, through every step and the normalisation."""
+    x3, dt = _ns_matrices(x, "newton_schulz_pullback"); d3, dd = _ns_matrices(dout, "newton_schulz_pullback"); st, co, ep = _ns_args(steps, coefficients, eps)
+    if dout.shape != x.shape or dd != dt or dout.device != x.device:
+        raise ValueError("newton_schulz_pullback: dout must have x's shape, type and device")
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if dx.numel() == 0:
+        return dx
+    B, R, K = x3.shape; L = _lib.lib()
+    with torch.cuda.device(x.device):
+        ws = _ns_workspace(L.md2_newton_schulz_workspace(B, R, K, st, 1), x.device, "newton_schulz_pullback")
+        _check(L.md2_newton_schulz_bwd(x3.data_ptr(), d3.data_ptr(), dx.data_ptr(), B, R, K, (C.c_int64 * 3)(*x3.stride()), (C.c_int64 * 3)(*d3.stride()), dt, st, co, ep, ws.data_ptr(), ws.numel(),
+                                       _stream()), None, "newton_schulz_bwd")
+    return dx
+
+
+def muon_raw(params, grads, momenta, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, adjust="spectral", steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, grad_scale=1.0):
+    """One Muon step of a list of weights at once (in place, like adam_raw): m <- momentum m + (1 - momentum) g with g scaled by grad_scale first, u = momentum m + (1 - momentum) g
+    (nesterov) or m, p <- (1 - lr weight_decay) p - lr s newton_schulz(u).  s = sqrt(max(1, rows / cols)) for adjust="spectral", 0.2 sqrt(max(rows, cols)) for "rms" (an ADAM step's
+    size).  Weights are contiguous float32 tensors of two or more dimensions, one matrix each: shape[0] rows (a convolution's output channels).  No tensor may appear twice."""
+    params, grads, momenta = list(params), list(grads), list(momenta); n = len(params)
+    if len(grads) != n or len(momenta) != n:
+        raise ValueError("muon_raw: params, grads and momenta must be lists of one length")
+    if adjust not in _MUON_ADJUST:
+        raise ValueError("muon_raw: adjust must be 'spectral' or 'rms'")
+    st, co, ep = _ns_args(steps, coefficients, eps); keep = []
+    for p, g, m in zip(params, grads, momenta):
+        for t in (p, g, m):
+            _dev(t)
+        if p.dim() < 2 or g.shape != p.shape or m.shape != p.shape:
+            raise ValueError("muon_raw: a weight needs two or more dimensions, and a gradient and a momentum of its shape (got %s, %s, %s)" % (tuple(p.shape), tuple(g.shape), tuple(m.shape)))
+        if not (p.device == g.device == m.device == params[0].device):
+            raise ValueError("muon_raw: every tensor must be on one device")
+        if p.numel():
+            keep.append((p.data_ptr(), g.data_ptr(), m.data_ptr(), p.shape[0], p.numel() // p.shape[0]))
+    if not keep:
+        return
+    n = len(keep); P, G, M, R, K = zip(*keep); R, K = (C.c_int64 * n)(*R), (C.c_int64 * n)(*K); L = _lib.lib(); dev = params[0].device
+    with torch.cuda.device(dev):
+        ws = _ns_workspace(L.md2_muon_workspace(R, K, n, st), dev, "muon_raw")
+        _check(L.md2_muon_raw((C.c_void_p * n)(*P), (C.c_void_p * n)(*G), (C.c_void_p * n)(*M), R, K, n, float(lr), float(momentum), int(bool(nesterov)), float(weight_decay),
+                              _MUON_ADJUST[adjust], float(grad_scale), st, co, ep, ws.data_ptr(), ws.numel(), _stream()), None, "muon_raw")
+
+
 def conv2d_bnstats(x, w, stride=1, pad=0):
     """Encoder conv (no bias) + the training-BatchNorm statistics its epilogue accumulates: -> (y, mean[Cout], invstd[Cout])."""
     x, w = _f32(x), _f32(w); N, Cin, H, W = x.shape; Cout, _, k, _ = w.shape

@@ -1,0 +1,372 @@
+"""Muon: newton_schulz, newton_schulz_pullback and muon_raw against plain implementations in 64 bits, their refusals (host logic, no GPU), and the ways they are called.
+
+Tolerances.  Inside, a matrix element is a pair of f16 (off by at most 2^-22 of its value) and a product drops lo * lo (2^-22 again): a step's operands put at most e = 3 * 2^-22 of the
+iterate's norm into the next iterate, which later steps amplify by at most a = 3.4445 each.  Summed over five steps that is e * a^5 / (a - 1) = 1.4e-4 per singular direction, where a
+result of full rank has singular values of 0.68 and more: 2.1e-4 of the result's norm in the worst case (LOOSE).  Roundings do not all point one way: the error is also held to twice
+that of the same formulas in plain fp32, with a floor of 2e-6 (a few 2^-24 through a^5 = 485, averaged over the directions)."""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import md2amd
+
+gpu = pytest.mark.gpu
+LOOSE = 2.1e-4
+HALF = {torch.float32: 0.0, torch.bfloat16: torch.finfo(torch.bfloat16).eps / 2, torch.float16: torch.finfo(torch.float16).eps / 2}
+COEF = (3.4445, -4.7750, 2.0315)
+
+
+def md():
+    return md2amd.monodepth
+
+
+def ns_plain(x, steps=5, coef=COEF, eps=1e-7):
+    """The definition, in x's type (the norm in 64 bits), for (..., rows, cols)."""
+    a, b, c = coef
+    norm = x.double().square().sum((-2, -1), keepdim=True).sqrt().clamp_min(eps)
+    x = (x.double() / norm).to(x.dtype)
+    tall = x.shape[-2] > x.shape[-1]
+    x = x.transpose(-1, -2).contiguous() if tall else x
+    for _ in range(steps):
+        g = x @ x.transpose(-1, -2).contiguous()
+        x = a * x + (b * g + c * (g @ g)) @ x
+    return x.transpose(-1, -2) if tall else x
+
+
+def rel(a, b):
+    a, b = a.detach().double().cpu(), b.detach().double().cpu()
+    return float((a - b).norm() / (b.norm() + 1e-300))
+
+
+def gradient_like(shape, seed, noise=0.3, scale=1e-3):
+    g = torch.Generator().manual_seed(seed); r, c = shape[-2:]; k = min(r, c, 8); lead = tuple(shape[:-2])
+    u = torch.randn(lead + (r, k), generator=g, dtype=torch.float64) / torch.arange(1, k + 1)
+    return scale * (u @ torch.randn(lead + (k, c), generator=g, dtype=torch.float64) + noise * torch.randn(tuple(shape), generator=g, dtype=torch.float64))
+
+
+# ---- refusals: decided on the host, before anything reaches the GPU ---------------------------------------------------------
+def last_error():
+    return md2amd._lib.lib().md2_last_error(None).decode()
+
+
+def test_tensors_that_are_refused():
+    m = md()
+    for bad in (torch.zeros(4, 4), torch.zeros(4), [[1.0]], torch.zeros(4, 4, dtype=torch.float64)):
+        with pytest.raises(ValueError):
+            m.newton_schulz(bad)
+    with pytest.raises(ValueError):
+        m.newton_schulz_pullback(torch.zeros(4, 4), torch.zeros(4, 4))
+    with pytest.raises(ValueError):
+        m.muon_raw([torch.zeros(4, 4)], [torch.zeros(4, 4)], [torch.zeros(4, 4)])
+    with pytest.raises(ValueError):
+        m.muon_raw([torch.zeros(4, 4)], [], [torch.zeros(4, 4)])
+    with pytest.raises(ValueError):
+        m.muon_raw([], [], [], adjust="other")
+
+
+def test_workspace_sizes_and_refused_sizes():
+    L = md2amd._lib.lib()
+    for pull in (0, 1):
+        assert L.md2_newton_schulz_workspace(1, 1, 1, 5, pull) > 0
+        for bad in ((0, 4, 4), (1, 0, 4), (1, 4, 0), (-1, 4, 4), (1, -4, 4), (1, 1 << 21, 4), (1, 1 << 17, 1 << 17), (1 << 21, 4, 4)):
+            assert L.md2_newton_schulz_workspace(*bad, 5, pull) == -1, bad
+        for steps in (0, -1, 17):
+            assert L.md2_newton_schulz_workspace(1, 4, 4, steps, pull) == -1
+    assert L.md2_newton_schulz_workspace(3, 100, 200, 5, 0) < L.md2_newton_schulz_workspace(3, 100, 200, 5, 1)
+    I = ctypes.c_int64
+    assert L.md2_muon_workspace((I * 2)(3, 4), (I * 2)(5, 6), 2, 5) > 0 and L.md2_muon_workspace((I * 1)(3), (I * 1)(0), 1, 5) == -1 and L.md2_muon_workspace(None, None, 1, 5) == -1
+
+
+def ns_c(x=4096, y=8192, batch=1, rows=8, cols=8, strides=(64, 8, 1), dtype=0, steps=5, coef=COEF, eps=1e-7, ws=4096, nbytes=None):
+    L = md2amd._lib.lib()
+    st = (ctypes.c_int64 * 3)(*strides) if strides else None; co = (ctypes.c_double * 3)(*coef) if coef else None
+    return L.md2_newton_schulz(x, y, batch, rows, cols, st, dtype, steps, co, eps, ws, 0 if nbytes is None else nbytes, None)
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(strides=None), "strides"), (dict(coef=None), "coefficients"), (dict(dtype=3), "dtype"), (dict(dtype=-1), "dtype"), (dict(steps=0), "steps"), (dict(steps=17), "steps"),
+    (dict(eps=0.0), "eps"), (dict(eps=-1.0), "eps"), (dict(eps=math.nan), "eps"), (dict(eps=math.inf), "eps"), (dict(coef=(math.nan, 0, 0)), "finite"), (dict(coef=(9.0, 0, 0)), "past 4"),
+    (dict(coef=(3.4445, -4.775, 200.0)), "past"), (dict(x=None), "null"), (dict(y=None), "null"), (dict(rows=0), "sizes"), (dict(cols=-3), "sizes"), (dict(x=4097), "aligned"),
+    (dict(strides=(64, -8, 1)), "stride"), (dict(ws=None), "workspace"), (dict(), "workspace"), (dict(ws=4100, nbytes=1 << 40), "workspace")])
+def test_newton_schulz_refuses(kw, word):
+    """Every one of these is found before the first launch (the pointers are never followed): status 2 and a reason."""
+    assert ns_c(**kw) == 2 and word in last_error(), (kw, last_error())
+
+
+def test_pullback_refuses_steps_that_would_leave_the_range():
+    L = md2amd._lib.lib(); st = (ctypes.c_int64 * 3)(64, 8, 1); co = (ctypes.c_double * 3)(*COEF)
+    assert L.md2_newton_schulz_bwd(4096, 4096, 8192, 1, 8, 8, st, st, 0, 12, co, 1e-7, 4096, 0, None) == 2 and "pullback" in last_error()
+    assert L.md2_newton_schulz_bwd(4096, None, 8192, 1, 8, 8, st, st, 0, 5, co, 1e-7, 4096, 0, None) == 2 and "null" in last_error()
+    assert L.md2_newton_schulz_bwd(4096, 4096, 8192, 1, 8, 8, st, None, 0, 5, co, 1e-7, 4096, 0, None) == 2 and "strides" in last_error()
+
+
+def muon_c(p=(4096,), g=(8192,), m=(16384,), rows=(8,), cols=(8,), lr=0.02, momentum=0.95, decay=0.0, adjust=0, scale=1.0, steps=5, eps=1e-7, count=None):
+    L = md2amd._lib.lib(); n = len(p); V, I = ctypes.c_void_p, ctypes.c_int64
+    return L.md2_muon_raw((V * n)(*p), (V * n)(*g), (V * n)(*m), (I * n)(*rows), (I * n)(*cols), n if count is None else count, lr, momentum, 1, decay, adjust, scale, steps,
+                          (ctypes.c_double * 3)(*COEF), eps, 4096, 0, None)
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(count=0), "no weights"), (dict(rows=(0,)), "sizes"), (dict(lr=-1.0), "lr"), (dict(lr=math.nan), "lr"), (dict(momentum=1.0), "momentum"), (dict(momentum=-0.1), "momentum"),
+    (dict(decay=-1.0), "weight_decay"), (dict(decay=math.inf), "weight_decay"), (dict(adjust=2), "adjust"), (dict(scale=math.nan), "grad_scale"), (dict(steps=0), "steps"), (dict(eps=0.0), "eps"),
+    (dict(p=(None,)), "null"), (dict(p=(4098,)), "aligned"), (dict(), "workspace"),
+    (dict(p=(4096,), m=(4096,)), "overlaps"), (dict(p=(4096,), g=(4096 + 252,)), "overlaps"), (dict(m=(8192,)), "overlaps"),
+    (dict(p=(4096, 4096), g=(8192, 8192), m=(16384, 20480), rows=(8, 8), cols=(8, 8)), "overlaps"),
+    (dict(p=(4096, 4096 + 128), g=(8192, 8192), m=(16384, 20480), rows=(8, 8), cols=(8, 8)), "overlaps")])
+def test_muon_raw_refuses(kw, word):
+    assert muon_c(**kw) == 2 and word in last_error(), (kw, last_error())
+
+
+def test_two_weights_may_share_a_gradient():
+    """Only what the step writes has to be disjoint: the next refusal is the workspace's."""
+    assert muon_c(p=(4096, 4096 + 256), g=(8192, 8192), m=(16384, 20480), rows=(8, 8), cols=(8, 8)) == 2 and "workspace" in last_error()
+
+
+# ---- newton_schulz ------------------------------------------------------------------------------------------------------------
+SHAPES = [(1, 1), (1, 7), (9, 1), (2, 2), (16, 16), (31, 33), (64, 64), (65, 64), (64, 576), (127, 130), (128, 128), (129, 129), (200, 77), (33, 1000), (130, 300), (257, 96), (256, 640), (385, 514)]
+
+
+def check(y, x, steps=5, coef=COEF, eps=1e-7, name=""):
+    """y against 64 bits: within the worst-case bound, and within twice what plain fp32 loses (x as the kernel got it)."""
+    xd = x.detach().double().cpu(); exact = ns_plain(xd, steps, coef, eps); plain = ns_plain(xd.float(), steps, coef, eps)
+    e, ep = rel(y, exact), rel(plain, exact)
+    assert e <= HALF[y.dtype] + LOOSE and e <= HALF[y.dtype] + max(2 * ep, 2e-6), (name, tuple(x.shape), e, ep)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", list(HALF))
+@pytest.mark.parametrize("shape", SHAPES)
+def test_newton_schulz(shape, dtype):
+    x = gradient_like(shape, sum(shape)).to(dtype).cuda()
+    keep = x.clone(); y = md().newton_schulz(x)
+    assert y.shape == x.shape and y.dtype == dtype and y.is_contiguous() and torch.equal(x, keep)
+    check(y, x)
+
+
+@gpu
+@pytest.mark.parametrize("steps", [1, 2, 3, 7, 16])
+def test_newton_schulz_steps_and_coefficients(steps):
+    x = gradient_like((40, 100), 3).float().cuda()
+    check(md().newton_schulz(x, steps=steps, coefficients=(1.875, -1.25, 0.375)), x, steps, (1.875, -1.25, 0.375))
+    if steps <= 5:
+        check(md().newton_schulz(x, steps=steps), x, steps)
+
+
+@gpu
+def test_newton_schulz_batches_strides_and_views():
+    m = md()
+    base = gradient_like((3, 2, 70, 90), 5).float().cuda()
+    y = m.newton_schulz(base); assert y.shape == base.shape
+    for b in range(3):
+        for c in range(2):
+            assert torch.equal(y[b, c], m.newton_schulz(base[b, c]))              # a matrix does not depend on its batch
+    wide = gradient_like((5, 140, 211), 6).float().cuda()
+    for v in (wide.transpose(1, 2), wide[:, ::2, ::3], wide[:, 3:100, 1:88], wide[1:4].permute(0, 2, 1)[:, 5:], wide[0], wide[2].t(), wide[:1].expand(3, -1, -1)):
+        y = m.newton_schulz(v); assert y.is_contiguous() and torch.equal(y, m.newton_schulz(v.contiguous()))
+    flat = torch.empty(33 * 47 + 1, device="cuda", dtype=torch.bfloat16); x = flat[1:].view(33, 47); x.copy_(gradient_like((33, 47), 7))      # 2-byte aligned
+    assert torch.equal(m.newton_schulz(x), m.newton_schulz(x.clone()))
+    for shape in ((0, 4, 4), (3, 0, 5), (0, 7), (7, 0)):
+        assert m.newton_schulz(torch.empty(shape, device="cuda")).shape == shape
+
+
+@gpu
+@pytest.mark.parametrize("scale", [1e-30, 1e-12, 1e-9, 1.0, 1e18, 1e30])
+def test_newton_schulz_extreme_scales_and_the_clamp(scale):
+    x = (gradient_like((48, 80), 8, scale=1.0) * scale).float().cuda()
+    for eps in (1e-7, 1e-35):                                   # below eps the matrix is not brought to norm 1: its singular values only grow by a^5
+        check(md().newton_schulz(x, eps=eps), x, eps=eps, name=eps)
+
+
+@gpu
+def test_newton_schulz_zeros_nan_and_infinities_stay_in_their_matrix():
+    m = md(); x = gradient_like((4, 70, 140), 9).float().cuda(); y = m.newton_schulz(x)
+    z = x.clone(); z[0] = 0; z[1, 3, 5] = math.nan; z[2, 69, 139] = math.inf
+    w = m.newton_schulz(z)
+    assert torch.equal(w[0], torch.zeros_like(w[0])) and torch.isnan(w[1]).all() and torch.isnan(w[2]).all() and torch.equal(w[3], y[3])
+
+
+@gpu
+def test_newton_schulz_low_rank():
+    """Rank 3 of 40: the 37 null directions hold only what rounding leaves there, amplified by a^5: 1.4e-4 in each of 40 directions, of a result of norm 0.68 sqrt(3) or more."""
+    g = torch.Generator().manual_seed(1); x = (torch.randn(40, 3, generator=g, dtype=torch.float64) @ torch.randn(3, 90, generator=g, dtype=torch.float64)).float().cuda()
+    assert rel(md().newton_schulz(x), ns_plain(x.double().cpu())) <= 1.4e-4 * math.sqrt(40) / (0.68 * math.sqrt(3))
+
+
+# ---- the pullback ---------------------------------------------------------------------------------------------------------------
+def back_plain(x, dout, steps, coef, eps, dtype):
+    x = x.detach().to(dtype).requires_grad_(True); a, b, c = coef
+    norm = x.double().square().sum((-2, -1), keepdim=True).sqrt().clamp_min(eps)
+    y = (x.double() / norm).to(dtype)
+    tall = y.shape[-2] > y.shape[-1]
+    y = y.transpose(-1, -2) if tall else y
+    for _ in range(steps):
+        g = y @ y.transpose(-1, -2); y = a * y + (b * g + c * (g @ g)) @ y
+    return torch.autograd.grad(y.transpose(-1, -2) if tall else y, x, dout.detach().to(dtype))[0]
+
+
+def check_back(dx, x, dout, steps=5, coef=COEF, eps=1e-7):
+    """The pullback's products carry the same roundings as the iteration's, and G grows by at most about 4 a step as an iterate's singular values by 3.4: the same bounds, with two chains
+    (forward, back) of errors instead of one."""
+    xd, dd = x.double().cpu(), dout.double().cpu()
+    exact, plain = back_plain(xd, dd, steps, coef, eps, torch.float64), back_plain(xd, dd, steps, coef, eps, torch.float32)
+    e, ep = rel(dx, exact), rel(plain, exact)
+    assert e <= HALF[dx.dtype] + 4 * LOOSE and e <= HALF[dx.dtype] + max(2 * ep, 4e-6), (tuple(x.shape), e, ep)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", list(HALF))
+@pytest.mark.parametrize("shape", [(1, 7), (9, 1), (2, 3), (31, 33), (64, 64), (65, 64), (64, 576), (129, 131), (200, 77), (130, 300), (3, 40, 60), (2, 150, 37)])
+def test_newton_schulz_pullback(shape, dtype):
+    x = gradient_like(shape, sum(shape)).to(dtype).cuda(); d = torch.randn(shape, generator=torch.Generator().manual_seed(2), dtype=torch.float64).to(dtype).cuda()
+    keep = x.clone(), d.clone(); dx = md().newton_schulz_pullback(x, d)
+    assert dx.shape == x.shape and dx.dtype == dtype and dx.is_contiguous() and torch.equal(x, keep[0]) and torch.equal(d, keep[1])
+    check_back(dx, x, d)
+
+
+@gpu
+def test_pullback_against_differences_of_the_forward():
+    """<dx, v> against (f(x + h v) - f(x - h v)) / 2h of the kernel's own forward, contracted with dout.  The quotient's error: f's rounding (2e-6 of |y| |dout|) over h, and the third
+    derivative's h^2 |v|^3 / |x|^2 term: with h |v| = 1e-3 |x| both are a few 1e-3 of |dout| |y| / |x| |v|; the bound is 1e-2 of that."""
+    m = md(); x = gradient_like((24, 40), 11, noise=1.0, scale=1.0).float().cuda(); g = torch.Generator().manual_seed(4)
+    d = torch.randn(24, 40, generator=g).cuda(); dx = m.newton_schulz_pullback(x, d, steps=2)
+    for _ in range(4):
+        v = torch.randn(24, 40, generator=g).cuda(); h = 1e-3 * float(x.norm() / v.norm())
+        num = float(((m.newton_schulz(x + h * v, steps=2).double() - m.newton_schulz(x - h * v, steps=2).double()) / (2 * h) * d.double()).sum())
+        scale = float(d.norm() * m.newton_schulz(x, steps=2).norm() / x.norm() * v.norm())
+        assert abs(num - float((dx.double() * v.double()).sum())) <= 1e-2 * scale
+
+
+@gpu
+@pytest.mark.parametrize("steps", [1, 2, 6])
+def test_pullback_steps_strides_and_scales(steps):
+    m = md(); co = (1.875, -1.25, 0.375)
+    x = gradient_like((2, 90, 41), 12).float().cuda(); d = torch.randn(41, 90, generator=torch.Generator().manual_seed(5)).cuda().t().expand(2, 90, 41)
+    check_back(m.newton_schulz_pullback(x, d, steps=steps, coefficients=co), x, d, steps, co)
+    for s in (1e-25, 1e20):
+        a, b = m.newton_schulz_pullback(x, (d * s), steps=steps, coefficients=co), m.newton_schulz_pullback(x, d, steps=steps, coefficients=co)
+        assert rel(a.double() / s, b) <= 1e-6
+    assert torch.equal(m.newton_schulz_pullback(x, torch.zeros_like(d), steps=steps), torch.zeros_like(x))
+
+
+@gpu
+def test_pullback_of_a_clamped_and_of_a_zero_matrix():
+    """Below eps the normalisation is a division by a constant; at x = 0 that leaves a^steps / eps * dout."""
+    m = md(); x = gradient_like((20, 30), 13, scale=1e-9).float().cuda(); d = torch.randn(20, 30, generator=torch.Generator().manual_seed(6)).cuda()
+    check_back(m.newton_schulz_pullback(x, d), x, d)
+    z = m.newton_schulz_pullback(torch.zeros(20, 30, device="cuda"), d)
+    assert rel(z, d.double() * 3.4445 ** 5 / 1e-7) <= 1e-5
+
+
+@gpu
+def test_pullback_nan_stays_in_its_matrix():
+    m = md(); x = gradient_like((3, 40, 50), 14).float().cuda(); d = torch.randn(3, 40, 50, generator=torch.Generator().manual_seed(7)).cuda(); dx = m.newton_schulz_pullback(x, d)
+    d2, x2 = d.clone(), x.clone(); d2[0, 1, 2] = math.nan; x2[2, 0, 0] = math.inf
+    w = m.newton_schulz_pullback(x2, d2)
+    assert torch.isnan(w[0]).all() and torch.equal(w[1], dx[1]) and torch.isnan(w[2]).all()
+
+
+# ---- muon_raw -------------------------------------------------------------------------------------------------------------------
+def muon_plain(p, g, m, lr, momentum, nesterov, weight_decay, adjust, grad_scale, steps=5, coef=COEF, eps=1e-7):
+    r, c = p.shape[0], p[0].numel(); g = grad_scale * g.double(); m = momentum * m.double() + (1 - momentum) * g
+    u = momentum * m + (1 - momentum) * g if nesterov else m
+    s = 0.2 * math.sqrt(max(r, c)) if adjust == "rms" else math.sqrt(max(1.0, r / c))
+    step = lr * s * ns_plain(u.reshape(r, c), steps, coef, eps).reshape(p.shape)
+    return (1 - lr * weight_decay) * p.double() - step, m, step
+
+
+WEIGHTS = [(64, 3, 3, 3), (37, 53), (1, 700), (129, 65), (300, 1), (1, 1), (16, 16, 1, 1), (96, 8, 3, 3), (255, 257), (64, 63)]
+
+
+@gpu
+@pytest.mark.parametrize("kw", [dict(), dict(nesterov=False, weight_decay=0.1), dict(adjust="rms", momentum=0.0, lr=1e-3), dict(lr=0.0, weight_decay=0.5), dict(grad_scale=-0.125)])
+def test_muon_raw(kw):
+    """Two steps of odd weights packed with gaps: weights and momenta against 64 bits, the gaps and the gradients as they were.  A weight is off by its own two roundings and the
+    orthogonalisation's error times the step."""
+    hyper = dict(lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, adjust="spectral", grad_scale=1.0); hyper.update(kw)
+    sizes = [int(np.prod(s)) for s in WEIGHTS]; gap = 3; n = sum(sizes) + gap * len(sizes)
+    bufs = {k: torch.full((n,), 7.25, device="cuda") for k in "pgm"}; views = {k: [] for k in "pgm"}; at = 0; mask = torch.ones(n, dtype=torch.bool)
+    for i, (s, k) in enumerate(zip(WEIGHTS, sizes)):
+        for q in "pgm":
+            views[q].append(bufs[q][at:at + k].view(s))
+        views["p"][-1].copy_(torch.randn(s, generator=torch.Generator().manual_seed(i)) * 0.1)
+        for q, off in (("g", 50), ("m", 90)):
+            views[q][-1].copy_(gradient_like((s[0], k // s[0]), i + off).reshape(s))
+        mask[at:at + k] = False; at += k + gap
+    for _ in range(2):
+        before = [tuple(views[q][i].double().cpu() for q in "pgm") for i in range(len(WEIGHTS))]; grads = bufs["g"].clone()
+        md().muon_raw(views["p"], views["g"], views["m"], **hyper)
+        assert torch.equal(bufs["g"], grads)
+        for q in "pm":
+            assert (bufs[q].cpu()[mask] == 7.25).all()
+        for i, (p, g, m) in enumerate(before):
+            ep, em, step = muon_plain(p, g, m, **hyper)
+            assert float((views["m"][i].double().cpu() - em).abs().max()) <= 3 * 2.0 ** -24 * float(m.abs().max() + g.abs().max() * abs(hyper["grad_scale"]))
+            err = (views["p"][i].double().cpu() - ep).norm(); assert float(err) <= float(2 * 2.0 ** -24 * (p.norm() + step.norm()) + 2e-5 * step.norm()), WEIGHTS[i]
+
+
+@gpu
+def test_muon_raw_list_order_and_company_do_not_matter():
+    m = md(); shapes = [(70, 90), (16, 40), (130, 64), (200, 200)] * 9                   # 36 weights: more than one argument block of the set-up kernel
+    def make():
+        return [[gradient_like(s, i + 100 * k).float().cuda() for i, s in enumerate(shapes)] for k in range(3)]
+    a, b = make(), make()
+    m.muon_raw(*a)
+    for i in reversed(range(len(shapes))):
+        m.muon_raw([b[0][i]], [b[1][i]], [b[2][i]])
+    assert all(torch.equal(x, y) for k in (0, 2) for x, y in zip(a[k], b[k]))
+    m.muon_raw([], [], [])
+    with pytest.raises(ValueError):
+        m.muon_raw([a[0][0].t()], [a[1][0].t()], [a[2][0].t()])
+    with pytest.raises(ValueError):
+        m.muon_raw([a[0][0][0]], [a[1][0][0]], [a[2][0][0]])
+    with pytest.raises(ValueError):
+        m.muon_raw([a[0][0]], [a[1][1]], [a[2][0]])
+    with pytest.raises(RuntimeError, match="overlaps"):
+        m.muon_raw([a[0][0], a[0][0]], [a[1][0], a[1][0]], [a[2][0], a[2][4]])
+
+
+# ---- streams, graphs, repeatability ---------------------------------------------------------------------------------------------------
+@gpu
+def test_side_streams_and_two_calls_at_once():
+    m = md(); xs = [gradient_like((200, 500), i).float().cuda() for i in range(2)]; want = [m.newton_schulz(x) for x in xs]; back = m.newton_schulz_pullback(xs[0], xs[1]); torch.cuda.synchronize()
+    st = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(5):
+        got = []
+        for s, x in zip(st, xs):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                got.append(m.newton_schulz(x)); got.append(m.newton_schulz_pullback(xs[0], xs[1]))
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[2], want[1]) and torch.equal(got[1], back) and torch.equal(got[3], back)
+
+
+@gpu
+def test_captured_and_replayed():
+    """newton_schulz, its pullback and a Muon step in graphs, replayed between eager calls on other data; two graphs of one pool."""
+    m = md(); x = gradient_like((2, 90, 150), 20).float().cuda(); d = torch.randn(2, 90, 150, generator=torch.Generator().manual_seed(8)).cuda()
+    p, g, mo = [gradient_like((90, 300), 21 + i).float().cuda() for i in range(3)]
+    m.newton_schulz(x); torch.cuda.synchronize()
+    g1 = torch.cuda.CUDAGraph(); g2 = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g1):
+        y, dx = m.newton_schulz(x), m.newton_schulz_pullback(x, d)
+    with torch.cuda.graph(g2, pool=g1.pool()):
+        m.muon_raw([p], [g], [mo])
+    for r in range(4):
+        x.copy_(gradient_like((2, 90, 150), 30 + r)); p0, m0 = p.clone(), mo.clone()
+        g1.replay(); torch.cuda.synchronize()
+        assert torch.equal(y, m.newton_schulz(x)) and torch.equal(dx, m.newton_schulz_pullback(x, d))
+        g2.replay(); torch.cuda.synchronize()
+        m.muon_raw([p0], [g], [m0]); assert torch.equal(p, p0) and torch.equal(mo, m0)
+
+
+@gpu
+def test_orthogonalised_weight_trains_through_its_pullback():
+    """A run of the operators together: w = newton_schulz(v), loss 1/2 |w - target|^2, dv by the pullback, v stepped by muon_raw; every step's gradient against 64 bits."""
+    m = md(); v = gradient_like((48, 96), 40, noise=1.0, scale=1.0).float().cuda(); t = m.newton_schulz(gradient_like((48, 96), 41, noise=1.0).float().cuda()); mo = torch.zeros_like(v)
+    for _ in range(3):
+        w = m.newton_schulz(v); dv = m.newton_schulz_pullback(v, w - t)
+        check(w, v); check_back(dv, v, w - t)
+        m.muon_raw([v], [dv], [mo], lr=0.05)
