@@ -31,19 +31,23 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 namespace {
 
-constexpr int TILE = 128;                 // rows and columns of a product tile; 4 waves of 64 x 64
+constexpr int PAD = 128;                  // rows of a pair matrix are padded to this, columns of X too
 constexpr int PK_ROWS = 64, PK_COLS = 128;   // tile of the norm / pack kernels
+enum { GRAM = 0, POLY = 1, SYM_S = 2, SYM_V = 3, SYMS = 4 };      // the symmetric products: A = X X^T | B = b A + c A A | S = G X^T + X G^T | V = b S + c (S A + A S)
+constexpr int PART = 64 * 64 * 4;         // unit of the split products' partial sums, bytes
 
-// what the host passes per weight (or per batch of equal matrices), by value
+// how one weight (or batch of equal matrices) takes part in one product
+struct Use { int32_t first, red, part, tile, chunk, split; };      // first item, first reduction item, first partial sum, tile side, K blocks per item, items per tile
+// what the host passes per weight, by value
 struct Desc {
     const void* x; const void* d; void* y;                    // matrix | dout | result;  Muon: momentum | gradient | weight
     int64_t xb, xs, xl, db, ds, dl, yb, ys, yl;               // strides in elements: batch, along the short side, along the long side
     int64_t ws0, ws1;                                         // first matrix's buffers (bytes into the workspace), bytes per matrix
-    int32_t m, n, batch, first;                               // short side, long side, matrices, index of the first
-    int32_t sym0, nn0, pk0;                                   // first work items
+    int32_t m, n, batch, first, pk0, nn0, nn_tile;            // short side, long side, matrices, index of the first, first work items
     float alpha;                                              // Muon: lr * shape factor
+    Use sym[SYMS];
 };
-constexpr int DESCS = 16;                 // 16 * 168 bytes of kernel arguments
+constexpr int DESCS = 12;                 // 12 * 240 bytes of kernel arguments
 struct DescPack { Desc d[DESCS]; };
 
 // the same per matrix, on the device
@@ -54,34 +58,44 @@ struct Mat {
     int32_t m, n, mp, np, pk0, pkn, nn0, nnn;
     float alpha;
 };
-struct Item { int32_t mat, ti, tj, pad; };
+// one workgroup's work; everything a product needs before its first load is in here
+struct Item { char* buf; int32_t m, n, mat, ti, tj, tile, k0, k1, part, pad; };      // K blocks [k0, k1); part: where the partial sum goes, -1 = the result itself (reduction: k1 = how many)
 
 struct Fac { float inv2; int q; };                             // a clamped matrix is carried 2^q larger (ns_pack_kernel): 2^-2q, q
-struct Ws { Mat* mats; Item *sym, *nn, *pk; Fac* fac; double* part; char* buf; };      // part: [3][pk items] sums of squares of x, of dout, and [nn items] of X0 G
+struct Ws { Mat* mats; Item *sym[SYMS], *red[SYMS], *nn, *pk; Fac* fac; double* part; char* split; char* buf; };      // part: [2][pk items] sums of squares of x, of dout, and [nn items] of X0 G
 
-__global__ __launch_bounds__(256) void ns_setup_kernel(DescPack dp, int dt_bytes_x, int dt_bytes_y, Ws ws) {
+__host__ __device__ inline int cdiv(int a, int b) { return (a + b - 1) / b; }
+__host__ __device__ inline int kblocks(int kind, int m, int n) { return (kind >= SYM_S ? 2 : 1) * cdiv(kind == GRAM || kind == SYM_S ? n : m, 32); }
+
+__global__ __launch_bounds__(256) void ns_setup_kernel(DescPack dp, int dt_bytes, Ws ws) {
     const Desc& D = dp.d[blockIdx.y];
-    const int mt = (D.m + TILE - 1) / TILE, nt = (D.n + TILE - 1) / TILE;
-    const int nsym = mt * (mt + 1) / 2, nnn = mt * nt, npk = mt * (TILE / PK_ROWS) * nt * (TILE / PK_COLS);
+    const int mp = cdiv(D.m, PAD) * PAD, np = cdiv(D.n, PAD) * PAD, npk = mp / PK_ROWS * (np / PK_COLS), pr = mp / PK_ROWS, nr = cdiv(D.m, D.nn_tile), nnn = nr * cdiv(D.n, D.nn_tile);
     for (int b = blockIdx.x; b < D.batch; b += gridDim.x) {
-        const int id = D.first + b;
+        const int id = D.first + b; char* buf = ws.buf + D.ws0 + D.ws1 * b;
         if (threadIdx.x == 0) {
             Mat M;
-            M.x = (const char*)D.x + D.xb * b * dt_bytes_x; M.d = (const char*)D.d + D.db * b * dt_bytes_x; M.y = (char*)D.y + D.yb * b * dt_bytes_y;
+            M.x = (const char*)D.x + D.xb * b * dt_bytes; M.d = (const char*)D.d + D.db * b * dt_bytes; M.y = (char*)D.y + D.yb * b * dt_bytes;
             M.xs = D.xs; M.xl = D.xl; M.ds = D.ds; M.dl = D.dl; M.ys = D.ys; M.yl = D.yl;
-            M.buf = ws.buf + D.ws0 + D.ws1 * b;
-            M.m = D.m; M.n = D.n; M.mp = mt * TILE; M.np = nt * TILE;
-            M.xbytes = (int64_t)M.mp * M.np * 4; M.abytes = (int64_t)M.mp * M.mp * 4;
+            M.buf = buf; M.m = D.m; M.n = D.n; M.mp = mp; M.np = np;
+            M.xbytes = (int64_t)mp * np * 4; M.abytes = (int64_t)mp * mp * 4;
             M.pk0 = D.pk0 + npk * b; M.pkn = npk; M.nn0 = D.nn0 + nnn * b; M.nnn = nnn; M.alpha = D.alpha;
             ws.mats[id] = M;
         }
-        for (int q = threadIdx.x; q < mt * mt; q += 256) {
-            const int i = q / mt, j = q % mt;
-            if (j >= i) ws.sym[D.sym0 + nsym * b + i * mt - i * (i - 1) / 2 + (j - i)] = Item{id, i, j, 0};
+        for (int kind = 0; kind < SYMS; ++kind) {
+            const Use& u = D.sym[kind];
+            if (!u.tile) continue;
+            const int mt = cdiv(D.m, u.tile), tri = mt * (mt + 1) / 2, kb = kblocks(kind, D.m, D.n), per = u.tile * u.tile * 4 / PART;
+            for (int q = threadIdx.x; q < mt * mt; q += 256) {
+                const int i = q / mt, j = q % mt;
+                if (j < i) continue;
+                const int e = i * mt - i * (i - 1) / 2 + (j - i), part = u.part + (tri * b + e) * u.split * per;
+                for (int k = 0; k < u.split; ++k)
+                    ws.sym[kind][u.first + (tri * b + e) * u.split + k] = Item{buf, D.m, D.n, id, i, j, u.tile, k * u.chunk, min(kb, (k + 1) * u.chunk), u.split > 1 ? part + k * per : -1, 0};
+                if (u.split > 1) ws.red[kind][u.red + tri * b + e] = Item{buf, D.m, D.n, id, i, j, u.tile, 0, u.split, part, 0};
+            }
         }
-        for (int q = threadIdx.x; q < nnn; q += 256) ws.nn[D.nn0 + nnn * b + q] = Item{id, q % mt, q / mt, 0};
-        const int pr = mt * (TILE / PK_ROWS);
-        for (int q = threadIdx.x; q < npk; q += 256) ws.pk[D.pk0 + npk * b + q] = Item{id, q % pr, q / pr, 0};
+        for (int q = threadIdx.x; q < nnn; q += 256) ws.nn[D.nn0 + nnn * b + q] = Item{buf, D.m, D.n, id, q % nr, q / nr, D.nn_tile, 0, 0, 0, 0};
+        for (int q = threadIdx.x; q < npk; q += 256) ws.pk[D.pk0 + npk * b + q] = Item{buf, D.m, D.n, id, q % pr, q / pr, 0, 0, 0, 0, 0};
     }
 }
 
@@ -199,175 +213,306 @@ template <int DT, int SRC> __global__ __launch_bounds__(256) void ns_pack_kernel
 // ---- products -------------------------------------------------------------------------------------------------------------
 struct Slot { int x, a; };                                                      // buffer = x * xbytes + a * abytes behind the matrix's first
 __device__ inline char* slot(const Mat& M, Slot s) { return M.buf + s.x * M.xbytes + s.a * M.abytes; }
-__device__ inline f32x16 mfma3(f16x8 ah, f16x8 al, f16x8 bh, f16x8 bl, f32x16 c) {
-    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh, c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl, c, 0, 0, 0);
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, c, 0, 0, 0);
+struct Dims { int64_t xrb, arb, xbytes, abytes; };                              // row bytes and buffer bytes of X's and of A's kind
+__device__ inline Dims dims(const Item& it) {
+    const int mp = cdiv(it.m, PAD) * PAD, np = cdiv(it.n, PAD) * PAD;
+    return Dims{(int64_t)np * 4, (int64_t)mp * 4, (int64_t)mp * np * 4, (int64_t)mp * mp * 4};
 }
-// 128 rows x 32 columns of a pair matrix, 16 KB of LDS: row r's eight 16-byte chunks (hi k 0..7, 8..15, 16..23, 24..31, then lo) are stored at chunk ^ (r & 7), so that eight
-// neighbouring rows' reads of one chunk meet eight different bank groups
-__device__ inline void stage_rows(char* lds, const char* src, int64_t rb) {
+__device__ inline char* slot(const Item& it, const Dims& d, Slot s) { return it.buf + s.x * d.xbytes + s.a * d.abytes; }
+
+typedef const __attribute__((address_space(1))) void* glb_t;
+typedef __attribute__((address_space(3))) void* lds_t;
+constexpr int STAGE = 16384;              // bytes of LDS one staged operand takes: 128 rows (or columns) x 32 K of pairs, or four waves' 64 x 32 of their own
+constexpr int LDS_BYTES = 4 * STAGE;      // 128-tiles: two operands, double buffered.  64-tiles: two operands, four waves.  Epilogue: a 128 x 128 fp32 tile, or four 64 x 64
+
+// Direct loads (global memory -> LDS, 16 bytes a lane; a wave writes 1 KB in lane order, so the bank swizzle is in which chunk a lane FETCHES).
+// Rows: ROWS x 32 columns of a pair matrix; row r's eight 16-byte chunks (hi k 0..7, 8..15, 16..23, 24..31, then lo) are stored at chunk ^ (r & 7), so that eight neighbouring rows'
+// reads of one chunk meet eight different bank groups.
+template <int ROWS, int THREADS> __device__ inline void stage_rows(char* lds, const char* src, int64_t rb, int tid) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const int id = q * 256 + threadIdx.x, r = id >> 3, c = id & 7;
-        *reinterpret_cast<f32x4*>(lds + r * 128 + ((c ^ (r & 7)) << 4)) = *reinterpret_cast<const f32x4*>(src + r * rb + c * 16);
+    for (int q = 0; q < ROWS * 8 / THREADS; ++q) {
+        const int id = q * THREADS + tid, r = id >> 3, c = (id & 7) ^ (r & 7);
+        __builtin_amdgcn_global_load_lds((glb_t)(src + r * rb + c * 16), (lds_t)(lds + q * THREADS * 16 + (tid & ~63) * 16), 16, 0, 0);
     }
 }
 __device__ inline f16x8 frag_rows(const char* lds, int r, int c) { return *reinterpret_cast<const f16x8*>(lds + r * 128 + ((c ^ (r & 7)) << 4)); }
-// 32 rows (the K axis) x 128 columns, 16 KB: a row's sixteen 32-byte units are stored at unit ^ (k & 7), so that the four rows of a transposed read meet different banks
-__device__ inline void stage_cols(char* lds, const char* src, int64_t rb) {
+// Columns: 32 rows (the K axis) x COLS columns; a row's 32-byte units are stored at unit ^ (k & 7), so that the four rows of a transposed read meet different banks
+template <int COLS, int THREADS> __device__ inline void stage_cols(char* lds, const char* src, int64_t rb, int tid) {
+    constexpr int CH = COLS / 4;          // 16-byte chunks a row
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const int id = q * 256 + threadIdx.x, k = id >> 5, c = id & 31;
-        *reinterpret_cast<f32x4*>(lds + k * 512 + (((c >> 1) ^ (k & 7)) << 5) + (c & 1) * 16) = *reinterpret_cast<const f32x4*>(src + k * rb + c * 16);
+    for (int q = 0; q < 32 * CH / THREADS; ++q) {
+        const int id = q * THREADS + tid, k = id / CH, c = (id % CH) ^ ((k & 7) << 1);
+        __builtin_amdgcn_global_load_lds((glb_t)(src + k * rb + c * 16), (lds_t)(lds + q * THREADS * 16 + (tid & ~63) * 16), 16, 0, 0);
     }
 }
 // The MFMA operand of 32 columns from c0 and 16 rows from k0 (lane: column lane % 32, rows (lane / 32) * 8 .. + 8).  ds_read_b64_tr_b16: within 16 lanes, lane s gives the
 // address of 4 columns of row s / 4 and receives the four rows of column s; so two reads of 4 rows make the operand.
-__device__ inline f16x8 frag_cols(const char* lds, int k0, int c0, int lo) {
+template <int COLS> __device__ inline f16x8 frag_cols(const char* lds, int k0, int c0, int lo) {
     const int l = threadIdx.x & 63, s = l & 15, g = l >> 4;
     const int col = c0 + (g & 1) * 16 + (s & 3) * 4, unit = (col >> 5) * 4 + lo * 2 + ((col >> 4) & 1);
     f16x8 r;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int k = k0 + (g >> 1) * 8 + h * 4 + (s >> 2);
-        const char* p = lds + k * 512 + ((unit ^ (k & 7)) << 5) + (col & 15) * 2;
+        const char* p = lds + k * (COLS * 4) + ((unit ^ (k & 7)) << 5) + (col & 15) * 2;
         const s16x4 q = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
 #pragma unroll
         for (int e = 0; e < 4; ++e) r[h * 4 + e] = __builtin_bit_cast(_Float16, (short)q[e]);
     }
     return r;
 }
-
-struct SymArgs { Slot l[2], r[2], e, out; int nseg, k_is_n, have_e; float acc, ecoef; };      // out = acc * (sum of l r^T) + ecoef * e, in the buffers' own scales (with e: a factor A too many)
-// A tile on or above the diagonal of a symmetric result, and its mirror image
-__global__ __launch_bounds__(256, 2) void ns_sym_kernel(Ws ws, SymArgs a) {
-    __shared__ __attribute__((aligned(16))) char lds[2 * 16384];
-    const Item it = ws.sym[blockIdx.x]; const Mat M = ws.mats[it.mat];
-    const int t = threadIdx.x, lane = t & 63, wv = t >> 6, wi = (wv >> 1) * 64, wj = (wv & 1) * 64, lr = lane & 31, lk = lane >> 5;
-    const int64_t rb = (int64_t)(a.k_is_n ? M.np : M.mp) * 4; const int kb = ((a.k_is_n ? M.n : M.m) + 31) / 32;
-    f32x16 c[2][2] = {};
-    for (int sg = 0; sg < a.nseg; ++sg) {
-        const char* L = slot(M, a.l[sg]) + (int64_t)it.ti * TILE * rb; const char* R = slot(M, a.r[sg]) + (int64_t)it.tj * TILE * rb;
-        for (int k = 0; k < kb; ++k) {
-            __syncthreads();
-            stage_rows(lds, L + k * 128, rb); stage_rows(lds + 16384, R + k * 128, rb);
-            __syncthreads();
+__device__ inline f32x16 mfma3(f16x8 ah, f16x8 al, f16x8 bh, f16x8 bl, f32x16 c) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl, c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, c, 0, 0, 0);
+}
+struct Frags { f16x8 ah[2][2], al[2][2], bh[2][2], bl[2][2]; };      // [K half][32 columns of the wave's 64]
+// a: read as rows, or (COLS > 0) transposed out of COLS staged columns
+template <int COLS> __device__ inline void read_frags(Frags& f, const char* la, const char* lb, int wa, int wb) {
+    const int lane = threadIdx.x & 63, lr = lane & 31, lk = lane >> 5;
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                f16x8 ah[2], al[2], bh[2], bl[2];
+    for (int s = 0; s < 2; ++s)
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    ah[q] = frag_rows(lds, wi + q * 32 + lr, s * 2 + lk); al[q] = frag_rows(lds, wi + q * 32 + lr, s * 2 + lk + 4);
-                    bh[q] = frag_rows(lds + 16384, wj + q * 32 + lr, s * 2 + lk); bl[q] = frag_rows(lds + 16384, wj + q * 32 + lr, s * 2 + lk + 4);
-                }
-#pragma unroll
-                for (int p = 0; p < 2; ++p)
-#pragma unroll
-                    for (int q = 0; q < 2; ++q) c[p][q] = mfma3(ah[p], al[p], bh[q], bl[q], c[p][q]);
-            }
+        for (int q = 0; q < 2; ++q) {
+            if constexpr (COLS > 0) { f.ah[s][q] = frag_cols<COLS>(la, s * 16, wa + q * 32, 0); f.al[s][q] = frag_cols<COLS>(la, s * 16, wa + q * 32, 1); }
+            else { f.ah[s][q] = frag_rows(la, wa + q * 32 + lr, s * 2 + lk); f.al[s][q] = frag_rows(la, wa + q * 32 + lr, s * 2 + lk + 4); }
+            f.bh[s][q] = frag_rows(lb, wb + q * 32 + lr, s * 2 + lk); f.bl[s][q] = frag_rows(lb, wb + q * 32 + lr, s * 2 + lk + 4);
         }
+}
+__device__ inline void multiply(const Frags& f, f32x16 c[2][2]) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) c[p][q] = mfma3(f.ah[s][p], f.al[s][p], f.bh[s][q], f.bl[s][q], c[p][q]);
+}
+// (LDS operations and loads in flight of this wave have landed; the direct loads are counted by vmcnt)
+__device__ inline void landed() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
+
+// One operand pair of a product: a's and b's first bytes and what a K block advances them by
+struct Seg { const char *a, *b; int64_t arb, brb, ak, bk; };
+// sum over the K blocks [k0, k1) of a b^T (NN: a's K axis runs along its rows).  The blocks of the second segment begin at `kb`; c is multiplied by `mid` there.
+// T = 128: four waves of 64 x 64, operands staged for all of them, two buffers: a step's loads are issued behind the reads of the step before and have its MFMAs to land in.
+// T = 64: every wave has the whole tile and each fourth K block, its own 16 KB of LDS and no barrier; the four sums meet in the epilogue.
+template <int T, bool NN> __device__ inline void product(char* lds, const Seg seg[2], int kb, int k0, int k1, float mid, f32x16 c[2][2]) {
+    const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
+    const int step = T == 128 ? 1 : 4, wa = T == 128 ? (wv >> 1) * 64 : 0, wb = T == 128 ? (wv & 1) * 64 : 0;
+    Frags f;
+    auto issue = [&](int k, int buf) {
+        const Seg& sg = seg[k >= kb]; const int kk = k >= kb ? k - kb : k;
+        const char *pa = sg.a + kk * sg.ak, *pb = sg.b + kk * sg.bk;
+        if constexpr (T == 128) {
+            char* l = lds + buf * 2 * STAGE;
+            if constexpr (NN) stage_cols<128, 256>(l, pa, sg.arb, t); else stage_rows<128, 256>(l, pa, sg.arb, t);
+            stage_rows<128, 256>(l + STAGE, pb, sg.brb, t);
+        } else {
+            char* l = lds + wv * STAGE;
+            if constexpr (NN) stage_cols<64, 64>(l, pa, sg.arb, lane); else stage_rows<64, 64>(l, pa, sg.arb, lane);
+            stage_rows<64, 64>(l + STAGE / 2, pb, sg.brb, lane);
+        }
+    };
+    const int first = k0 + (T == 128 ? 0 : wv); bool second = first >= kb;
+    if (first < k1) issue(first, 0);
+    int buf = 0;
+    for (int k = first; k < k1; k += step) {
+        landed();
+        if constexpr (T == 128) __syncthreads();
+        const char* l = T == 128 ? lds + buf * 2 * STAGE : lds + wv * STAGE;
+        read_frags<NN ? T : 0>(f, l, l + (T == 128 ? STAGE : STAGE / 2), wa, wb);
+        if (k + step < k1) {
+            if constexpr (T != 128) landed();                    // the same buffer again: its reads have landed
+            issue(k + step, buf ^ 1);
+        }
+        if (!second && k >= kb) {                                // the second product's scale is another power of two
+            second = true;
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+#pragma unroll
+                for (int q = 0; q < 2; ++q) c[p][q] *= mid;
+        }
+        multiply(f, c);
+        buf ^= 1;
     }
-    // lane: column j, registers: rows i .. i + 3
-    const int64_t arb = (int64_t)M.mp * 4; char* out = slot(M, a.out); const char* E = slot(M, a.e); const float facc = a.have_e ? a.acc * ws.fac[it.mat].inv2 : a.acc;
+    if (!second && kb < k1)                                      // (this wave's share ended before the second product)
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) c[p][q] *= mid;
+}
+
+// The tile in LDS as fp32, rows = b's axis, columns = a's: 16-byte units at unit ^ row, so that writes along the lanes' rows and reads along a row both meet every bank
+template <int T> __device__ inline int tile_at(int r, int c) { return r * T + ((((c >> 2) ^ r) & (T / 4 - 1)) << 2) + (c & 3); }
+template <int T> __device__ inline void tile_store(float* tile, const f32x16 c[2][2]) {
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, lr = lane & 31, lk = lane >> 5, wa = T == 128 ? (wv >> 1) * 64 : 0, wb = T == 128 ? (wv & 1) * 64 : 0;
+    float* l = tile + (T == 128 ? 0 : wv * 64 * 64);
+    __syncthreads();                                             // the staged operands have been read by every wave
 #pragma unroll
     for (int p = 0; p < 2; ++p)
 #pragma unroll
         for (int q = 0; q < 2; ++q)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const int i = it.ti * TILE + wi + p * 32 + g * 8 + lk * 4, j = it.tj * TILE + wj + q * 32 + lr;
-                const int64_t o = pair_off(arb, j, i);
-                float v[4]; f16x4 hi, lo;
+                f32x4 w;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = facc * c[p][q][g * 4 + e];
-                if (a.have_e) {
-                    const f16x4 eh = *reinterpret_cast<const f16x4*>(E + o), el = *reinterpret_cast<const f16x4*>(E + o + 64);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] += a.ecoef * ((float)eh[e] + (float)el[e]);
-                }
-                split4(v, hi, lo);
-                *reinterpret_cast<f16x4*>(out + o) = hi; *reinterpret_cast<f16x4*>(out + o + 64) = lo;
-                if (it.ti != it.tj)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) { char* w = out + pair_off(arb, i + e, j); *reinterpret_cast<_Float16*>(w) = hi[e]; *reinterpret_cast<_Float16*>(w + 64) = lo[e]; }
+                for (int e = 0; e < 4; ++e) w[e] = c[p][q][g * 4 + e];
+                *reinterpret_cast<f32x4*>(l + tile_at<T>(wb + q * 32 + lr, wa + p * 32 + g * 8 + lk * 4)) = w;
             }
+    __syncthreads();
+}
+// eight neighbouring columns of a row; 64-tiles: of the four waves' sums
+template <int T> __device__ inline void tile_row8(const float* tile, int planes, int r, int c, float v[8]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        f32x4 w = *reinterpret_cast<const f32x4*>(tile + tile_at<T>(r, c + h * 4));
+        if (T == 64 && planes == 4) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(tile + 4096 + tile_at<T>(r, c + h * 4)), y = *reinterpret_cast<const f32x4*>(tile + 8192 + tile_at<T>(r, c + h * 4)),
+                        z = *reinterpret_cast<const f32x4*>(tile + 12288 + tile_at<T>(r, c + h * 4));
+            w = (w + x) + (y + z);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[h * 4 + e] = w[e];
+    }
+}
+template <int T> __device__ inline float tile_el(const float* tile, int planes, int r, int c) {
+    const int o = tile_at<T>(r, c);
+    return T == 64 && planes == 4 ? (tile[o] + tile[4096 + o]) + (tile[8192 + o] + tile[12288 + o]) : tile[o];
+}
+__device__ inline void load_pair8(const char* p, float v[8]) {
+    const f16x8 h = *reinterpret_cast<const f16x8*>(p), l = *reinterpret_cast<const f16x8*>(p + 64);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (float)h[e] + (float)l[e];
+}
+__device__ inline void store_pair8(char* p, const float v[8]) {
+    f16x4 h[2], l[2]; split4(v, h[0], l[0]); split4(v + 4, h[1], l[1]);
+    *reinterpret_cast<f16x8*>(p) = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7); *reinterpret_cast<f16x8*>(p + 64) = __builtin_shufflevector(l[0], l[1], 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+struct SymArgs { Slot l[2], r[2], e, out; int kind, nseg, have_e; float acc, ecoef; };      // out = acc * (sum of l r^T) + ecoef * e, in the buffers' own scales (with e: a factor A too many)
+// the tile (rows: tj's, columns: ti's) to its place and, off the diagonal, to its mirror image's
+template <int T> __device__ inline void sym_finish(const Item& it, const Dims& d, const SymArgs& a, const Fac* facs, const float* tile, int planes) {
+    const int t = threadIdx.x; constexpr int PER = T / 8;        // threads a row
+    char* out = slot(it, d, a.out); const char* E = slot(it, d, a.e); const float facc = a.have_e ? a.acc * facs[it.mat].inv2 : a.acc;
+#pragma unroll 1
+    for (int side = 0; side < (it.ti == it.tj ? 1 : 2); ++side)
+#pragma unroll 2
+        for (int z = 0; z < T * PER / 256; ++z) {
+            const int r = z * (256 / PER) + t / PER, c = (t % PER) * 8; float v[8];
+            if (side == 0) tile_row8<T>(tile, planes, r, c, v);
+            else
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = tile_el<T>(tile, planes, c + e, r);
+            const int64_t o = pair_off(d.arb, (side ? it.ti : it.tj) * T + r, (side ? it.tj : it.ti) * T + c);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] *= facc;
+            if (a.have_e) {
+                float x[8]; load_pair8(E + o, x);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] += a.ecoef * x[e];
+            }
+            store_pair8(out + o, v);
+        }
+}
+template <int T> __device__ inline void sym_tile(char* lds, const Item& it, const Ws& ws, const SymArgs& a) {
+    const Dims d = dims(it); const bool kn = a.kind == GRAM || a.kind == SYM_S; const int64_t rb = kn ? d.xrb : d.arb;
+    Seg seg[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) seg[s] = Seg{slot(it, d, a.l[s]) + (int64_t)it.ti * T * rb, slot(it, d, a.r[s]) + (int64_t)it.tj * T * rb, rb, rb, 128, 128};
+    f32x16 c[2][2] = {};
+    product<T, false>(lds, seg, a.nseg == 2 ? cdiv(kn ? it.n : it.m, 32) : 1 << 30, it.k0, it.k1, 1.f, c);
+    float* tile = reinterpret_cast<float*>(lds); tile_store<T>(tile, c);
+    if (it.part < 0) sym_finish<T>(it, d, a, ws.fac, tile, 4);
+    else {
+        constexpr int PER = T / 8; float* out = reinterpret_cast<float*>(ws.split + (int64_t)it.part * PART);
+#pragma unroll 2
+        for (int z = 0; z < T * PER / 256; ++z) {
+            const int r = z * (256 / PER) + threadIdx.x / PER; float v[8]; const int col = (threadIdx.x % PER) * 8; tile_row8<T>(tile, 4, r, col, v);
+            *reinterpret_cast<f32x4*>(out + r * T + col) = f32x4{v[0], v[1], v[2], v[3]}; *reinterpret_cast<f32x4*>(out + r * T + col + 4) = f32x4{v[4], v[5], v[6], v[7]};
+        }
+    }
+}
+// A tile on or above the diagonal of a symmetric result, or its share of a split K axis
+__global__ __launch_bounds__(256, 2) void ns_sym_kernel(Ws ws, SymArgs a) {
+    __shared__ __attribute__((aligned(16))) char lds[LDS_BYTES];
+    const Item it = ws.sym[a.kind][blockIdx.x];
+    if (it.tile == 128) sym_tile<128>(lds, it, ws, a); else sym_tile<64>(lds, it, ws, a);
+}
+// the shares of a tile, summed in order
+template <int T> __device__ inline void reduce_tile(float* tile, const Item& it, const Ws& ws, const SymArgs& a) {
+    constexpr int PER = T / 8; const float* in = reinterpret_cast<const float*>(ws.split + (int64_t)it.part * PART);
+#pragma unroll 2
+    for (int z = 0; z < T * PER / 256; ++z) {
+        const int r = z * (256 / PER) + threadIdx.x / PER, col = (threadIdx.x % PER) * 8; f32x4 v[2] = {};
+        for (int k = 0; k < it.k1; ++k)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) v[h] += *reinterpret_cast<const f32x4*>(in + (int64_t)k * T * T + r * T + col + h * 4);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) *reinterpret_cast<f32x4*>(tile + tile_at<T>(r, col + h * 4)) = v[h];
+    }
+    __syncthreads();
+    sym_finish<T>(it, dims(it), a, ws.fac, tile, 1);
+}
+__global__ __launch_bounds__(256) void ns_reduce_kernel(Ws ws, SymArgs a) {
+    __shared__ __attribute__((aligned(16))) float tile[128 * 128];
+    const Item it = ws.red[a.kind][blockIdx.x];
+    if (it.tile == 128) reduce_tile<128>(tile, it, ws, a); else reduce_tile<64>(tile, it, ws, a);
 }
 
 enum { OUT_PAIR = 0, OUT_Y = 1, OUT_MUON = 2, OUT_BACK = 3 };
 struct NnArgs { Slot l[2], r[2], e, out, x0; int nseg; float acc, ecoef, mid, decay; };      // value = acc * (mid * l0 r0 + l1 r1) + ecoef * e; one product: acc * l0 r0 + ecoef * e
-// A tile of (symmetric m x m) x (m x n)
-template <int DT, int OUT> __global__ __launch_bounds__(256, 2) void ns_nn_kernel(Ws ws, NnArgs a, double* dots) {
-    __shared__ __attribute__((aligned(16))) char lds[2 * 16384]; __shared__ double red[4];
-    const Item it = ws.nn[blockIdx.x]; const Mat M = ws.mats[it.mat];
-    const int t = threadIdx.x, lane = t & 63, wv = t >> 6, wi = (wv >> 1) * 64, wj = (wv & 1) * 64, lr = lane & 31, lk = lane >> 5;
-    const int64_t arb = (int64_t)M.mp * 4, xrb = (int64_t)M.np * 4; const int kb = (M.m + 31) / 32;
-    f32x16 c[2][2] = {};                                           // [j][i]: lane = row i, registers = four neighbouring columns j
-    for (int sg = 0; sg < a.nseg; ++sg) {
-        if (sg)                                                    // the second product's scale is another power of two
+template <int T, int DT, int OUT> __device__ inline void nn_tile(char* lds, double* red, const Item& it, const Ws& ws, const NnArgs& a, double* dots) {
+    const Dims d = dims(it); const int kb = cdiv(it.m, 32), t = threadIdx.x;
+    const Fac fac = ws.fac[it.mat]; const float facc = a.acc * fac.inv2;
+    Seg seg[2];
 #pragma unroll
-            for (int p = 0; p < 2; ++p)
+    for (int s = 0; s < 2; ++s) seg[s] = Seg{slot(it, d, a.r[s]) + (int64_t)it.tj * T * 4, slot(it, d, a.l[s]) + (int64_t)it.ti * T * d.arb, d.xrb, d.arb, 32 * d.xrb, 128};
+    f32x16 c[2][2] = {};
+    product<T, true>(lds, seg, a.nseg == 2 ? kb : 1 << 30, 0, a.nseg * kb, a.mid, c);
+    float* tile = reinterpret_cast<float*>(lds); tile_store<T>(tile, c);
+    constexpr int PER = T / 8; const char* E = slot(it, d, a.e); double dot = 0;
+#pragma unroll 2
+    for (int z = 0; z < T * PER / 256; ++z) {
+        const int r = z * (256 / PER) + t / PER, col = (t % PER) * 8; float v[8], x[8];
+        tile_row8<T>(tile, 4, r, col, v);
+        const int64_t o = pair_off(d.xrb, it.ti * T + r, it.tj * T + col);
+        load_pair8(E + o, x);
 #pragma unroll
-                for (int q = 0; q < 2; ++q) c[p][q] *= a.mid;
-        const char* L = slot(M, a.l[sg]) + (int64_t)it.ti * TILE * arb; const char* R = slot(M, a.r[sg]) + (int64_t)it.tj * TILE * 4;
-        for (int k = 0; k < kb; ++k) {
-            __syncthreads();
-            stage_rows(lds, L + k * 128, arb); stage_cols(lds + 16384, R + (int64_t)k * 32 * xrb, xrb);
-            __syncthreads();
+        for (int e = 0; e < 8; ++e) v[e] = facc * v[e] + a.ecoef * x[e];
+        if constexpr (OUT == OUT_PAIR) store_pair8(slot(it, d, a.out) + o, v);
+        else if constexpr (OUT == OUT_BACK) {                    // G in fp32, and this tile's share of <X0, G>
+            load_pair8(slot(it, d, a.x0) + o, x);
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                f16x8 ah[2], al[2], bh[2], bl[2];
+            for (int e = 0; e < 8; ++e) dot += (double)x[e] * (double)v[e];
+            float* w = reinterpret_cast<float*>(slot(it, d, a.out) + (it.ti * T + r) * d.xrb + (int64_t)(it.tj * T + col) * 4);
+            *reinterpret_cast<f32x4*>(w) = f32x4{v[0], v[1], v[2], v[3]}; *reinterpret_cast<f32x4*>(w + 4) = f32x4{v[4], v[5], v[6], v[7]};
+        } else {
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    ah[q] = frag_cols(lds + 16384, s * 16, wj + q * 32, 0); al[q] = frag_cols(lds + 16384, s * 16, wj + q * 32, 1);
-                    bh[q] = frag_rows(lds, wi + q * 32 + lr, s * 2 + lk); bl[q] = frag_rows(lds, wi + q * 32 + lr, s * 2 + lk + 4);
-                }
-#pragma unroll
-                for (int p = 0; p < 2; ++p)
-#pragma unroll
-                    for (int q = 0; q < 2; ++q) c[p][q] = mfma3(ah[p], al[p], bh[q], bl[q], c[p][q]);
-            }
+            for (int h = 0; h < 2; ++h) *reinterpret_cast<f32x4*>(tile + tile_at<T>(r, col + h * 4)) = f32x4{v[h * 4], v[h * 4 + 1], v[h * 4 + 2], v[h * 4 + 3]};
         }
     }
-    const char* E = slot(M, a.e); double dot = 0; const Fac fac = ws.fac[it.mat]; const float facc = a.acc * fac.inv2;
-#pragma unroll
-    for (int p = 0; p < 2; ++p)
-#pragma unroll
-        for (int q = 0; q < 2; ++q)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int i = it.ti * TILE + wi + q * 32 + lr, j = it.tj * TILE + wj + p * 32 + g * 8 + lk * 4;
-                const int64_t o = pair_off(xrb, i, j);
-                const f16x4 eh = *reinterpret_cast<const f16x4*>(E + o), el = *reinterpret_cast<const f16x4*>(E + o + 64);
-                float v[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = facc * c[p][q][g * 4 + e] + a.ecoef * ((float)eh[e] + (float)el[e]);
-                if constexpr (OUT == OUT_PAIR) {
-                    f16x4 hi, lo; split4(v, hi, lo);
-                    char* w = slot(M, a.out) + o;
-                    *reinterpret_cast<f16x4*>(w) = hi; *reinterpret_cast<f16x4*>(w + 64) = lo;
-                } else if constexpr (OUT == OUT_BACK) {              // G in fp32, and this tile's share of <X0, G>
-                    const char* X0 = slot(M, a.x0) + o; const f16x4 xh = *reinterpret_cast<const f16x4*>(X0), xl = *reinterpret_cast<const f16x4*>(X0 + 64);
-                    f32x4 w;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) { w[e] = v[e]; dot += (double)((float)xh[e] + (float)xl[e]) * (double)v[e]; }
-                    *reinterpret_cast<f32x4*>(slot(M, a.out) + i * xrb + (int64_t)j * 4) = w;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = ldexpf(v[e], -fac.q);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (i < M.m && j + e < M.n) {
-                            const int64_t yo = i * M.ys + (j + e) * M.yl;
-                            if constexpr (OUT == OUT_Y) st_el<DT>(M.y, yo, v[e]);
-                            else { float* P = reinterpret_cast<float*>(M.y) + yo; *P = a.decay * *P - M.alpha * v[e]; }
-                        }
-                }
-            }
     if constexpr (OUT == OUT_BACK) {
         dot = block_sum(dot, red);
         if (t == 0) dots[blockIdx.x] = dot;
     }
+    if constexpr (OUT == OUT_Y || OUT == OUT_MUON) {             // element by element, neighbouring lanes along whichever axis is contiguous in the caller's memory
+        const Mat& M = ws.mats[it.mat]; const bool turn = M.ys == 1 && M.yl != 1;
+        __syncthreads();
+#pragma unroll 4
+        for (int z = 0; z < T * T / 256; ++z) {
+            const int q = z * 256 + t, r = turn ? q % T : q / T, col = turn ? q / T : q % T, i = it.ti * T + r, j = it.tj * T + col;
+            if (i < it.m && j < it.n) {
+                const float v = ldexpf(tile[tile_at<T>(r, col)], -fac.q); const int64_t o = i * M.ys + j * M.yl;
+                if constexpr (OUT == OUT_Y) st_el<DT>(M.y, o, v);
+                else { float* P = reinterpret_cast<float*>(M.y) + o; *P = a.decay * *P - M.alpha * v; }
+            }
+        }
+    }
+}
+// A tile of (symmetric m x m) x (m x n)
+template <int DT, int OUT> __global__ __launch_bounds__(256, 2) void ns_nn_kernel(Ws ws, NnArgs a, double* dots) {
+    __shared__ __attribute__((aligned(16))) char lds[LDS_BYTES]; __shared__ double red[4];
+    const Item it = ws.nn[blockIdx.x];
+    if (it.tile == 128) nn_tile<128, DT, OUT>(lds, red, it, ws, a, dots); else nn_tile<64, DT, OUT>(lds, red, it, ws, a, dots);
 }
 
 // dX = (G - X0 <X0, G>) / |X|_F, or G / eps where the norm was clamped; G carries gscale / |dout|_F
@@ -431,32 +576,59 @@ double pow2_below(double v) { return std::exp2(std::floor(std::log2(v))); }
 constexpr double SX = 8192.0, SA = 2048.0, SB = 512.0;            // scales of X (norm <= 4), A (<= 16) and B (<= 60): below 2^15, and f16 ends at 65504
 
 int64_t up(int64_t v, int64_t q) { return (v + q - 1) / q * q; }
-struct Layout { int64_t mats, sym, nn, pk, fac, part, buf, total; int64_t n_mats, n_sym, n_nn, n_pk; };
+struct Layout { int64_t mats, sym[SYMS], red[SYMS], nn, pk, fac, part, split, buf, total; int64_t n_mats, n_sym[SYMS], n_red[SYMS], n_nn, n_pk; };
 
 }  // namespace
 
-struct NsProblem { std::vector<Desc> d; int nX, nA; };
+struct NsProblem { std::vector<Desc> d; int nX, nA, kinds; };
 
+// Tiles and splits of a call's products.
+// 128-tiles share each staged row among two waves and are the faster ones where they fill the chip; with fewer than FILL of them (counting a long K axis cut into pieces of 256) a product takes
+// 64-tiles, whose four waves split K.  A K axis is then cut so that about FILL workgroups (two a CU) have the work between them, never below MIN_BLOCKS blocks of 32 an item.
+static constexpr int FILL = 512, MIN_BLOCKS = 8;
+static int64_t tri(int64_t m, int tile) { const int64_t t = (m + tile - 1) / tile; return t * (t + 1) / 2; }
 static Layout ns_layout(NsProblem& p) {
     Layout L{};
-    int64_t buf = 0;
+    int64_t buf = 0, split_max = 0;
+    for (int kind = 0; kind < p.kinds; ++kind) {
+        int64_t pieces = 0, work = 0, part = 0;
+        for (const Desc& d : p.d) pieces += d.batch * tri(d.m, 128) * ((kblocks(kind, d.m, d.n) + 7) / 8);
+        const int tile = pieces >= FILL / 2 ? 128 : 64;
+        for (const Desc& d : p.d) work += d.batch * tri(d.m, tile) * kblocks(kind, d.m, d.n);
+        const int64_t chunk = std::max<int64_t>(MIN_BLOCKS, (work + FILL - 1) / FILL);
+        for (Desc& d : p.d) {
+            Use& u = d.sym[kind]; const int64_t kb = kblocks(kind, d.m, d.n), tiles = d.batch * tri(d.m, tile);
+            u.tile = tile; u.split = (int)((kb + chunk - 1) / chunk); u.chunk = (int)((kb + u.split - 1) / u.split); u.split = (int)((kb + u.chunk - 1) / u.chunk);
+            u.first = (int)L.n_sym[kind]; u.red = (int)L.n_red[kind]; u.part = (int)part;
+            L.n_sym[kind] += tiles * u.split;
+            if (u.split > 1) { L.n_red[kind] += tiles; part += tiles * u.split * (tile * tile * 4 / PART); }
+        }
+        split_max = std::max(split_max, part);
+    }
+    int64_t nn128 = 0;
+    for (const Desc& d : p.d) nn128 += (int64_t)d.batch * cdiv(d.m, 128) * cdiv(d.n, 128);
     for (Desc& d : p.d) {
-        const int64_t mt = (d.m + TILE - 1) / TILE, nt = (d.n + TILE - 1) / TILE;
-        d.first = (int)L.n_mats; d.sym0 = (int)L.n_sym; d.nn0 = (int)L.n_nn; d.pk0 = (int)L.n_pk;
-        d.ws0 = buf; d.ws1 = (p.nX * mt * nt + p.nA * mt * mt) * (int64_t)TILE * TILE * 4;
-        L.n_mats += d.batch; L.n_sym += mt * (mt + 1) / 2 * d.batch; L.n_nn += mt * nt * d.batch; L.n_pk += mt * (TILE / PK_ROWS) * nt * (TILE / PK_COLS) * d.batch;
+        const int64_t mt = cdiv(d.m, PAD), nt = cdiv(d.n, PAD);
+        d.first = (int)L.n_mats; d.nn0 = (int)L.n_nn; d.pk0 = (int)L.n_pk; d.nn_tile = nn128 >= FILL / 2 ? 128 : 64;
+        d.ws0 = buf; d.ws1 = (p.nX * mt * nt + p.nA * mt * mt) * (int64_t)PAD * PAD * 4;
+        L.n_mats += d.batch; L.n_nn += (int64_t)cdiv(d.m, d.nn_tile) * cdiv(d.n, d.nn_tile) * d.batch; L.n_pk += mt * (PAD / PK_ROWS) * nt * (PAD / PK_COLS) * d.batch;
         buf += d.ws1 * d.batch;
     }
     int64_t at = 0;
     auto take = [&](int64_t bytes) { const int64_t r = at; at = up(at + bytes, 256); return r; };
-    L.mats = take(L.n_mats * sizeof(Mat)); L.sym = take(L.n_sym * sizeof(Item)); L.nn = take(L.n_nn * sizeof(Item)); L.pk = take(L.n_pk * sizeof(Item)); L.fac = take(L.n_mats * sizeof(Fac));
-    L.part = take((2 * L.n_pk + L.n_nn) * sizeof(double)); L.buf = take(buf); L.total = at;
+    L.mats = take(L.n_mats * sizeof(Mat));
+    for (int k = 0; k < SYMS; ++k) { L.sym[k] = take(L.n_sym[k] * sizeof(Item)); L.red[k] = take(L.n_red[k] * sizeof(Item)); }
+    L.nn = take(L.n_nn * sizeof(Item)); L.pk = take(L.n_pk * sizeof(Item)); L.fac = take(L.n_mats * sizeof(Fac));
+    L.part = take((2 * L.n_pk + L.n_nn) * sizeof(double)); L.split = take(split_max * PART); L.buf = take(buf); L.total = at;
     return L;
 }
 static bool fits(int64_t batch, int64_t rows, int64_t cols) {      // sizes whose work items and element counts stay far inside 31 bits
     return rows > 0 && cols > 0 && batch > 0 && rows <= (1 << 20) && cols <= (1 << 20) && rows * cols <= (1ll << 31) && batch <= (1 << 20);
 }
-static int64_t check_total(const Layout& L) { return (L.n_sym < (1ll << 30) && L.n_nn < (1ll << 30) && L.n_pk < (1ll << 30) && L.n_mats < (1ll << 24)) ? L.total : -1; }
+static int64_t check_total(const Layout& L) {
+    for (int k = 0; k < SYMS; ++k) if (L.n_sym[k] >= (1ll << 28)) return -1;
+    return (L.n_nn < (1ll << 28) && L.n_pk < (1ll << 28) && L.n_mats < (1ll << 24)) ? L.total : -1;
+}
 
 static Desc make_desc(const NsMatrices& q) {
     Desc d{}; const bool tall = q.rows > q.cols;
@@ -467,26 +639,31 @@ static Desc make_desc(const NsMatrices& q) {
     d.alpha = q.alpha;
     return d;
 }
-static void slots_of(int kind, int steps, int& nX, int& nA) {
+static void slots_of(int kind, int steps, NsProblem& p) {
+    int &nX = p.nX, &nA = p.nA; p.kinds = kind == NS_BACKWARD ? SYMS : 2;
     if (kind == NS_BACKWARD) { nX = steps + 2; nA = 2 * steps + 2; }      // every iterate and two G | every A, every B, S, V
     else { nX = 2; nA = 2; }                                             // X twice | A, B
 }
 int64_t ns_workspace(int kind, int steps, const NsMatrices* q, int count) {
     if (steps < 1 || steps > MD2_NS_MAX_STEPS) return -1;
-    NsProblem p; slots_of(kind, steps, p.nX, p.nA);
+    NsProblem p; slots_of(kind, steps, p);
     for (int i = 0; i < count; ++i) { if (!fits(q[i].batch, q[i].rows, q[i].cols)) return -1; p.d.push_back(make_desc(q[i])); }
     return check_total(ns_layout(p));
 }
 
 template <int DT> static void ns_launch(int kind, NsProblem& p, const Layout& L, char* base, const NsOptions& o, const Plan& P, hipStream_t s) {
-    Ws ws; ws.mats = (Mat*)(base + L.mats); ws.sym = (Item*)(base + L.sym); ws.nn = (Item*)(base + L.nn); ws.pk = (Item*)(base + L.pk); ws.fac = (Fac*)(base + L.fac); ws.part = (double*)(base + L.part); ws.buf = base + L.buf;
+    Ws ws; ws.mats = (Mat*)(base + L.mats); for (int k = 0; k < SYMS; ++k) { ws.sym[k] = (Item*)(base + L.sym[k]); ws.red[k] = (Item*)(base + L.red[k]); } ws.nn = (Item*)(base + L.nn); ws.pk = (Item*)(base + L.pk); ws.fac = (Fac*)(base + L.fac); ws.part = (double*)(base + L.part); ws.split = base + L.split; ws.buf = base + L.buf;
     const int bytes = DT == NS_F32 ? 4 : 2, steps = o.steps;
     for (size_t i = 0; i < p.d.size(); i += DESCS) {
         DescPack dp; const int n = (int)std::min<size_t>(DESCS, p.d.size() - i); int most = 1;
         for (int k = 0; k < n; ++k) { dp.d[k] = p.d[i + k]; most = std::max(most, dp.d[k].batch); }
-        hipLaunchKernelGGL(ns_setup_kernel, dim3(std::min(most, 256), n), dim3(256), 0, s, dp, bytes, bytes, ws);
+        hipLaunchKernelGGL(ns_setup_kernel, dim3(std::min(most, 256), n), dim3(256), 0, s, dp, bytes, ws);
     }
-    const dim3 blk(256), pk((unsigned)L.n_pk), sym((unsigned)L.n_sym), nn((unsigned)L.n_nn);
+    const dim3 blk(256), pk((unsigned)L.n_pk), nn((unsigned)L.n_nn);
+    auto sym = [&](const SymArgs& a) {
+        hipLaunchKernelGGL(ns_sym_kernel, dim3((unsigned)L.n_sym[a.kind]), blk, 0, s, ws, a);
+        if (L.n_red[a.kind]) hipLaunchKernelGGL(ns_reduce_kernel, dim3((unsigned)L.n_red[a.kind]), blk, 0, s, ws, a);
+    };
     const MuonArgs mu{(float)o.momentum, o.grad_scale, o.nesterov};
     double *xpart = ws.part, *dpart = ws.part + L.n_pk, *dots = ws.part + 2 * L.n_pk;
     if (kind == NS_MUON) {
@@ -503,10 +680,10 @@ template <int DT> static void ns_launch(int kind, NsProblem& p, const Layout& L,
     auto A = [&](int k) { return Slot{nX, back ? 2 * k : 0}; };
     auto B = [&](int k) { return Slot{nX, back ? 2 * k + 1 : 1}; };
     for (int k = 0; k < steps; ++k) {
-        SymArgs g{}; g.l[0] = g.r[0] = X(k); g.e = g.out = A(k); g.nseg = 1; g.k_is_n = 1; g.acc = (float)(SA / (SX * SX));
-        hipLaunchKernelGGL(ns_sym_kernel, sym, blk, 0, s, ws, g);
-        SymArgs q{}; q.l[0] = q.r[0] = q.e = A(k); q.out = B(k); q.nseg = 1; q.have_e = 1; q.acc = (float)(c * SB / (SA * SA)); q.ecoef = (float)(b * SB / SA);
-        hipLaunchKernelGGL(ns_sym_kernel, sym, blk, 0, s, ws, q);
+        SymArgs g{}; g.l[0] = g.r[0] = X(k); g.e = g.out = A(k); g.nseg = 1; g.kind = GRAM; g.acc = (float)(SA / (SX * SX));
+        sym(g);
+        SymArgs q{}; q.l[0] = q.r[0] = q.e = A(k); q.out = B(k); q.nseg = 1; q.kind = POLY; q.have_e = 1; q.acc = (float)(c * SB / (SA * SA)); q.ecoef = (float)(b * SB / SA);
+        sym(q);
         if (back && k == steps - 1) break;
         NnArgs f{}; f.l[0] = B(k); f.r[0] = f.e = X(k); f.out = X(k + 1); f.nseg = 1;
         if (k < steps - 1) { f.acc = (float)(1.0 / SB); f.ecoef = (float)a; hipLaunchKernelGGL((ns_nn_kernel<NS_F32, OUT_PAIR>), nn, blk, 0, s, ws, f, dots); }
@@ -525,10 +702,10 @@ template <int DT> static void ns_launch(int kind, NsProblem& p, const Layout& L,
     for (int k = steps - 1; k >= 0; --k, cur ^= 1) {
         const double gin = sg(k + 1), gout = sg(k), sbound = 2 * P.growth[k + 1] * P.s[k];
         const double ss = pow2_below(16384.0 / sbound), sv = pow2_below(16384.0 / (sbound * P.vgain[k]));
-        SymArgs q{}; q.l[0] = G[cur]; q.r[0] = X(k); q.l[1] = X(k); q.r[1] = G[cur]; q.e = q.out = S; q.nseg = 2; q.k_is_n = 1; q.acc = (float)(ss / (gin * SX));
-        hipLaunchKernelGGL(ns_sym_kernel, sym, blk, 0, s, ws, q);
-        SymArgs v{}; v.l[0] = S; v.r[0] = A(k); v.l[1] = A(k); v.r[1] = S; v.e = S; v.out = V; v.nseg = 2; v.have_e = 1; v.acc = (float)(c * sv / (ss * SA)); v.ecoef = (float)(b * sv / ss);
-        hipLaunchKernelGGL(ns_sym_kernel, sym, blk, 0, s, ws, v);
+        SymArgs q{}; q.l[0] = G[cur]; q.r[0] = X(k); q.l[1] = X(k); q.r[1] = G[cur]; q.e = q.out = S; q.nseg = 2; q.kind = SYM_S; q.acc = (float)(ss / (gin * SX));
+        sym(q);
+        SymArgs v{}; v.l[0] = S; v.r[0] = A(k); v.l[1] = A(k); v.r[1] = S; v.e = S; v.out = V; v.nseg = 2; v.kind = SYM_V; v.have_e = 1; v.acc = (float)(c * sv / (ss * SA)); v.ecoef = (float)(b * sv / ss);
+        sym(v);
         NnArgs f{}; f.l[0] = B(k); f.r[0] = f.e = G[cur]; f.l[1] = V; f.r[1] = X(k); f.out = G[cur ^ 1]; f.x0 = X(0); f.nseg = 2;
         f.mid = (float)(sv * SX / (SB * gin)); f.acc = (float)(gout / (sv * SX)); f.ecoef = (float)(a * gout / gin);
         if (k > 0) hipLaunchKernelGGL((ns_nn_kernel<NS_F32, OUT_PAIR>), nn, blk, 0, s, ws, f, dots);
@@ -542,7 +719,7 @@ int ns_run(int kind, int dtype, const NsMatrices* q, int count, const NsOptions&
     const Plan P = ns_bounds(o.steps, o.coef, kind == NS_BACKWARD);
     if (!P.ok) { *why = P.why; return 2; }
     const int el = dtype == NS_F32 ? 4 : 2;
-    NsProblem p; slots_of(kind, o.steps, p.nX, p.nA);
+    NsProblem p; slots_of(kind, o.steps, p);
     for (int i = 0; i < count; ++i) {
         const NsMatrices& m = q[i];
         if (!m.x || !m.y || (kind != NS_FORWARD && !m.d)) { *why = "null pointer"; return 2; }
