@@ -36,19 +36,19 @@ constexpr int PK_ROWS = 64, PK_COLS = 128;   // tile of the norm / pack kernels
 enum { GRAM = 0, POLY = 1, SYM_S = 2, SYM_V = 3, SYMS = 4 };      // the symmetric products: A = X X^T | B = b A + c A A | S = G X^T + X G^T | V = b S + c (S A + A S)
 constexpr int PART = 64 * 64 * 4;         // unit of the split products' partial sums, bytes
 
-// how one weight (or batch of equal matrices) takes part in one product
-struct Use { int32_t first, red, part, tile, chunk, split; };      // first item, first reduction item, first partial sum, tile side, K blocks per item, items per tile
+// where one weight (or batch of equal matrices) has its part of a product's lists
+struct Use { int32_t first, red, part; };                        // first item, first reduction item, first partial sum
+struct Cut { int32_t tile, chunk; };                             // a product's tile side, and at most how many K blocks an item has: the same for every weight of a call
 // what the host passes per weight, by value
 struct Desc {
     const void* x; const void* d; void* y;                    // matrix | dout | result;  Muon: momentum | gradient | weight
-    int64_t xb, xs, xl, db, ds, dl, yb, ys, yl;               // strides in elements: batch, along the short side, along the long side
     int64_t ws0, ws1;                                         // first matrix's buffers (bytes into the workspace), bytes per matrix
-    int32_t m, n, batch, first, pk0, nn0, nn_tile;            // short side, long side, matrices, index of the first, first work items
-    float alpha;                                              // Muon: lr * shape factor
-    Use sym[SYMS];
+    int32_t m, n, batch, first, pk0, nn0;                     // short side, long side, matrices, index of the first, first work items
+    float alpha; int32_t tall;                                // Muon: lr * shape factor | the short side is the columns
 };
-constexpr int DESCS = 12;                 // 12 * 240 bytes of kernel arguments
-struct DescPack { Desc d[DESCS]; };
+struct Strides { int64_t xb, xs, xl, db, ds, dl; };              // in elements: batch, along the short side, along the long side
+template <int N, int KINDS> struct DescPack { Desc d[N]; Use u[N][KINDS]; };
+constexpr int MUON_DESCS = 38;            // 38 * (72 + 2 * 12) bytes: a set-up launch's arguments stay below 4 KB
 
 // the same per matrix, on the device
 struct Mat {
@@ -67,34 +67,36 @@ struct Ws { Mat* mats; Item *sym[SYMS], *red[SYMS], *nn, *pk; Fac* fac; double* 
 __host__ __device__ inline int cdiv(int a, int b) { return (a + b - 1) / b; }
 __host__ __device__ inline int kblocks(int kind, int m, int n) { return (kind >= SYM_S ? 2 : 1) * cdiv(kind == GRAM || kind == SYM_S ? n : m, 32); }
 
-__global__ __launch_bounds__(256) void ns_setup_kernel(DescPack dp, int dt_bytes, Ws ws) {
-    const Desc& D = dp.d[blockIdx.y];
-    const int mp = cdiv(D.m, PAD) * PAD, np = cdiv(D.n, PAD) * PAD, npk = mp / PK_ROWS * (np / PK_COLS), pr = mp / PK_ROWS, nr = cdiv(D.m, D.nn_tile), nnn = nr * cdiv(D.n, D.nn_tile);
+struct Cuts { Cut sym[SYMS]; int32_t nn_tile; };
+// the tables and work lists of a call, from its weights' descriptions.  N = 1: a batch with strides of its own (and the pullback's products); else contiguous weights
+template <int N, int KINDS> __global__ __launch_bounds__(256) void ns_setup_kernel(DescPack<N, KINDS> dp, Strides st, Cuts cuts, int dt_bytes, Ws ws) {
+    const Desc& D = dp.d[N == 1 ? 0 : blockIdx.y];
+    const int mp = cdiv(D.m, PAD) * PAD, np = cdiv(D.n, PAD) * PAD, npk = mp / PK_ROWS * (np / PK_COLS), pr = mp / PK_ROWS, nr = cdiv(D.m, cuts.nn_tile), nnn = nr * cdiv(D.n, cuts.nn_tile);
     for (int b = blockIdx.x; b < D.batch; b += gridDim.x) {
-        const int id = D.first + b; char* buf = ws.buf + D.ws0 + D.ws1 * b;
+        const int id = D.first + b; char* buf = ws.buf + D.ws0 + D.ws1 * b; const int64_t ss = D.tall ? 1 : D.n, sl = D.tall ? D.m : 1;      // a contiguous matrix's strides
         if (threadIdx.x == 0) {
             Mat M;
-            M.x = (const char*)D.x + D.xb * b * dt_bytes; M.d = (const char*)D.d + D.db * b * dt_bytes; M.y = (char*)D.y + D.yb * b * dt_bytes;
-            M.xs = D.xs; M.xl = D.xl; M.ds = D.ds; M.dl = D.dl; M.ys = D.ys; M.yl = D.yl;
+            M.x = (const char*)D.x + (N == 1 ? st.xb * b * dt_bytes : 0); M.d = (const char*)D.d + (N == 1 ? st.db * b * dt_bytes : 0); M.y = (char*)D.y + (int64_t)D.m * D.n * b * dt_bytes;
+            M.xs = N == 1 ? st.xs : ss; M.xl = N == 1 ? st.xl : sl; M.ds = N == 1 ? st.ds : ss; M.dl = N == 1 ? st.dl : sl; M.ys = ss; M.yl = sl;
             M.buf = buf; M.m = D.m; M.n = D.n; M.mp = mp; M.np = np;
             M.xbytes = (int64_t)mp * np * 4; M.abytes = (int64_t)mp * mp * 4;
             M.pk0 = D.pk0 + npk * b; M.pkn = npk; M.nn0 = D.nn0 + nnn * b; M.nnn = nnn; M.alpha = D.alpha;
             ws.mats[id] = M;
         }
-        for (int kind = 0; kind < SYMS; ++kind) {
-            const Use& u = D.sym[kind];
-            if (!u.tile) continue;
-            const int mt = cdiv(D.m, u.tile), tri = mt * (mt + 1) / 2, kb = kblocks(kind, D.m, D.n), per = u.tile * u.tile * 4 / PART;
+#pragma unroll
+        for (int kind = 0; kind < KINDS; ++kind) {
+            const Use& u = dp.u[N == 1 ? 0 : blockIdx.y][kind]; const Cut cut = cuts.sym[kind];
+            const int mt = cdiv(D.m, cut.tile), tri = mt * (mt + 1) / 2, kb = kblocks(kind, D.m, D.n), per = cut.tile * cut.tile * 4 / PART, chunk = cdiv(kb, cdiv(kb, cut.chunk)), split = cdiv(kb, chunk);
             for (int q = threadIdx.x; q < mt * mt; q += 256) {
                 const int i = q / mt, j = q % mt;
                 if (j < i) continue;
-                const int e = i * mt - i * (i - 1) / 2 + (j - i), part = u.part + (tri * b + e) * u.split * per;
-                for (int k = 0; k < u.split; ++k)
-                    ws.sym[kind][u.first + (tri * b + e) * u.split + k] = Item{buf, D.m, D.n, id, i, j, u.tile, k * u.chunk, min(kb, (k + 1) * u.chunk), u.split > 1 ? part + k * per : -1, 0};
-                if (u.split > 1) ws.red[kind][u.red + tri * b + e] = Item{buf, D.m, D.n, id, i, j, u.tile, 0, u.split, part, 0};
+                const int e = tri * b + i * mt - i * (i - 1) / 2 + (j - i), part = u.part + e * split * per;
+                for (int k = 0; k < split; ++k)
+                    ws.sym[kind][u.first + e * split + k] = Item{buf, D.m, D.n, id, i, j, cut.tile, k * chunk, min(kb, (k + 1) * chunk), split > 1 ? part + k * per : -1, 0};
+                if (split > 1) ws.red[kind][u.red + e] = Item{buf, D.m, D.n, id, i, j, cut.tile, 0, split, part, 0};
             }
         }
-        for (int q = threadIdx.x; q < nnn; q += 256) ws.nn[D.nn0 + nnn * b + q] = Item{buf, D.m, D.n, id, q % nr, q / nr, D.nn_tile, 0, 0, 0, 0};
+        for (int q = threadIdx.x; q < nnn; q += 256) ws.nn[D.nn0 + nnn * b + q] = Item{buf, D.m, D.n, id, q % nr, q / nr, cuts.nn_tile, 0, 0, 0, 0};
         for (int q = threadIdx.x; q < npk; q += 256) ws.pk[D.pk0 + npk * b + q] = Item{buf, D.m, D.n, id, q % pr, q / pr, 0, 0, 0, 0, 0};
     }
 }
@@ -131,36 +133,73 @@ __device__ inline double block_sum(double v, double* red) {
 struct MuonArgs { float beta, gscale; int nesterov; };
 enum { SRC_X = 0, SRC_DOUT = 1, SRC_MUON = 2 };
 
-// One 64 x 128 tile of the source, 8 values of each of the thread's four columns: v[p][e] = element (p * 8 + t / 32, (t % 32) * 4 + e).
-// A source whose short side is the contiguous one goes through LDS, so that either way neighbouring lanes read neighbouring addresses.
-template <int DT, int SRC, bool UPDATE> __device__ inline void load_tile(const Mat& M, const Item& it, const MuonArgs& mu, float v[8][4], float* lds) {
-    const int t = threadIdx.x, i0 = it.ti * PK_ROWS, j0 = it.tj * PK_COLS;
-    const char* src = SRC == SRC_DOUT ? M.d : M.x; const int64_t ss = SRC == SRC_DOUT ? M.ds : M.xs, sl = SRC == SRC_DOUT ? M.dl : M.xl;
-    auto get = [&](int i, int j) -> float {
-        if (i >= M.m || j >= M.n) return 0.f;
-        const int64_t o = i * ss + j * sl;
-        if constexpr (SRC != SRC_MUON) return ld_el<DT>(src, o);
-        else {
-            float* mom = reinterpret_cast<float*>(const_cast<char*>(M.x)); const float g = mu.gscale * reinterpret_cast<const float*>(M.d)[o];
-            float mm = mom[o];
-            if constexpr (UPDATE) { mm = mu.beta * mm + (1.f - mu.beta) * g; mom[o] = mm; }
-            return mu.nesterov ? mu.beta * mm + (1.f - mu.beta) * g : mm;
-        }
-    };
-    if (ss == 1 && sl != 1) {
-        for (int q = 0; q < PK_COLS / 4; ++q) { const int j = q * 4 + (t >> 6), i = t & 63; lds[i * (PK_COLS + 1) + j] = get(i0 + i, j0 + j); }
-        __syncthreads();
+// four neighbouring elements, aligned to their size together
+template <int DT> __device__ inline f32x4 ld_el4(const char* p, int64_t i) {
+    if constexpr (DT == NS_F32) return *reinterpret_cast<const f32x4*>(p + i * 4);
+    else {
+        const s16x4 q = *reinterpret_cast<const s16x4*>(p + i * 2); f32x4 r;
 #pragma unroll
-        for (int p = 0; p < 8; ++p)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[p][e] = lds[(p * 8 + (t >> 5)) * (PK_COLS + 1) + (t & 31) * 4 + e];
-        __syncthreads();
-    } else {
-#pragma unroll
-        for (int p = 0; p < 8; ++p)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[p][e] = get(i0 + p * 8 + (t >> 5), j0 + (t & 31) * 4 + e);
+        for (int e = 0; e < 4; ++e) r[e] = DT == NS_F16 ? (float)__builtin_bit_cast(_Float16, (short)q[e]) : __uint_as_float((uint32_t)(uint16_t)q[e] << 16);
+        return r;
     }
+}
+__device__ inline float momentum_step(float m, float g, const MuonArgs& mu) { return mu.beta * m + (1.f - mu.beta) * (mu.gscale * g); }
+__device__ inline float muon_u(float m, float g, const MuonArgs& mu) { return mu.nesterov ? mu.beta * m + (1.f - mu.beta) * (mu.gscale * g) : m; }
+// One 64 x 128 tile of the source, 8 values of each of the thread's four columns: v[p][e] = element (p * 8 + t / 32, (t % 32) * 4 + e).
+// Rows whose long side is contiguous and aligned are read as vectors; any other source element by element along its contiguous side (neighbouring lanes, neighbouring addresses) and
+// through LDS.  All of a thread's loads are issued before the first is used.  UPDATE: the momentum moves on and is written back.
+template <int DT, int SRC, bool UPDATE> __device__ inline void load_tile(const Mat& M, const Item& it, const MuonArgs& mu, float v[8][4], float* lds) {
+    const int t = threadIdx.x, i0 = it.ti * PK_ROWS, j0 = it.tj * PK_COLS; constexpr int EL = DT == NS_F32 ? 4 : 2;
+    const char* src = SRC == SRC_DOUT ? M.d : M.x; const int64_t ss = SRC == SRC_DOUT ? M.ds : M.xs, sl = SRC == SRC_DOUT ? M.dl : M.xl;
+    float* mom = reinterpret_cast<float*>(const_cast<char*>(M.x));
+    const uintptr_t align = reinterpret_cast<uintptr_t>(src) | (SRC == SRC_MUON ? reinterpret_cast<uintptr_t>(M.d) : 0);
+    if (sl == 1 && align % (4 * EL) == 0 && ss % 4 == 0 && j0 + PK_COLS <= M.n) {
+        f32x4 x[8], g[8]; const int j = j0 + (t & 31) * 4;
+#pragma unroll
+        for (int p = 0; p < 8; ++p) {
+            const int i = i0 + p * 8 + (t >> 5); const int64_t o = i * ss + j;
+            x[p] = i < M.m ? ld_el4<DT>(src, o) : f32x4{0, 0, 0, 0};
+            if constexpr (SRC == SRC_MUON) g[p] = i < M.m ? *reinterpret_cast<const f32x4*>(M.d + o * 4) : f32x4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int p = 0; p < 8; ++p) {
+            const int i = i0 + p * 8 + (t >> 5);
+            if constexpr (SRC == SRC_MUON && UPDATE) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[p][e] = momentum_step(x[p][e], g[p][e], mu);
+                if (i < M.m) *reinterpret_cast<f32x4*>(mom + i * ss + j) = x[p];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[p][e] = SRC == SRC_MUON ? muon_u(x[p][e], g[p][e], mu) : x[p][e];
+        }
+        return;
+    }
+    const bool turn = ss == 1 && sl != 1;
+#pragma unroll 1
+    for (int h = 0; h < 2; ++h) {
+        float x[16], g[16];
+        auto at = [&](int q, int& i, int& j) { const int id = h * 4096 + q * 256 + t; i = turn ? id & 63 : id >> 7; j = turn ? id >> 6 : id & 127; };
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+            int i, j; at(q, i, j); const bool in = i0 + i < M.m && j0 + j < M.n; const int64_t o = (i0 + i) * ss + (j0 + j) * sl;
+            x[q] = in ? ld_el<DT>(src, o) : 0.f;
+            if constexpr (SRC == SRC_MUON) g[q] = in ? reinterpret_cast<const float*>(M.d)[o] : 0.f;
+        }
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+            int i, j; at(q, i, j);
+            if constexpr (SRC == SRC_MUON && UPDATE) {
+                x[q] = momentum_step(x[q], g[q], mu);
+                if (i0 + i < M.m && j0 + j < M.n) mom[(i0 + i) * ss + (j0 + j) * sl] = x[q];
+            }
+            lds[i * (PK_COLS + 1) + j] = SRC == SRC_MUON ? muon_u(x[q], g[q], mu) : x[q];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int p = 0; p < 8; ++p)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[p][e] = lds[(p * 8 + (t >> 5)) * (PK_COLS + 1) + (t & 31) * 4 + e];
 }
 
 // sum of squares of every tile (Muon: after moving the momentum on)
@@ -378,40 +417,48 @@ template <int T> __device__ inline float tile_el(const float* tile, int planes, 
     const int o = tile_at<T>(r, c);
     return T == 64 && planes == 4 ? (tile[o] + tile[4096 + o]) + (tile[8192 + o] + tile[12288 + o]) : tile[o];
 }
-__device__ inline void load_pair8(const char* p, float v[8]) {
-    const f16x8 h = *reinterpret_cast<const f16x8*>(p), l = *reinterpret_cast<const f16x8*>(p + 64);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = (float)h[e] + (float)l[e];
-}
 __device__ inline void store_pair8(char* p, const float v[8]) {
     f16x4 h[2], l[2]; split4(v, h[0], l[0]); split4(v + 4, h[1], l[1]);
     *reinterpret_cast<f16x8*>(p) = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7); *reinterpret_cast<f16x8*>(p + 64) = __builtin_shufflevector(l[0], l[1], 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
 struct SymArgs { Slot l[2], r[2], e, out; int kind, nseg, have_e; float acc, ecoef; };      // out = acc * (sum of l r^T) + ecoef * e, in the buffers' own scales (with e: a factor A too many)
-// the tile (rows: tj's, columns: ti's) to its place and, off the diagonal, to its mirror image's
-template <int T> __device__ inline void sym_finish(const Item& it, const Dims& d, const SymArgs& a, const Fac* facs, const float* tile, int planes) {
-    const int t = threadIdx.x; constexpr int PER = T / 8;        // threads a row
+__device__ inline void unpack8(const f16x8 h, const f16x8 l, float v[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (float)h[e] + (float)l[e];
+}
+// R rows (tj's, from r0) of a tile with T columns (ti's) to their place and, off the diagonal, to their mirror image's; what is read of e is read before anything is written
+template <int T, int R> __device__ inline void sym_finish(const Item& it, const SymArgs& a, const Fac* facs, const float* tile, int planes, int r0) {
+    const int t = threadIdx.x; const Dims d = dims(it);
     char* out = slot(it, d, a.out); const char* E = slot(it, d, a.e); const float facc = a.have_e ? a.acc * facs[it.mat].inv2 : a.acc;
-#pragma unroll 1
-    for (int side = 0; side < (it.ti == it.tj ? 1 : 2); ++side)
-#pragma unroll 2
-        for (int z = 0; z < T * PER / 256; ++z) {
-            const int r = z * (256 / PER) + t / PER, c = (t % PER) * 8; float v[8];
+    constexpr int N = R * T / 8 / 256;                           // groups of 8 values a thread
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+        if (side && it.ti == it.tj) break;
+        f16x8 eh[N], el[N]; int64_t off[N];
+#pragma unroll
+        for (int z = 0; z < N; ++z) {
+            const int id = z * 256 + t, r = side ? id / (R / 8) : id / (T / 8), c = side ? id % (R / 8) * 8 : id % (T / 8) * 8;
+            off[z] = pair_off(d.arb, side ? it.ti * T + r : it.tj * T + r0 + r, side ? it.tj * T + r0 + c : it.ti * T + c);
+            if (a.have_e) { eh[z] = *reinterpret_cast<const f16x8*>(E + off[z]); el[z] = *reinterpret_cast<const f16x8*>(E + off[z] + 64); }
+        }
+#pragma unroll
+        for (int z = 0; z < N; ++z) {
+            const int id = z * 256 + t, r = side ? id / (R / 8) : id / (T / 8), c = side ? id % (R / 8) * 8 : id % (T / 8) * 8; float v[8];
             if (side == 0) tile_row8<T>(tile, planes, r, c, v);
             else
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] = tile_el<T>(tile, planes, c + e, r);
-            const int64_t o = pair_off(d.arb, (side ? it.ti : it.tj) * T + r, (side ? it.tj : it.ti) * T + c);
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] *= facc;
             if (a.have_e) {
-                float x[8]; load_pair8(E + o, x);
+                float x[8]; unpack8(eh[z], el[z], x);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] += a.ecoef * x[e];
             }
-            store_pair8(out + o, v);
+            store_pair8(out + off[z], v);
         }
+    }
 }
 template <int T> __device__ inline void sym_tile(char* lds, const Item& it, const Ws& ws, const SymArgs& a) {
     const Dims d = dims(it); const bool kn = a.kind == GRAM || a.kind == SYM_S; const int64_t rb = kn ? d.xrb : d.arb;
@@ -421,7 +468,7 @@ template <int T> __device__ inline void sym_tile(char* lds, const Item& it, cons
     f32x16 c[2][2] = {};
     product<T, false>(lds, seg, a.nseg == 2 ? cdiv(kn ? it.n : it.m, 32) : 1 << 30, it.k0, it.k1, 1.f, c);
     float* tile = reinterpret_cast<float*>(lds); tile_store<T>(tile, c);
-    if (it.part < 0) sym_finish<T>(it, d, a, ws.fac, tile, 4);
+    if (it.part < 0) sym_finish<T, T>(it, a, ws.fac, tile, 4, 0);
     else {
         constexpr int PER = T / 8; float* out = reinterpret_cast<float*>(ws.split + (int64_t)it.part * PART);
 #pragma unroll 2
@@ -437,25 +484,27 @@ __global__ __launch_bounds__(256, 2) void ns_sym_kernel(Ws ws, SymArgs a) {
     const Item it = ws.sym[a.kind][blockIdx.x];
     if (it.tile == 128) sym_tile<128>(lds, it, ws, a); else sym_tile<64>(lds, it, ws, a);
 }
-// the shares of a tile, summed in order
-template <int T> __device__ inline void reduce_tile(float* tile, const Item& it, const Ws& ws, const SymArgs& a) {
-    constexpr int PER = T / 8; const float* in = reinterpret_cast<const float*>(ws.split + (int64_t)it.part * PART);
-#pragma unroll 2
-    for (int z = 0; z < T * PER / 256; ++z) {
-        const int r = z * (256 / PER) + threadIdx.x / PER, col = (threadIdx.x % PER) * 8; f32x4 v[2] = {};
-        for (int k = 0; k < it.k1; ++k)
+// the shares of a tile, summed in order: 32 rows of it a workgroup
+template <int T> __device__ inline void reduce_tile(float* tile, const Item& it, const Ws& ws, const SymArgs& a, int r0) {
+    constexpr int N = 32 * T / 8 / 256; const float* in = reinterpret_cast<const float*>(ws.split + (int64_t)it.part * PART) + r0 * T + threadIdx.x * 8;
+    f32x4 v[N][2] = {};
+#pragma unroll 4
+    for (int k = 0; k < it.k1; ++k)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) v[h] += *reinterpret_cast<const f32x4*>(in + (int64_t)k * T * T + r * T + col + h * 4);
+        for (int z = 0; z < N; ++z)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) *reinterpret_cast<f32x4*>(tile + tile_at<T>(r, col + h * 4)) = v[h];
-    }
+            for (int h = 0; h < 2; ++h) v[z][h] += *reinterpret_cast<const f32x4*>(in + (int64_t)k * T * T + z * 2048 + h * 4);
+#pragma unroll
+    for (int z = 0; z < N; ++z)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) *reinterpret_cast<f32x4*>(tile + tile_at<T>((z * 256 + threadIdx.x) / (T / 8), threadIdx.x % (T / 8) * 8 + h * 4)) = v[z][h];
     __syncthreads();
-    sym_finish<T>(it, dims(it), a, ws.fac, tile, 1);
+    sym_finish<T, 32>(it, a, ws.fac, tile, 1, r0);
 }
-__global__ __launch_bounds__(256) void ns_reduce_kernel(Ws ws, SymArgs a) {
-    __shared__ __attribute__((aligned(16))) float tile[128 * 128];
-    const Item it = ws.red[a.kind][blockIdx.x];
-    if (it.tile == 128) reduce_tile<128>(tile, it, ws, a); else reduce_tile<64>(tile, it, ws, a);
+template <int T> __global__ __launch_bounds__(256) void ns_reduce_kernel(Ws ws, SymArgs a) {
+    __shared__ __attribute__((aligned(16))) float tile[32 * T];
+    const Item it = ws.red[a.kind][blockIdx.x / (T / 32)];
+    reduce_tile<T>(tile, it, ws, a, blockIdx.x % (T / 32) * 32);
 }
 
 enum { OUT_PAIR = 0, OUT_Y = 1, OUT_MUON = 2, OUT_BACK = 3 };
@@ -468,23 +517,43 @@ template <int T, int DT, int OUT> __device__ inline void nn_tile(char* lds, doub
     for (int s = 0; s < 2; ++s) seg[s] = Seg{slot(it, d, a.r[s]) + (int64_t)it.tj * T * 4, slot(it, d, a.l[s]) + (int64_t)it.ti * T * d.arb, d.xrb, d.arb, 32 * d.xrb, 128};
     f32x16 c[2][2] = {};
     product<T, true>(lds, seg, a.nseg == 2 ? kb : 1 << 30, 0, a.nseg * kb, a.mid, c);
+    // everything the epilogue reads is read before it writes anything: the loads are in flight together
+    constexpr int N = T * T / 8 / 256; const char* E = slot(it, d, a.e); double dot = 0;
+    f16x8 eh[N], el[N], xh[N], xl[N]; f32x4 P[N][2]; int64_t off[N];
+    const Mat* M = &ws.mats[it.mat]; float* Y = OUT == OUT_MUON ? reinterpret_cast<float*>(M->y) : nullptr; int64_t ys = 0; bool rows = false;      // rows: the weight's rows as vectors
+    if constexpr (OUT == OUT_MUON) { ys = M->ys; rows = M->yl == 1 && reinterpret_cast<uintptr_t>(Y) % 16 == 0 && ys % 4 == 0 && it.tj * T + T <= it.n; }
+#pragma unroll
+    for (int z = 0; z < N; ++z) {
+        const int r = (z * 256 + t) / (T / 8), col = t % (T / 8) * 8, i = it.ti * T + r, j = it.tj * T + col;
+        off[z] = pair_off(d.xrb, i, j);
+        eh[z] = *reinterpret_cast<const f16x8*>(E + off[z]); el[z] = *reinterpret_cast<const f16x8*>(E + off[z] + 64);
+        if constexpr (OUT == OUT_BACK) { xh[z] = *reinterpret_cast<const f16x8*>(slot(it, d, a.x0) + off[z]); xl[z] = *reinterpret_cast<const f16x8*>(slot(it, d, a.x0) + off[z] + 64); }
+        if constexpr (OUT == OUT_MUON)
+            if (rows && i < it.m) { P[z][0] = *reinterpret_cast<const f32x4*>(Y + i * ys + j); P[z][1] = *reinterpret_cast<const f32x4*>(Y + i * ys + j + 4); }
+    }
     float* tile = reinterpret_cast<float*>(lds); tile_store<T>(tile, c);
-    constexpr int PER = T / 8; const char* E = slot(it, d, a.e); double dot = 0;
-#pragma unroll 2
-    for (int z = 0; z < T * PER / 256; ++z) {
-        const int r = z * (256 / PER) + t / PER, col = (t % PER) * 8; float v[8], x[8];
+#pragma unroll
+    for (int z = 0; z < N; ++z) {
+        const int r = (z * 256 + t) / (T / 8), col = t % (T / 8) * 8, i = it.ti * T + r, j = it.tj * T + col; float v[8], x[8];
         tile_row8<T>(tile, 4, r, col, v);
-        const int64_t o = pair_off(d.xrb, it.ti * T + r, it.tj * T + col);
-        load_pair8(E + o, x);
+        unpack8(eh[z], el[z], x);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = facc * v[e] + a.ecoef * x[e];
-        if constexpr (OUT == OUT_PAIR) store_pair8(slot(it, d, a.out) + o, v);
+        if constexpr (OUT == OUT_PAIR) store_pair8(slot(it, d, a.out) + off[z], v);
         else if constexpr (OUT == OUT_BACK) {                    // G in fp32, and this tile's share of <X0, G>
-            load_pair8(slot(it, d, a.x0) + o, x);
+            unpack8(xh[z], xl[z], x);
 #pragma unroll
             for (int e = 0; e < 8; ++e) dot += (double)x[e] * (double)v[e];
-            float* w = reinterpret_cast<float*>(slot(it, d, a.out) + (it.ti * T + r) * d.xrb + (int64_t)(it.tj * T + col) * 4);
+            float* w = reinterpret_cast<float*>(slot(it, d, a.out) + i * d.xrb + (int64_t)j * 4);
             *reinterpret_cast<f32x4*>(w) = f32x4{v[0], v[1], v[2], v[3]}; *reinterpret_cast<f32x4*>(w + 4) = f32x4{v[4], v[5], v[6], v[7]};
+        } else if (OUT == OUT_MUON && rows) {
+            if (i < it.m)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) P[z][h][e] = a.decay * P[z][h][e] - M->alpha * ldexpf(v[h * 4 + e], -fac.q);
+                    *reinterpret_cast<f32x4*>(Y + i * ys + j + h * 4) = P[z][h];
+                }
         } else {
 #pragma unroll
             for (int h = 0; h < 2; ++h) *reinterpret_cast<f32x4*>(tile + tile_at<T>(r, col + h * 4)) = f32x4{v[h * 4], v[h * 4 + 1], v[h * 4 + 2], v[h * 4 + 3]};
@@ -494,16 +563,23 @@ template <int T, int DT, int OUT> __device__ inline void nn_tile(char* lds, doub
         dot = block_sum(dot, red);
         if (t == 0) dots[blockIdx.x] = dot;
     }
-    if constexpr (OUT == OUT_Y || OUT == OUT_MUON) {             // element by element, neighbouring lanes along whichever axis is contiguous in the caller's memory
-        const Mat& M = ws.mats[it.mat]; const bool turn = M.ys == 1 && M.yl != 1;
+    if constexpr (OUT == OUT_Y || OUT == OUT_MUON) if (!rows) {  // element by element, neighbouring lanes along whichever axis is contiguous in the caller's memory
+        const bool turn = M->ys == 1 && M->yl != 1; const int64_t yl = M->yl, yS = M->ys; char* y = M->y; const float alpha = M->alpha;
         __syncthreads();
-#pragma unroll 4
-        for (int z = 0; z < T * T / 256; ++z) {
-            const int q = z * 256 + t, r = turn ? q % T : q / T, col = turn ? q / T : q % T, i = it.ti * T + r, j = it.tj * T + col;
-            if (i < it.m && j < it.n) {
-                const float v = ldexpf(tile[tile_at<T>(r, col)], -fac.q); const int64_t o = i * M.ys + j * M.yl;
-                if constexpr (OUT == OUT_Y) st_el<DT>(M.y, o, v);
-                else { float* P = reinterpret_cast<float*>(M.y) + o; *P = a.decay * *P - M.alpha * v; }
+#pragma unroll 1
+        for (int b = 0; b < T * T / 256; b += 16) {
+            float old[16]; int64_t o[16];
+#pragma unroll
+            for (int z = 0; z < 16; ++z) {
+                const int q = (b + z) * 256 + t, r = turn ? q % T : q / T, col = turn ? q / T : q % T, i = it.ti * T + r, j = it.tj * T + col;
+                o[z] = i < it.m && j < it.n ? i * yS + j * yl : -1;
+                if constexpr (OUT == OUT_MUON) old[z] = o[z] >= 0 ? reinterpret_cast<float*>(y)[o[z]] : 0.f;
+            }
+#pragma unroll
+            for (int z = 0; z < 16; ++z) {
+                const int q = (b + z) * 256 + t, r = turn ? q % T : q / T, col = turn ? q / T : q % T;
+                const float v = ldexpf(tile[tile_at<T>(r, col)], -fac.q);
+                if (o[z] >= 0) { if constexpr (OUT == OUT_Y) st_el<DT>(y, o[z], v); else reinterpret_cast<float*>(y)[o[z]] = a.decay * old[z] - alpha * v; }
             }
         }
     }
@@ -580,38 +656,47 @@ struct Layout { int64_t mats, sym[SYMS], red[SYMS], nn, pk, fac, part, split, bu
 
 }  // namespace
 
-struct NsProblem { std::vector<Desc> d; int nX, nA, kinds; };
+struct NsProblem { std::vector<Desc> d; std::vector<Use> u; Strides st{}; int nX, nA, kinds; Cuts cuts{}; };      // u: [weight][kinds]
 
-// Tiles and splits of a call's products.
-// 128-tiles share each staged row among two waves and are the faster ones where they fill the chip; with fewer than FILL of them (counting a long K axis cut into pieces of 256) a product takes
-// 64-tiles, whose four waves split K.  A K axis is then cut so that about FILL workgroups (two a CU) have the work between them, never below MIN_BLOCKS blocks of 32 an item.
-static constexpr int FILL = 512, MIN_BLOCKS = 8;
+// Tiles and splits of a call's products, from its sizes alone.
+// 128-tiles share a staged row between two waves (half the loads of 64-tiles, whose four waves split K instead), so they are taken wherever they occupy half the CUs, counting a long K axis
+// as pieces of MIN128 blocks of 32.  The K axis is cut where that makes the launch shorter by this model: a CU has its share of the workgroups, a step of one costs STEP us (the rate of two a CU), and
+// a cut K axis costs a second launch and its partial sums' way to memory and back.
+static constexpr int CUS = 256, MIN128 = 8, MIN64 = 32;
+static constexpr double STEP = 0.8, LAUNCH = 6.0, PART_US = 64.0 * 1024 * 2 / 3.0e6;      // us; a 64 KB partial sum written and read at 3 TB/s
 static int64_t tri(int64_t m, int tile) { const int64_t t = (m + tile - 1) / tile; return t * (t + 1) / 2; }
 static Layout ns_layout(NsProblem& p) {
-    Layout L{};
+    Layout L{}; p.u.assign(p.d.size() * p.kinds, Use{});
     int64_t buf = 0, split_max = 0;
     for (int kind = 0; kind < p.kinds; ++kind) {
-        int64_t pieces = 0, work = 0, part = 0;
-        for (const Desc& d : p.d) pieces += d.batch * tri(d.m, 128) * ((kblocks(kind, d.m, d.n) + 7) / 8);
-        const int tile = pieces >= FILL / 2 ? 128 : 64;
-        for (const Desc& d : p.d) work += d.batch * tri(d.m, tile) * kblocks(kind, d.m, d.n);
-        const int64_t chunk = std::max<int64_t>(MIN_BLOCKS, (work + FILL - 1) / FILL);
-        for (Desc& d : p.d) {
-            Use& u = d.sym[kind]; const int64_t kb = kblocks(kind, d.m, d.n), tiles = d.batch * tri(d.m, tile);
-            u.tile = tile; u.split = (int)((kb + chunk - 1) / chunk); u.chunk = (int)((kb + u.split - 1) / u.split); u.split = (int)((kb + u.chunk - 1) / u.chunk);
-            u.first = (int)L.n_sym[kind]; u.red = (int)L.n_red[kind]; u.part = (int)part;
-            L.n_sym[kind] += tiles * u.split;
-            if (u.split > 1) { L.n_red[kind] += tiles; part += tiles * u.split * (tile * tile * 4 / PART); }
+        int64_t pieces = 0, part = 0; int most = 1;
+        for (const Desc& d : p.d) { const int kb = kblocks(kind, d.m, d.n); pieces += d.batch * tri(d.m, 128) * cdiv(kb, MIN128); most = std::max(most, kb); }
+        const int tile = pieces >= CUS / 2 ? 128 : 64, least = tile == 128 ? MIN128 : MIN64;
+        int chunk = most; double best = 1e30;
+        for (int c = most;; c = std::max(least, std::min(c - 1, c * 7 / 8))) {
+            int64_t items = 0, parts = 0; 
+            for (const Desc& d : p.d) { const int64_t t = d.batch * tri(d.m, tile), sp = cdiv(kblocks(kind, d.m, d.n), c); items += t * sp; if (sp > 1) parts += t * sp; }
+            const double us = (double)((items + CUS - 1) / CUS) * std::min(c, most) * STEP / (tile == 128 ? 1 : 4) + (parts ? LAUNCH : 0) + parts * PART_US / (tile == 128 ? 1 : 4);
+            if (us < best) { best = us; chunk = c; }
+            if (c <= least) break;
+        }
+        p.cuts.sym[kind] = Cut{tile, chunk};
+        for (size_t i = 0; i < p.d.size(); ++i) {
+            const Desc& d = p.d[i]; Use& u = p.u[i * p.kinds + kind]; const int kb = kblocks(kind, d.m, d.n), split = cdiv(kb, cdiv(kb, cdiv(kb, chunk))); const int64_t tiles = d.batch * tri(d.m, tile);
+            u = Use{(int)L.n_sym[kind], (int)L.n_red[kind], (int)part};
+            L.n_sym[kind] += tiles * split;
+            if (split > 1) { L.n_red[kind] += tiles; part += tiles * split * (tile * tile * 4 / PART); }
         }
         split_max = std::max(split_max, part);
     }
     int64_t nn128 = 0;
     for (const Desc& d : p.d) nn128 += (int64_t)d.batch * cdiv(d.m, 128) * cdiv(d.n, 128);
+    p.cuts.nn_tile = nn128 >= CUS / 2 ? 128 : 64;
     for (Desc& d : p.d) {
         const int64_t mt = cdiv(d.m, PAD), nt = cdiv(d.n, PAD);
-        d.first = (int)L.n_mats; d.nn0 = (int)L.n_nn; d.pk0 = (int)L.n_pk; d.nn_tile = nn128 >= FILL / 2 ? 128 : 64;
+        d.first = (int)L.n_mats; d.nn0 = (int)L.n_nn; d.pk0 = (int)L.n_pk;
         d.ws0 = buf; d.ws1 = (p.nX * mt * nt + p.nA * mt * mt) * (int64_t)PAD * PAD * 4;
-        L.n_mats += d.batch; L.n_nn += (int64_t)cdiv(d.m, d.nn_tile) * cdiv(d.n, d.nn_tile) * d.batch; L.n_pk += mt * (PAD / PK_ROWS) * nt * (PAD / PK_COLS) * d.batch;
+        L.n_mats += d.batch; L.n_nn += (int64_t)cdiv(d.m, p.cuts.nn_tile) * cdiv(d.n, p.cuts.nn_tile) * d.batch; L.n_pk += mt * (PAD / PK_ROWS) * nt * (PAD / PK_COLS) * d.batch;
         buf += d.ws1 * d.batch;
     }
     int64_t at = 0;
@@ -633,10 +718,7 @@ static int64_t check_total(const Layout& L) {
 static Desc make_desc(const NsMatrices& q) {
     Desc d{}; const bool tall = q.rows > q.cols;
     d.x = q.x; d.d = q.d; d.y = q.y; d.m = (int)std::min(q.rows, q.cols); d.n = (int)std::max(q.rows, q.cols); d.batch = (int)q.batch;
-    d.xb = q.xs[0]; d.xs = q.xs[tall ? 2 : 1]; d.xl = q.xs[tall ? 1 : 2];
-    d.db = q.ds[0]; d.ds = q.ds[tall ? 2 : 1]; d.dl = q.ds[tall ? 1 : 2];
-    d.yb = q.rows * q.cols; d.ys = tall ? 1 : q.cols; d.yl = tall ? q.cols : 1;
-    d.alpha = q.alpha;
+    d.alpha = q.alpha; d.tall = tall;
     return d;
 }
 static void slots_of(int kind, int steps, NsProblem& p) {
@@ -648,21 +730,30 @@ int64_t ns_workspace(int kind, int steps, const NsMatrices* q, int count) {
     if (steps < 1 || steps > MD2_NS_MAX_STEPS) return -1;
     NsProblem p; slots_of(kind, steps, p);
     for (int i = 0; i < count; ++i) { if (!fits(q[i].batch, q[i].rows, q[i].cols)) return -1; p.d.push_back(make_desc(q[i])); }
+    std::stable_sort(p.d.begin(), p.d.end(), [](const Desc& a, const Desc& b) { return a.m > b.m; });
     return check_total(ns_layout(p));
 }
 
 template <int DT> static void ns_launch(int kind, NsProblem& p, const Layout& L, char* base, const NsOptions& o, const Plan& P, hipStream_t s) {
     Ws ws; ws.mats = (Mat*)(base + L.mats); for (int k = 0; k < SYMS; ++k) { ws.sym[k] = (Item*)(base + L.sym[k]); ws.red[k] = (Item*)(base + L.red[k]); } ws.nn = (Item*)(base + L.nn); ws.pk = (Item*)(base + L.pk); ws.fac = (Fac*)(base + L.fac); ws.part = (double*)(base + L.part); ws.split = base + L.split; ws.buf = base + L.buf;
     const int bytes = DT == NS_F32 ? 4 : 2, steps = o.steps;
-    for (size_t i = 0; i < p.d.size(); i += DESCS) {
-        DescPack dp; const int n = (int)std::min<size_t>(DESCS, p.d.size() - i); int most = 1;
-        for (int k = 0; k < n; ++k) { dp.d[k] = p.d[i + k]; most = std::max(most, dp.d[k].batch); }
-        hipLaunchKernelGGL(ns_setup_kernel, dim3(std::min(most, 256), n), dim3(256), 0, s, dp, bytes, ws);
+    if (kind == NS_MUON)
+        for (size_t i = 0; i < p.d.size(); i += MUON_DESCS) {
+            DescPack<MUON_DESCS, 2> dp; const int n = (int)std::min<size_t>(MUON_DESCS, p.d.size() - i);
+            for (int k = 0; k < n; ++k) { dp.d[k] = p.d[i + k]; for (int u = 0; u < 2; ++u) dp.u[k][u] = p.u[(i + k) * 2 + u]; }
+            hipLaunchKernelGGL((ns_setup_kernel<MUON_DESCS, 2>), dim3(1, n), dim3(256), 0, s, dp, p.st, p.cuts, bytes, ws);
+        }
+    else {
+        const dim3 grid(std::min(p.d[0].batch, 1024));
+        if (kind == NS_BACKWARD) { DescPack<1, 4> dp; dp.d[0] = p.d[0]; for (int u = 0; u < 4; ++u) dp.u[0][u] = p.u[u]; hipLaunchKernelGGL((ns_setup_kernel<1, 4>), grid, dim3(256), 0, s, dp, p.st, p.cuts, bytes, ws); }
+        else { DescPack<1, 2> dp; dp.d[0] = p.d[0]; for (int u = 0; u < 2; ++u) dp.u[0][u] = p.u[u]; hipLaunchKernelGGL((ns_setup_kernel<1, 2>), grid, dim3(256), 0, s, dp, p.st, p.cuts, bytes, ws); }
     }
     const dim3 blk(256), pk((unsigned)L.n_pk), nn((unsigned)L.n_nn);
     auto sym = [&](const SymArgs& a) {
         hipLaunchKernelGGL(ns_sym_kernel, dim3((unsigned)L.n_sym[a.kind]), blk, 0, s, ws, a);
-        if (L.n_red[a.kind]) hipLaunchKernelGGL(ns_reduce_kernel, dim3((unsigned)L.n_red[a.kind]), blk, 0, s, ws, a);
+        if (!L.n_red[a.kind]) return;
+        if (p.cuts.sym[a.kind].tile == 128) hipLaunchKernelGGL((ns_reduce_kernel<128>), dim3((unsigned)L.n_red[a.kind] * 4), blk, 0, s, ws, a);
+        else hipLaunchKernelGGL((ns_reduce_kernel<64>), dim3((unsigned)L.n_red[a.kind] * 2), blk, 0, s, ws, a);
     };
     const MuonArgs mu{(float)o.momentum, o.grad_scale, o.nesterov};
     double *xpart = ws.part, *dpart = ws.part + L.n_pk, *dots = ws.part + 2 * L.n_pk;
@@ -728,6 +819,8 @@ int ns_run(int kind, int dtype, const NsMatrices* q, int count, const NsOptions&
         for (int k = 0; k < 3; ++k) if (m.xs[k] < 0 || m.ds[k] < 0) { *why = "negative stride"; return 2; }
         p.d.push_back(make_desc(m));
     }
+    if (kind != NS_MUON) { const bool tall = p.d[0].tall; const int64_t *x = q[0].xs, *d = q[0].ds; p.st = Strides{x[0], x[tall ? 2 : 1], x[tall ? 1 : 2], d[0], d[tall ? 2 : 1], d[tall ? 1 : 2]}; }
+    std::stable_sort(p.d.begin(), p.d.end(), [](const Desc& a, const Desc& b) { return a.m > b.m; });      // the longest work items first
     const Layout L = ns_layout(p);
     if (check_total(L) < 0) { *why = "too many matrices"; return 2; }
     if (!wsp || (uintptr_t)wsp % 256 || ws_bytes < L.total) { *why = "the workspace is missing, too small or not aligned to 256 bytes"; return 2; }
