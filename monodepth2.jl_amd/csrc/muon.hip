@@ -14,7 +14,7 @@
 // sixteenth.  The pairs are scaled by powers of two that come from bounds of the iterates' norms (ns_plan), so that no hi overflows and the lo of a typical entry is a normal number.
 // a X is added in fp32 in the epilogue: inside B (B + a I) its rounding would be the largest error of all.  Norms are sums in 64 bits.
 //
-// Layout.  A pair matrix is row-major in blocks of 32 columns, 128 bytes each: 32 hi, then 32 lo -- one cache line holds what an MFMA K-step reads of a row.  Rows are padded to 128,
+// Layout.  A pair matrix is row-major in blocks of 16 columns, 64 bytes each: 16 hi, then 16 lo -- what an MFMA K-step reads of a row is contiguous.  Rows are padded to 128,
 // columns of X to 128, with zeros that every step keeps (rows of B beyond m are 0), so the products need no bounds checks.
 #include "md2_internal.h"
 #include "muon.h"
@@ -65,9 +65,15 @@ struct Fac { float inv2; int q; };                             // a clamped matr
 struct Ws { Mat* mats; Item *sym[SYMS], *red[SYMS], *nn, *pk; Fac* fac; double* part; char* split; char* buf; };      // part: [2][pk items] sums of squares of x, of dout, and [nn items] of X0 G
 
 __host__ __device__ inline int cdiv(int a, int b) { return (a + b - 1) / b; }
-__host__ __device__ inline int kblocks(int kind, int m, int n) { return (kind >= SYM_S ? 2 : 1) * cdiv(kind == GRAM || kind == SYM_S ? n : m, 32); }
+__host__ __device__ inline int kblocks(int kind, int m, int n) { return (kind >= SYM_S ? 2 : 1) * cdiv(kind == GRAM || kind == SYM_S ? n : m, 16); }
 
 struct Cuts { Cut sym[SYMS]; int32_t nn_tile; };
+// Workgroup b runs on XCD b % 8, each with an L2 of its own.  Of `groups` groups of `size` items, the items of one share an operand: eight groups at a time are dealt to the XCDs, a group
+// to one.  -> the place of item `i` of group `g` (the last groups, fewer than eight, are dealt among themselves)
+__device__ inline int dealt(int g, int i, int groups, int size) {
+    const int full = groups / 8 * 8, r = groups - full;
+    return g < full ? g / 8 * 8 * size + i * 8 + g % 8 : full * size + i * r + (g - full);
+}
 // the tables and work lists of a call, from its weights' descriptions.  N = 1: a batch with strides of its own (and the pullback's products); else contiguous weights
 template <int N, int KINDS> __global__ __launch_bounds__(256) void ns_setup_kernel(DescPack<N, KINDS> dp, Strides st, Cuts cuts, int dt_bytes, Ws ws) {
     const Desc& D = dp.d[N == 1 ? 0 : blockIdx.y];
@@ -90,13 +96,13 @@ template <int N, int KINDS> __global__ __launch_bounds__(256) void ns_setup_kern
             for (int q = threadIdx.x; q < mt * mt; q += 256) {
                 const int i = q / mt, j = q % mt;
                 if (j < i) continue;
-                const int e = tri * b + i * mt - i * (i - 1) / 2 + (j - i), part = u.part + e * split * per;
-                for (int k = 0; k < split; ++k)
-                    ws.sym[kind][u.first + e * split + k] = Item{buf, D.m, D.n, id, i, j, cut.tile, k * chunk, min(kb, (k + 1) * chunk), split > 1 ? part + k * per : -1, 0};
+                const int own = i * mt - i * (i - 1) / 2 + (j - i), e = tri * b + own, part = u.part + e * split * per;
+                for (int k = 0; k < split; ++k)      // (the tiles of one piece of the K axis read the same columns)
+                    ws.sym[kind][u.first + tri * b * split + dealt(k, own, split, tri)] = Item{buf, D.m, D.n, id, i, j, cut.tile, k * chunk, min(kb, (k + 1) * chunk), split > 1 ? part + k * per : -1, 0};
                 if (split > 1) ws.red[kind][u.red + e] = Item{buf, D.m, D.n, id, i, j, cut.tile, 0, split, part, 0};
             }
         }
-        for (int q = threadIdx.x; q < nnn; q += 256) ws.nn[D.nn0 + nnn * b + q] = Item{buf, D.m, D.n, id, q % nr, q / nr, cuts.nn_tile, 0, 0, 0, 0};
+        for (int q = threadIdx.x; q < nnn; q += 256) ws.nn[D.nn0 + nnn * b + dealt(q / nr, q % nr, nnn / nr, nr)] = Item{buf, D.m, D.n, id, q % nr, q / nr, cuts.nn_tile, 0, 0, 0, 0};
         for (int q = threadIdx.x; q < npk; q += 256) ws.pk[D.pk0 + npk * b + q] = Item{buf, D.m, D.n, id, q % pr, q / pr, 0, 0, 0, 0, 0};
     }
 }
@@ -118,7 +124,8 @@ __device__ inline void split4(const float v[4], f16x4& hi, f16x4& lo) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) { float x = v[e]; asm("" : "+v"(x)); hi[e] = (_Float16)x; lo[e] = (_Float16)(x - (float)hi[e]); }
 }
-__device__ inline int64_t pair_off(int64_t row_bytes, int i, int j) { return i * row_bytes + (j >> 5) * 128 + (j & 31) * 2; }      // bytes of hi(i, j); lo is 64 behind it
+constexpr int LO = 32;                    // bytes from a hi to its lo
+__device__ inline int64_t pair_off(int64_t row_bytes, int i, int j) { return i * row_bytes + (j >> 4) * 64 + (j & 15) * 2; }      // bytes of hi(i, j)
 
 // sum over the block in a fixed order (256 threads); every thread gets it
 __device__ inline double block_sum(double v, double* red) {
@@ -245,7 +252,7 @@ template <int DT, int SRC> __global__ __launch_bounds__(256) void ns_pack_kernel
         for (int e = 0; e < 4; ++e) w[e] = ldexpf(v[p][e], fe) * f;
         split4(w, hi, lo);
         char* o = out + pair_off(rb, it.ti * PK_ROWS + p * 8 + (threadIdx.x >> 5), it.tj * PK_COLS + (threadIdx.x & 31) * 4);
-        *reinterpret_cast<f16x4*>(o) = hi; *reinterpret_cast<f16x4*>(o + 64) = lo;
+        *reinterpret_cast<f16x4*>(o) = hi; *reinterpret_cast<f16x4*>(o + LO) = lo;
     }
 }
 
@@ -261,117 +268,120 @@ __device__ inline char* slot(const Item& it, const Dims& d, Slot s) { return it.
 
 typedef const __attribute__((address_space(1))) void* glb_t;
 typedef __attribute__((address_space(3))) void* lds_t;
-constexpr int STAGE = 16384;              // bytes of LDS one staged operand takes: 128 rows (or columns) x 32 K of pairs, or four waves' 64 x 32 of their own
-constexpr int LDS_BYTES = 4 * STAGE;      // 128-tiles: two operands, double buffered.  64-tiles: two operands, four waves.  Epilogue: a 128 x 128 fp32 tile, or four 64 x 64
+// LDS of a product: RING stages of 16 K of both operands.  128-tiles: shared by the workgroup, 16 KB each, so that two workgroups share a CU; 64-tiles: each wave's own, 8 KB each
+template <int T> struct Ring { static constexpr int N = T == 128 ? 5 : 4, STAGE = T == 128 ? 16384 : 8192, THREADS = T == 128 ? 256 : 64, LOADS = STAGE / THREADS / 32, BYTES = T == 128 ? N * STAGE : 4 * N * STAGE; };      // LOADS: a wave's instructions per stage and operand
 
-// Direct loads (global memory -> LDS, 16 bytes a lane; a wave writes 1 KB in lane order, so the bank swizzle is in which chunk a lane FETCHES).
-// Rows: ROWS x 32 columns of a pair matrix; row r's eight 16-byte chunks (hi k 0..7, 8..15, 16..23, 24..31, then lo) are stored at chunk ^ (r & 7), so that eight neighbouring rows'
-// reads of one chunk meet eight different bank groups.
-template <int ROWS, int THREADS> __device__ inline void stage_rows(char* lds, const char* src, int64_t rb, int tid) {
+// Direct loads (global memory -> LDS, 16 bytes a lane; a wave writes 1 KB in lane order, so the bank swizzle is in which chunk a lane FETCHES).  Written as assembly because the compiler
+// lets a transposed LDS read wait for every direct load in flight that it knows of; it has no register result, and the product counts and waits itself.
+__device__ inline void direct_load(unsigned lds, const char* base, unsigned off) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(lds), "v"(off), "s"(base) : "memory");
+}
+// Rows: T x 16 columns of a pair matrix; row r's four 16-byte chunks (hi k 0..7, 8..15, lo 0..7, 8..15) are stored at chunk ^ row_swizzle(r), which spreads neighbouring rows' reads of one
+// chunk over the 64 banks (four rows wide).
+__device__ inline int row_swizzle(int r) { return ((r >> 2) & 1) | ((((r >> 1) ^ (r >> 3)) & 1) << 1); }
+// Columns: 16 rows (the K axis) x T columns; a row's 32-byte units are stored at unit ^ col_swizzle(k), so that the four rows and two units of 32 lanes' transposed read meet eight
+// different places of the 64 banks
+__device__ inline int col_swizzle(int k) { return (k & 1) | (((k >> 1) & 1) << 2) | (((k >> 3) & 1) << 1); }
+// a lane's bytes behind the stage's first, per instruction
+template <int T, bool COLS> __device__ inline void lane_offsets(unsigned off[Ring<T>::LOADS], int64_t rb, int tid) {
 #pragma unroll
-    for (int q = 0; q < ROWS * 8 / THREADS; ++q) {
-        const int id = q * THREADS + tid, r = id >> 3, c = (id & 7) ^ (r & 7);
-        __builtin_amdgcn_global_load_lds((glb_t)(src + r * rb + c * 16), (lds_t)(lds + q * THREADS * 16 + (tid & ~63) * 16), 16, 0, 0);
+    for (int q = 0; q < Ring<T>::LOADS; ++q) {
+        const int id = q * Ring<T>::THREADS + tid;
+        if constexpr (COLS) { constexpr int CH = T / 4; const int k = id / CH; off[q] = (unsigned)(k * rb) + ((id % CH) ^ (col_swizzle(k) << 1)) * 16; }
+        else { const int r = id >> 2; off[q] = (unsigned)(r * rb) + ((id & 3) ^ row_swizzle(r)) * 16; }
     }
 }
-__device__ inline f16x8 frag_rows(const char* lds, int r, int c) { return *reinterpret_cast<const f16x8*>(lds + r * 128 + ((c ^ (r & 7)) << 4)); }
-// Columns: 32 rows (the K axis) x COLS columns; a row's 32-byte units are stored at unit ^ (k & 7), so that the four rows of a transposed read meet different banks
-template <int COLS, int THREADS> __device__ inline void stage_cols(char* lds, const char* src, int64_t rb, int tid) {
-    constexpr int CH = COLS / 4;          // 16-byte chunks a row
-#pragma unroll
-    for (int q = 0; q < 32 * CH / THREADS; ++q) {
-        const int id = q * THREADS + tid, k = id / CH, c = (id % CH) ^ ((k & 7) << 1);
-        __builtin_amdgcn_global_load_lds((glb_t)(src + k * rb + c * 16), (lds_t)(lds + q * THREADS * 16 + (tid & ~63) * 16), 16, 0, 0);
-    }
+__device__ inline f16x8 frag_rows(const char* lds, int r, int c) { return *reinterpret_cast<const f16x8*>(lds + r * 64 + ((c ^ row_swizzle(r)) << 4)); }
+// The MFMA operands of 64 columns from c0 (two of 32) and 16 rows (lane: column lane % 32, rows (lane / 32) * 8 .. + 8), hi and lo.
+// ds_read_b64_tr_b16: within 16 lanes, lane s gives the address of 4 columns of row s / 4 and receives the four rows of column s; two reads, four rows apart, make an operand.
+// 32 columns on and lo each flip one bit of the swizzled unit (128 and 32 bytes).
+template <int T> __device__ inline unsigned cols_at(int c0) {
+    const int l = threadIdx.x & 63, s = l & 15, g = l >> 4, k = (g >> 1) * 8 + (s >> 2), col = c0 + (g & 1) * 16 + (s & 3) * 4;
+    return k * (T * 4) + ((((col >> 4) * 2) ^ col_swizzle(k)) << 5) + (col & 15) * 2;
 }
-// The MFMA operand of 32 columns from c0 and 16 rows from k0 (lane: column lane % 32, rows (lane / 32) * 8 .. + 8).  ds_read_b64_tr_b16: within 16 lanes, lane s gives the
-// address of 4 columns of row s / 4 and receives the four rows of column s; so two reads of 4 rows make the operand.
-template <int COLS> __device__ inline f16x8 frag_cols(const char* lds, int k0, int c0, int lo) {
-    const int l = threadIdx.x & 63, s = l & 15, g = l >> 4;
-    const int col = c0 + (g & 1) * 16 + (s & 3) * 4, unit = (col >> 5) * 4 + lo * 2 + ((col >> 4) & 1);
-    f16x8 r;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int k = k0 + (g >> 1) * 8 + h * 4 + (s >> 2);
-        const char* p = lds + k * (COLS * 4) + ((unit ^ (k & 7)) << 5) + (col & 15) * 2;
-        const s16x4 q = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) r[h * 4 + e] = __builtin_bit_cast(_Float16, (short)q[e]);
-    }
-    return r;
+template <int T> __device__ inline f16x8 frag_cols(unsigned at) {
+    typedef __attribute__((address_space(3))) s16x4* p4;
+    const s16x4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p4)(uintptr_t)at), v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p4)(uintptr_t)(at + 4 * T * 4));
+    typedef short s16x8 __attribute__((ext_vector_type(8)));
+    return __builtin_bit_cast(f16x8, (s16x8)__builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7));
 }
-__device__ inline f32x16 mfma3(f16x8 ah, f16x8 al, f16x8 bh, f16x8 bl, f32x16 c) {
-    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh, c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl, c, 0, 0, 0);
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, c, 0, 0, 0);
-}
-struct Frags { f16x8 ah[2][2], al[2][2], bh[2][2], bl[2][2]; };      // [K half][32 columns of the wave's 64]
-// a: read as rows, or (COLS > 0) transposed out of COLS staged columns
-template <int COLS> __device__ inline void read_frags(Frags& f, const char* la, const char* lb, int wa, int wb) {
-    const int lane = threadIdx.x & 63, lr = lane & 31, lk = lane >> 5;
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            if constexpr (COLS > 0) { f.ah[s][q] = frag_cols<COLS>(la, s * 16, wa + q * 32, 0); f.al[s][q] = frag_cols<COLS>(la, s * 16, wa + q * 32, 1); }
-            else { f.ah[s][q] = frag_rows(la, wa + q * 32 + lr, s * 2 + lk); f.al[s][q] = frag_rows(la, wa + q * 32 + lr, s * 2 + lk + 4); }
-            f.bh[s][q] = frag_rows(lb, wb + q * 32 + lr, s * 2 + lk); f.bl[s][q] = frag_rows(lb, wb + q * 32 + lr, s * 2 + lk + 4);
-        }
-}
-__device__ inline void multiply(const Frags& f, f32x16 c[2][2]) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int p = 0; p < 2; ++p)
-#pragma unroll
-            for (int q = 0; q < 2; ++q) c[p][q] = mfma3(f.ah[s][p], f.al[s][p], f.bh[s][q], f.bl[s][q], c[p][q]);
-}
-// (LDS operations and loads in flight of this wave have landed; the direct loads are counted by vmcnt)
-__device__ inline void landed() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
+struct Frags { f16x8 ah[2], al[2], bh[2], bl[2]; };              // [32 columns of the wave's 64]
 
-// One operand pair of a product: a's and b's first bytes and what a K block advances them by
+// One operand pair of a product: a's and b's first bytes and what a K block of 16 advances them by
 struct Seg { const char *a, *b; int64_t arb, brb, ak, bk; };
 // sum over the K blocks [k0, k1) of a b^T (NN: a's K axis runs along its rows).  The blocks of the second segment begin at `kb`; c is multiplied by `mid` there.
-// T = 128: four waves of 64 x 64, operands staged for all of them, two buffers: a step's loads are issued behind the reads of the step before and have its MFMAs to land in.
-// T = 64: every wave has the whole tile and each fourth K block, its own 16 KB of LDS and no barrier; the four sums meet in the epilogue.
+// T = 128: four waves of 64 x 64, operands staged for all of them.  T = 64: every wave has the whole tile and each fourth K block, LDS of its own and no barrier; the four sums meet in
+// the epilogue.
+// Per step of 16 K (384 cycles of MFMAs a wave): wait for the next stage's loads, counted -- the younger stages' stay in flight, RING - 1 steps ahead, a way from memory -- and for this
+// step's operands, which were read during the last step's MFMAs; barrier; then a third of the MFMAs, the next operands' reads, a third, the loads into the stage just freed, a third.
+// The statements with a memory clobber keep LDS reads where they are (its address went into the direct loads); the operands go through the one that ends their reads.
 template <int T, bool NN> __device__ inline void product(char* lds, const Seg seg[2], int kb, int k0, int k1, float mid, f32x16 c[2][2]) {
-    const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
-    const int step = T == 128 ? 1 : 4, wa = T == 128 ? (wv >> 1) * 64 : 0, wb = T == 128 ? (wv & 1) * 64 : 0;
-    Frags f;
-    auto issue = [&](int k, int buf) {
-        const Seg& sg = seg[k >= kb]; const int kk = k >= kb ? k - kb : k;
-        const char *pa = sg.a + kk * sg.ak, *pb = sg.b + kk * sg.bk;
-        if constexpr (T == 128) {
-            char* l = lds + buf * 2 * STAGE;
-            if constexpr (NN) stage_cols<128, 256>(l, pa, sg.arb, t); else stage_rows<128, 256>(l, pa, sg.arb, t);
-            stage_rows<128, 256>(l + STAGE, pb, sg.brb, t);
-        } else {
-            char* l = lds + wv * STAGE;
-            if constexpr (NN) stage_cols<64, 64>(l, pa, sg.arb, lane); else stage_rows<64, 64>(l, pa, sg.arb, lane);
-            stage_rows<64, 64>(l + STAGE / 2, pb, sg.brb, lane);
+    using R = Ring<T>;
+    const int t = threadIdx.x, lane = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6), lr = lane & 31, lk = lane >> 5;
+    constexpr int step = T == 128 ? 1 : 4, HALF = R::STAGE / 2; const int wa = T == 128 ? (wv >> 1) * 64 : 0, wb = T == 128 ? (wv & 1) * 64 : 0;
+    char* ring = lds + (T == 128 ? 0 : wv * R::N * R::STAGE); const unsigned ring_at = (unsigned)(uintptr_t)(lds_t)ring, mine = ring_at + (T == 128 ? wv * 1024 : 0), cols = NN ? cols_at<T>(wa) + ring_at : 0;
+    unsigned oa[R::LOADS], ob[R::LOADS];
+    lane_offsets<T, NN>(oa, seg[0].arb, T == 128 ? t : lane); lane_offsets<T, false>(ob, seg[0].brb, T == 128 ? t : lane);
+    auto issue = [&](int k, int at) {
+        const bool s2 = k >= kb; const int kk = s2 ? k - kb : k;
+        const char *pa = (s2 ? seg[1].a : seg[0].a) + kk * seg[0].ak, *pb = (s2 ? seg[1].b : seg[0].b) + kk * seg[0].bk;
+#pragma unroll
+        for (int q = 0; q < R::LOADS; ++q) { direct_load(mine + at + q * R::THREADS * 16, pa, oa[q]); direct_load(mine + at + HALF + q * R::THREADS * 16, pb, ob[q]); }
+    };
+    auto read = [&](Frags& f, int at) {
+        const char *la = ring + at, *lb = la + HALF;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            if constexpr (NN) { const unsigned u = (cols ^ (q * 128)) + at; f.ah[q] = frag_cols<T>(u); f.al[q] = frag_cols<T>(u ^ 32); }
+            else { f.ah[q] = frag_rows(la, wa + q * 32 + lr, lk); f.al[q] = frag_rows(la, wa + q * 32 + lr, lk + 2); }
+            f.bh[q] = frag_rows(lb, wb + q * 32 + lr, lk); f.bl[q] = frag_rows(lb, wb + q * 32 + lr, lk + 2);
         }
     };
     const int first = k0 + (T == 128 ? 0 : wv); bool second = first >= kb;
-    if (first < k1) issue(first, 0);
-    int buf = 0;
-    for (int k = first; k < k1; k += step) {
-        landed();
-        if constexpr (T == 128) __syncthreads();
-        const char* l = T == 128 ? lds + buf * 2 * STAGE : lds + wv * STAGE;
-        read_frags<NN ? T : 0>(f, l, l + (T == 128 ? STAGE : STAGE / 2), wa, wb);
-        if (k + step < k1) {
-            if constexpr (T != 128) landed();                    // the same buffer again: its reads have landed
-            issue(k + step, buf ^ 1);
-        }
-        if (!second && k >= kb) {                                // the second product's scale is another power of two
-            second = true;
+    if (first < k1) {
+#pragma unroll
+        for (int i = 0; i < R::N; ++i) if (first + i * step < k1) issue(first + i * step, i * R::STAGE);
+        if (first + (R::N - 1) * step < k1) asm volatile("s_waitcnt vmcnt(%0)" :: "n"((R::N - 1) * 2 * R::LOADS) : "memory"); else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if constexpr (T == 128) asm volatile("s_barrier" ::: "memory");
+        Frags f0, f1; int at = 0;
+        read(f0, 0);
+        auto turn = [&](Frags& f, Frags& next, int k) {
+            const int on = at == (R::N - 1) * R::STAGE ? 0 : at + R::STAGE; const bool more = k + step < k1, load = k + R::N * step < k1;
+            if (k + (R::N - 1) * step < k1) asm volatile("s_waitcnt vmcnt(%0)" :: "n"((R::N - 2) * 2 * R::LOADS) : "memory"); else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(f.ah[0]), "+v"(f.al[0]), "+v"(f.bh[0]), "+v"(f.bl[0]), "+v"(f.ah[1]), "+v"(f.al[1]), "+v"(f.bh[1]), "+v"(f.bl[1]) :: "memory");
+            if constexpr (T == 128) asm volatile("s_barrier" ::: "memory");
+            if (!second && k >= kb) {                            // the second product's scale is another power of two
+                second = true;
+#pragma unroll
+                for (int p = 0; p < 2; ++p)
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) c[p][q] *= mid;
+            }
+            // c += (ah + al) (bh + bl) without al bl: small terms first, the four accumulators in turn (an accumulator's next product waits for its last)
 #pragma unroll
             for (int p = 0; p < 2; ++p)
 #pragma unroll
-                for (int q = 0; q < 2; ++q) c[p][q] *= mid;
+                for (int q = 0; q < 2; ++q) c[p][q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.al[p], f.bh[q], c[p][q], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            if (more) read(next, on);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+#pragma unroll
+                for (int q = 0; q < 2; ++q) c[p][q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ah[p], f.bl[q], c[p][q], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            if (load) issue(k + R::N * step, at);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+#pragma unroll
+                for (int q = 0; q < 2; ++q) c[p][q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ah[p], f.bh[q], c[p][q], 0, 0, 0);
+            at = on;
+        };
+        for (int k = first; k < k1; k += 2 * step) {
+            turn(f0, f1, k);
+            if (k + step < k1) turn(f1, f0, k + step);
         }
-        multiply(f, c);
-        buf ^= 1;
     }
     if (!second && kb < k1)                                      // (this wave's share ended before the second product)
 #pragma unroll
@@ -419,7 +429,7 @@ template <int T> __device__ inline float tile_el(const float* tile, int planes, 
 }
 __device__ inline void store_pair8(char* p, const float v[8]) {
     f16x4 h[2], l[2]; split4(v, h[0], l[0]); split4(v + 4, h[1], l[1]);
-    *reinterpret_cast<f16x8*>(p) = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7); *reinterpret_cast<f16x8*>(p + 64) = __builtin_shufflevector(l[0], l[1], 0, 1, 2, 3, 4, 5, 6, 7);
+    *reinterpret_cast<f16x8*>(p) = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7); *reinterpret_cast<f16x8*>(p + LO) = __builtin_shufflevector(l[0], l[1], 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
 struct SymArgs { Slot l[2], r[2], e, out; int kind, nseg, have_e; float acc, ecoef; };      // out = acc * (sum of l r^T) + ecoef * e, in the buffers' own scales (with e: a factor A too many)
@@ -440,7 +450,7 @@ template <int T, int R> __device__ inline void sym_finish(const Item& it, const 
         for (int z = 0; z < N; ++z) {
             const int id = z * 256 + t, r = side ? id / (R / 8) : id / (T / 8), c = side ? id % (R / 8) * 8 : id % (T / 8) * 8;
             off[z] = pair_off(d.arb, side ? it.ti * T + r : it.tj * T + r0 + r, side ? it.tj * T + r0 + c : it.ti * T + c);
-            if (a.have_e) { eh[z] = *reinterpret_cast<const f16x8*>(E + off[z]); el[z] = *reinterpret_cast<const f16x8*>(E + off[z] + 64); }
+            if (a.have_e) { eh[z] = *reinterpret_cast<const f16x8*>(E + off[z]); el[z] = *reinterpret_cast<const f16x8*>(E + off[z] + LO); }
         }
 #pragma unroll
         for (int z = 0; z < N; ++z) {
@@ -464,9 +474,9 @@ template <int T> __device__ inline void sym_tile(char* lds, const Item& it, cons
     const Dims d = dims(it); const bool kn = a.kind == GRAM || a.kind == SYM_S; const int64_t rb = kn ? d.xrb : d.arb;
     Seg seg[2];
 #pragma unroll
-    for (int s = 0; s < 2; ++s) seg[s] = Seg{slot(it, d, a.l[s]) + (int64_t)it.ti * T * rb, slot(it, d, a.r[s]) + (int64_t)it.tj * T * rb, rb, rb, 128, 128};
+    for (int s = 0; s < 2; ++s) seg[s] = Seg{slot(it, d, a.l[s]) + (int64_t)it.ti * T * rb, slot(it, d, a.r[s]) + (int64_t)it.tj * T * rb, rb, rb, 64, 64};
     f32x16 c[2][2] = {};
-    product<T, false>(lds, seg, a.nseg == 2 ? cdiv(kn ? it.n : it.m, 32) : 1 << 30, it.k0, it.k1, 1.f, c);
+    product<T, false>(lds, seg, a.nseg == 2 ? cdiv(kn ? it.n : it.m, 16) : 1 << 30, it.k0, it.k1, 1.f, c);
     float* tile = reinterpret_cast<float*>(lds); tile_store<T>(tile, c);
     if (it.part < 0) sym_finish<T, T>(it, a, ws.fac, tile, 4, 0);
     else {
@@ -479,10 +489,10 @@ template <int T> __device__ inline void sym_tile(char* lds, const Item& it, cons
     }
 }
 // A tile on or above the diagonal of a symmetric result, or its share of a split K axis
-__global__ __launch_bounds__(256, 2) void ns_sym_kernel(Ws ws, SymArgs a) {
-    __shared__ __attribute__((aligned(16))) char lds[LDS_BYTES];
+template <int T> __global__ __launch_bounds__(256, T == 128 ? 2 : 1) void ns_sym_kernel(Ws ws, SymArgs a) {
+    __shared__ __attribute__((aligned(16))) char lds[Ring<T>::BYTES];
     const Item it = ws.sym[a.kind][blockIdx.x];
-    if (it.tile == 128) sym_tile<128>(lds, it, ws, a); else sym_tile<64>(lds, it, ws, a);
+    sym_tile<T>(lds, it, ws, a);
 }
 // the shares of a tile, summed in order: 32 rows of it a workgroup
 template <int T> __device__ inline void reduce_tile(float* tile, const Item& it, const Ws& ws, const SymArgs& a, int r0) {
@@ -510,11 +520,11 @@ template <int T> __global__ __launch_bounds__(256) void ns_reduce_kernel(Ws ws, 
 enum { OUT_PAIR = 0, OUT_Y = 1, OUT_MUON = 2, OUT_BACK = 3 };
 struct NnArgs { Slot l[2], r[2], e, out, x0; int nseg; float acc, ecoef, mid, decay; };      // value = acc * (mid * l0 r0 + l1 r1) + ecoef * e; one product: acc * l0 r0 + ecoef * e
 template <int T, int DT, int OUT> __device__ inline void nn_tile(char* lds, double* red, const Item& it, const Ws& ws, const NnArgs& a, double* dots) {
-    const Dims d = dims(it); const int kb = cdiv(it.m, 32), t = threadIdx.x;
+    const Dims d = dims(it); const int kb = cdiv(it.m, 16), t = threadIdx.x;
     const Fac fac = ws.fac[it.mat]; const float facc = a.acc * fac.inv2;
     Seg seg[2];
 #pragma unroll
-    for (int s = 0; s < 2; ++s) seg[s] = Seg{slot(it, d, a.r[s]) + (int64_t)it.tj * T * 4, slot(it, d, a.l[s]) + (int64_t)it.ti * T * d.arb, d.xrb, d.arb, 32 * d.xrb, 128};
+    for (int s = 0; s < 2; ++s) seg[s] = Seg{slot(it, d, a.r[s]) + (int64_t)it.tj * T * 4, slot(it, d, a.l[s]) + (int64_t)it.ti * T * d.arb, d.xrb, d.arb, 16 * d.xrb, 64};
     f32x16 c[2][2] = {};
     product<T, true>(lds, seg, a.nseg == 2 ? kb : 1 << 30, 0, a.nseg * kb, a.mid, c);
     // everything the epilogue reads is read before it writes anything: the loads are in flight together
@@ -526,8 +536,8 @@ template <int T, int DT, int OUT> __device__ inline void nn_tile(char* lds, doub
     for (int z = 0; z < N; ++z) {
         const int r = (z * 256 + t) / (T / 8), col = t % (T / 8) * 8, i = it.ti * T + r, j = it.tj * T + col;
         off[z] = pair_off(d.xrb, i, j);
-        eh[z] = *reinterpret_cast<const f16x8*>(E + off[z]); el[z] = *reinterpret_cast<const f16x8*>(E + off[z] + 64);
-        if constexpr (OUT == OUT_BACK) { xh[z] = *reinterpret_cast<const f16x8*>(slot(it, d, a.x0) + off[z]); xl[z] = *reinterpret_cast<const f16x8*>(slot(it, d, a.x0) + off[z] + 64); }
+        eh[z] = *reinterpret_cast<const f16x8*>(E + off[z]); el[z] = *reinterpret_cast<const f16x8*>(E + off[z] + LO);
+        if constexpr (OUT == OUT_BACK) { xh[z] = *reinterpret_cast<const f16x8*>(slot(it, d, a.x0) + off[z]); xl[z] = *reinterpret_cast<const f16x8*>(slot(it, d, a.x0) + off[z] + LO); }
         if constexpr (OUT == OUT_MUON)
             if (rows && i < it.m) { P[z][0] = *reinterpret_cast<const f32x4*>(Y + i * ys + j); P[z][1] = *reinterpret_cast<const f32x4*>(Y + i * ys + j + 4); }
     }
@@ -585,10 +595,10 @@ template <int T, int DT, int OUT> __device__ inline void nn_tile(char* lds, doub
     }
 }
 // A tile of (symmetric m x m) x (m x n)
-template <int DT, int OUT> __global__ __launch_bounds__(256, 2) void ns_nn_kernel(Ws ws, NnArgs a, double* dots) {
-    __shared__ __attribute__((aligned(16))) char lds[LDS_BYTES]; __shared__ double red[4];
+template <int T, int DT, int OUT> __global__ __launch_bounds__(256, T == 128 ? 2 : 1) void ns_nn_kernel(Ws ws, NnArgs a, double* dots) {
+    __shared__ __attribute__((aligned(16))) char lds[Ring<T>::BYTES];
     const Item it = ws.nn[blockIdx.x];
-    if (it.tile == 128) nn_tile<128, DT, OUT>(lds, red, it, ws, a, dots); else nn_tile<64, DT, OUT>(lds, red, it, ws, a, dots);
+    nn_tile<T, DT, OUT>(lds, reinterpret_cast<double*>(lds + 65536), it, ws, a, dots);      // (the epilogue's tile takes the first 64 KB)
 }
 
 // dX = (G - X0 <X0, G>) / |X|_F, or G / eps where the norm was clamped; G carries gscale / |dout|_F
@@ -606,7 +616,7 @@ template <int DT> __global__ __launch_bounds__(256) void ns_back_finish_kernel(W
     for (int p = 0; p < 8; ++p) {
         const int li = p * 8 + (t >> 5), lj = (t & 31) * 4, i = it.ti * PK_ROWS + li, j = it.tj * PK_COLS + lj;
         const f32x4 G = *reinterpret_cast<const f32x4*>(slot(M, g) + i * xrb + (int64_t)j * 4);
-        const char* X0 = slot(M, x0) + pair_off(xrb, i, j); const f16x4 xh = *reinterpret_cast<const f16x4*>(X0), xl = *reinterpret_cast<const f16x4*>(X0 + 64);
+        const char* X0 = slot(M, x0) + pair_off(xrb, i, j); const f16x4 xh = *reinterpret_cast<const f16x4*>(X0), xl = *reinterpret_cast<const f16x4*>(X0 + LO);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float v = clamped ? G[e] * fg : G[e] * fg - ((float)xh[e] + (float)xl[e]) * fx;
@@ -660,10 +670,10 @@ struct NsProblem { std::vector<Desc> d; std::vector<Use> u; Strides st{}; int nX
 
 // Tiles and splits of a call's products, from its sizes alone.
 // 128-tiles share a staged row between two waves (half the loads of 64-tiles, whose four waves split K instead), so they are taken wherever they occupy half the CUs, counting a long K axis
-// as pieces of MIN128 blocks of 32.  The K axis is cut where that makes the launch shorter by this model: a CU has its share of the workgroups, a step of one costs STEP us (the rate of two a CU), and
+// as pieces of MIN128 blocks of 16.  The K axis is cut where that makes the launch shorter by this model: a CU has its share of the workgroups, a step of one costs STEP us (the rate of two a CU), and
 // a cut K axis costs a second launch and its partial sums' way to memory and back.
-static constexpr int CUS = 256, MIN128 = 8, MIN64 = 32;
-static constexpr double STEP = 0.8, LAUNCH = 6.0, PART_US = 64.0 * 1024 * 2 / 3.0e6;      // us; a 64 KB partial sum written and read at 3 TB/s
+static constexpr int CUS = 256, MIN128 = 16, MIN64 = 64;
+static constexpr double STEP = 0.4, LAUNCH = 6.0, PART_US = 64.0 * 1024 * 2 / 3.0e6;      // us; a 64 KB partial sum written and read at 3 TB/s
 static int64_t tri(int64_t m, int tile) { const int64_t t = (m + tile - 1) / tile; return t * (t + 1) / 2; }
 static Layout ns_layout(NsProblem& p) {
     Layout L{}; p.u.assign(p.d.size() * p.kinds, Use{});
@@ -749,8 +759,11 @@ template <int DT> static void ns_launch(int kind, NsProblem& p, const Layout& L,
         else { DescPack<1, 2> dp; dp.d[0] = p.d[0]; for (int u = 0; u < 2; ++u) dp.u[0][u] = p.u[u]; hipLaunchKernelGGL((ns_setup_kernel<1, 2>), grid, dim3(256), 0, s, dp, p.st, p.cuts, bytes, ws); }
     }
     const dim3 blk(256), pk((unsigned)L.n_pk), nn((unsigned)L.n_nn);
+#define NN(dt, out) do { if (p.cuts.nn_tile == 128) hipLaunchKernelGGL((ns_nn_kernel<128, dt, out>), nn, blk, 0, s, ws, f, dots); \
+                         else hipLaunchKernelGGL((ns_nn_kernel<64, dt, out>), nn, blk, 0, s, ws, f, dots); } while (0)
     auto sym = [&](const SymArgs& a) {
-        hipLaunchKernelGGL(ns_sym_kernel, dim3((unsigned)L.n_sym[a.kind]), blk, 0, s, ws, a);
+        if (p.cuts.sym[a.kind].tile == 128) hipLaunchKernelGGL((ns_sym_kernel<128>), dim3((unsigned)L.n_sym[a.kind]), blk, 0, s, ws, a);
+        else hipLaunchKernelGGL((ns_sym_kernel<64>), dim3((unsigned)L.n_sym[a.kind]), blk, 0, s, ws, a);
         if (!L.n_red[a.kind]) return;
         if (p.cuts.sym[a.kind].tile == 128) hipLaunchKernelGGL((ns_reduce_kernel<128>), dim3((unsigned)L.n_red[a.kind] * 4), blk, 0, s, ws, a);
         else hipLaunchKernelGGL((ns_reduce_kernel<64>), dim3((unsigned)L.n_red[a.kind] * 2), blk, 0, s, ws, a);
@@ -777,11 +790,11 @@ template <int DT> static void ns_launch(int kind, NsProblem& p, const Layout& L,
         sym(q);
         if (back && k == steps - 1) break;
         NnArgs f{}; f.l[0] = B(k); f.r[0] = f.e = X(k); f.out = X(k + 1); f.nseg = 1;
-        if (k < steps - 1) { f.acc = (float)(1.0 / SB); f.ecoef = (float)a; hipLaunchKernelGGL((ns_nn_kernel<NS_F32, OUT_PAIR>), nn, blk, 0, s, ws, f, dots); }
+        if (k < steps - 1) { f.acc = (float)(1.0 / SB); f.ecoef = (float)a; NN(NS_F32, OUT_PAIR); }
         else {
             f.acc = (float)(1.0 / (SB * SX)); f.ecoef = (float)(a / SX); f.decay = (float)(1.0 - o.lr * o.weight_decay);
-            if (kind == NS_MUON) hipLaunchKernelGGL((ns_nn_kernel<NS_F32, OUT_MUON>), nn, blk, 0, s, ws, f, dots);
-            else hipLaunchKernelGGL((ns_nn_kernel<DT, OUT_Y>), nn, blk, 0, s, ws, f, dots);
+            if (kind == NS_MUON) NN(NS_F32, OUT_MUON);
+            else NN(DT, OUT_Y);
         }
     }
     if (!back) return;
@@ -799,10 +812,11 @@ template <int DT> static void ns_launch(int kind, NsProblem& p, const Layout& L,
         sym(v);
         NnArgs f{}; f.l[0] = B(k); f.r[0] = f.e = G[cur]; f.l[1] = V; f.r[1] = X(k); f.out = G[cur ^ 1]; f.x0 = X(0); f.nseg = 2;
         f.mid = (float)(sv * SX / (SB * gin)); f.acc = (float)(gout / (sv * SX)); f.ecoef = (float)(a * gout / gin);
-        if (k > 0) hipLaunchKernelGGL((ns_nn_kernel<NS_F32, OUT_PAIR>), nn, blk, 0, s, ws, f, dots);
-        else hipLaunchKernelGGL((ns_nn_kernel<NS_F32, OUT_BACK>), nn, blk, 0, s, ws, f, dots);
+        if (k > 0) NN(NS_F32, OUT_PAIR);
+        else NN(NS_F32, OUT_BACK);
     }
     hipLaunchKernelGGL((ns_back_finish_kernel<DT>), pk, blk, 0, s, ws, xpart, dpart, dots, G[cur], X(0), sg(0), SX, o.eps);
+#undef NN
 }
 
 int ns_run(int kind, int dtype, const NsMatrices* q, int count, const NsOptions& o, void* wsp, int64_t ws_bytes, hipStream_t s, const char** why) {
