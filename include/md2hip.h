@@ -142,6 +142,16 @@ int32_t md2_get_conv_products(int32_t* fwd_dgrad, int32_t* wgrad);
  * (src/Monodepth.jl:191-194) omit; with md2_params_get/set this gives true resume. */
 int32_t md2_opt_state_get(md2_handle* h, float* host_m, float* host_v, int64_t n, double* beta1p, double* beta2p);
 int32_t md2_opt_state_set(md2_handle* h, const float* host_m, const float* host_v, int64_t n, double beta1p, double beta2p);
+/* Muon instead of ADAM for the matrices: the hidden convolutions (every one but the stem, the disparity heads and the pose decoder's last) take md2_muon_raw's update, Cout x Cin k k
+ * each, all other parameters the ADAM step of md2_adam_step (its eta, its moments).  Arguments as for md2_muon_raw; grads scaled by grad_scale first.  The first call allocates the
+ * momentum and a workspace (so it cannot be captured into a graph; later ones can) and makes the handle Muon's: md2_adam_step and md2_train_step's update then return an error, because the
+ * hidden convolutions' ADAM moments are no longer kept, until md2_muon_state_set(h, NULL, 0). */
+int32_t md2_muon_step(md2_handle* h, double lr, double momentum, int32_t nesterov, double weight_decay, int32_t adjust, int32_t steps, const double* host_coefficients, double eps, float grad_scale);
+/* Muon's momentum (Flux parameter layout, host; 0 where ADAM steps): count = md2_params_count(h) once the handle has it, 0 before.  set gives the handle Muon state (a resumed run);
+ * set(h, NULL, 0) drops it and starts ADAM anew (moments zero, beta powers 1); md2_params_set does both, too. */
+int64_t md2_muon_state_count(md2_handle* h);
+int32_t md2_muon_state_get(md2_handle* h, float* host_momentum, int64_t n);
+int32_t md2_muon_state_set(md2_handle* h, const float* host_momentum, int64_t n);
 /* automasking_loss(ssim, x, x[:,:,:,target,:]; source_ids), src/training.jl:9-11 -> [N][1][H][W] */
 int32_t md2_automasking_loss(md2_handle* h, const float* x, float* out);
 
@@ -159,7 +169,7 @@ int32_t md2_comm_world(md2_handle* h, int32_t* rank, int32_t* world);
 int32_t md2_comm_bucket_plan(const md2_config* cfg, int64_t* lo4, int64_t* hi4, int64_t* count);
 int32_t md2_allreduce_grads(md2_handle* h);                 /* sum over ranks of the gradient buffer; no-op when md2_backward already reduced it */
 int32_t md2_comm_allreduce(md2_handle* h, float* dev_buf, int64_t n);   /* in-place sum of any device buffer (loss logging, self-checks) */
-int32_t md2_broadcast_state(md2_handle* h, int32_t root);   /* parameters, ADAM moments + beta powers, BatchNorm running statistics of `root` to every rank */
+int32_t md2_broadcast_state(md2_handle* h, int32_t root);   /* parameters, ADAM moments + beta powers, Muon's momentum (a rank without any gets it, a root without any takes it away), BatchNorm running statistics of `root` to every rank */
 
 /* The loss half alone (src/training.jl:28-77) given disparities and poses; pullbacks may be NULL.
  * ddisp_i like disp_i; drvec/dtvec [2][N][3]. */

@@ -98,6 +98,10 @@ _SIGS = {
     "md2_newton_schulz_bwd": (I32, [P, P, P, I64, I64, I64, C.POINTER(I64), C.POINTER(I64), I32, I32, C.POINTER(F64), F64, P, I64, P]),
     "md2_muon_workspace": (I64, [C.POINTER(I64), C.POINTER(I64), I32, I32]),
     "md2_muon_raw": (I32, [C.POINTER(P), C.POINTER(P), C.POINTER(P), C.POINTER(I64), C.POINTER(I64), I32, F64, F64, I32, F64, I32, C.c_float, I32, C.POINTER(F64), F64, P, I64, P]),
+    "md2_muon_step": (I32, [P, F64, F64, I32, F64, I32, I32, C.POINTER(F64), F64, C.c_float]),
+    "md2_muon_state_count": (I64, [P]),
+    "md2_muon_state_get": (I32, [P, P, I64]),
+    "md2_muon_state_set": (I32, [P, P, I64]),
     "md2_set_lr": (I32, [P, F64]),
     "md2_set_testmode": (I32, [P, I32]),
     "md2_bn_state_count": (I64, [P]),

@@ -948,6 +948,29 @@ __global__ void adam_tail_kernel(float* __restrict__ p, const float* __restrict_
     m[i] = 0.9f * m[i] + (1.f - 0.9f) * ge; v[i] = 0.999f * v[i] + (1.f - 0.999f) * ge * ge;
     p[i] -= m[i] / c1 / (sqrtf(v[i] / c2) + 1e-8f) * lr;
 }
+// the same for the listed ranges of the flat buffers only (what Muon leaves to ADAM): r[i] = {first float4, float4s before this range}, r[n] = {-, all of them}
+__global__ __launch_bounds__(256) void adam_ranges_kernel(float* __restrict__ p, const float* __restrict__ g, float* __restrict__ m, float* __restrict__ v, const long2* __restrict__ r, int n, float c1, float c2,
+                                                          float lr, float gs) {
+    const long n4 = r[n].y;
+    for (long i = blockIdx.x * (long)blockDim.x + threadIdx.x; i < n4; i += (long)gridDim.x * blockDim.x) {
+        int lo = 0, hi = n - 1;
+        while (lo < hi) { const int q = (lo + hi + 1) / 2; if (r[q].y <= i) lo = q; else hi = q - 1; }
+        const long at = (r[lo].x + (i - r[lo].y)) * 4;
+        float4 P = ld4(p + at), G = ld4(g + at), M = ld4(m + at), V = ld4(v + at);
+        float* pp = &P.x; float* gg = &G.x; float* mm = &M.x; float* vv = &V.x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float ge = gg[e] * gs;
+            mm[e] = 0.9f * mm[e] + (1.f - 0.9f) * ge;
+            vv[e] = 0.999f * vv[e] + (1.f - 0.999f) * ge * ge;
+            pp[e] -= mm[e] / c1 / (sqrtf(vv[e] / c2) + 1e-8f) * lr;
+        }
+        st4(p + at, P); st4(m + at, M); st4(v + at, V);
+    }
+}
+void launch_adam_ranges(float* p, const float* g, float* m, float* v, const void* ranges, int n, long n4, float c1, float c2, float lr, float gscale, hipStream_t s) {
+    if (n4 > 0) hipLaunchKernelGGL(adam_ranges_kernel, dim3(grid_for(n4, 256, 1024)), dim3(256), 0, s, p, g, m, v, (const long2*)ranges, n, c1, c2, lr, gscale);
+}
 void launch_adam(float* p, const float* g, float* m, float* v, long n, float c1, float c2, float lr, float gscale, hipStream_t s) {
     const bool aligned = ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v)) & 15) == 0;
     const long n4 = aligned ? n / 4 : 0;

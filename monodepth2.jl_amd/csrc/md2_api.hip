@@ -57,6 +57,7 @@ struct md2_handle {
     float K[9], invK[9];
     long n_int = 0, n_flux = 0;
     float *P = nullptr, *G = nullptr, *M = nullptr, *V = nullptr, *WD = nullptr;
+    float* MU = nullptr; void* mu_ws = nullptr; long* mu_ranges = nullptr; int mu_nranges = 0; long mu_n4 = 0;      // Muon (md2_muon_step): momentum (set: the handle is Muon's), workspace, the ranges ADAM keeps
     bool bs = false; uint16_t *Pb = nullptr, *WDb = nullptr;      // precision 2: activations in bf16; bf16 copies of the weights, refreshed from P / WD once per step
     double beta1p = 1.0, beta2p = 1.0;
     ConvL stem; BNL stem_bn; Block blk[16]; int nblk = 8, depth = 18, bf16 = 0; int stages[5] = {64, 64, 128, 256, 512};
@@ -962,6 +963,7 @@ extern "C" {
 const char* md2_last_error(md2_handle* h) { return h ? h->err.c_str() : g_create_err.c_str(); }
 
 static void destroy_handle(md2_handle* h);
+static void muon_free(md2_handle* h);
 
 // argument checks of md2_create: pure host work, before anything touches the device (also the front end of md2_comm_bucket_plan)
 static int validate_cfg(const md2_config* cfg) {
@@ -1098,6 +1100,7 @@ static void comm_destroy(md2_handle* h);
 static void destroy_handle(md2_handle* h) {          // also the failure path of md2_create: every member is null until it was created
     (void)hipDeviceSynchronize();
     comm_destroy(h);
+    muon_free(h);
     for (auto& e : h->evts) { (void)hipEventDestroy(e.a); (void)hipEventDestroy(e.b); }
     for (int i = 0; i < 64; ++i) if (h->ev_pool[i]) (void)hipEventDestroy(h->ev_pool[i]);
     for (int i = 0; i < 8; ++i) { if (h->ev_cm[i]) (void)hipEventDestroy(h->ev_cm[i]); if (h->ev_cs[i]) (void)hipEventDestroy(h->ev_cs[i]); }
@@ -1126,6 +1129,7 @@ int32_t md2_params_set(md2_handle* h, const float* host, int64_t n) {
     HIPCHK(hipStreamSynchronize(h->stream));
     HIPCHK(hipMemcpy(h->P, in.data(), in.size() * sizeof(float), hipMemcpyHostToDevice));
     HIPCHK(hipMemset(h->M, 0, in.size() * sizeof(float))); HIPCHK(hipMemset(h->V, 0, in.size() * sizeof(float)));
+    muon_free(h);                                       // the optimiser starts anew, whichever it was
     h->beta1p = h->beta2p = 1.0;
     return 0;
 }
@@ -1184,12 +1188,15 @@ int32_t md2_backward(md2_handle* h) {
     if (!h->have_fwd) { h->err = "md2_backward: call md2_train_loss first"; return 2; }
     return model_backward(h);                   // ddisp_lo / drvec / dtvec were filled by md2_train_loss
 }
+static const char* kMuonOwns = "the handle is stepped by Muon (md2_muon_step), which does not keep the hidden convolutions' ADAM moments: md2_muon_state_set(h, NULL, 0) first";
 int32_t md2_adam_step(md2_handle* h, float grad_scale) {
+    if (h->MU) { h->err = kMuonOwns; return 2; }
     h->beta1p *= 0.9; h->beta2p *= 0.999;
     launch_adam(h->P, h->G, h->M, h->V, h->n_int, (float)(1.0 - h->beta1p), (float)(1.0 - h->beta2p), (float)h->cfg.lr, grad_scale, h->stream);
     KCHK(); return 0;
 }
 int32_t md2_train_step(md2_handle* h, const float* x, const float* auto_loss, float* loss, int32_t do_update) {
+    if (do_update && h->MU) { h->err = kMuonOwns; return 2; }
     static const bool no_defer = md2_tune_set("MD2_NO_DEFER_TAIL");
     h->defer_tail = h->two_streams && h->s3 && !no_defer;            // the pullback follows at once: the loss's tail opens its pose stream (loss_train / model_backward)
     if (int r = md2_train_loss(h, x, auto_loss, loss)) { h->defer_tail = false; h->tail.pending = false; return r; }
@@ -1569,6 +1576,75 @@ int32_t md2_muon_raw(float* const* p, const float* const* g, float* const* m, co
     )
 }
 
+// ---- Muon on a handle's parameters --------------------------------------------------------------------------------------
+// the hidden convolutions: internal weights [Cout][taps][Cin] are contiguous matrices (their columns are a permutation of Flux's, which orthogonalisation does not see)
+static std::vector<const ConvL*> muon_convs(const md2_handle* h) {
+    std::vector<const ConvL*> v;
+    for (const ConvL* c : h->convs) if (c->kind == 0 && c != &h->pose[2]) v.push_back(c);
+    return v;
+}
+static void muon_free(md2_handle* h) {
+    if (h->MU) (void)hipFree(h->MU);
+    if (h->mu_ws) (void)hipFree(h->mu_ws);
+    if (h->mu_ranges) (void)hipFree(h->mu_ranges);
+    h->MU = nullptr; h->mu_ws = nullptr; h->mu_ranges = nullptr;
+}
+static int muon_alloc(md2_handle* h) {
+    const auto convs = muon_convs(h); std::vector<NsMatrices> q; std::vector<long> r; long at = 0, n4 = 0;
+    auto keep = [&](long lo, long hi) { if (hi > lo) { r.push_back(lo / 4); r.push_back(n4); n4 += (hi - lo) / 4; } };      // (every offset is a multiple of 16 floats)
+    for (const ConvL* c : convs) { NsMatrices m; m.rows = c->coutP; m.cols = (int64_t)c->taps * c->cinP; q.push_back(m); keep(at, c->w); at = (c->w + c->wn() + 15) / 16 * 16; }
+    keep(at, h->n_int); h->mu_nranges = (int)(r.size() / 2); h->mu_n4 = n4; r.push_back(0); r.push_back(n4);
+    int dev = 0; HIPCHK(hipGetDevice(&dev)); HIPCHK(hipSetDevice(h->cfg.device));
+    const int64_t bytes = ns_workspace(NS_MUON, 1, q.data(), (int)q.size());               // (does not depend on the number of steps)
+    float* mu = nullptr;
+    const bool ok = bytes >= 0 && hipMalloc((void**)&mu, (size_t)h->n_int * sizeof(float)) == hipSuccess && hipMalloc(&h->mu_ws, (size_t)bytes) == hipSuccess
+                    && hipMalloc((void**)&h->mu_ranges, r.size() * sizeof(long)) == hipSuccess && hipMemcpy(h->mu_ranges, r.data(), r.size() * sizeof(long), hipMemcpyHostToDevice) == hipSuccess;
+    h->MU = mu;
+    if (ok) launch_fill(h->MU, h->n_int, 0.f, h->stream);
+    else { muon_free(h); h->err = "md2_muon_step: no device memory for the momentum and the workspace (the first call cannot be captured into a graph)"; (void)hipGetLastError(); }
+    (void)hipSetDevice(dev);
+    return ok ? 0 : 3;
+}
+int32_t md2_muon_step(md2_handle* h, double lr, double momentum, int32_t nesterov, double weight_decay, int32_t adjust, int32_t steps, const double* co, double eps, float grad_scale) {
+    try {
+        if (!h->net_ok) { h->err = "this handle is loss-only (height/width below 64 or not multiples of 32): the model entry points are unavailable"; return 2; }
+        const MuonHyper y{lr, momentum, nesterov, weight_decay, adjust, grad_scale, steps, co, eps}; const char* why = "";
+        if ((why = muon_check(y)) || (why = co ? ns_check(steps, co, eps) : "null coefficients")) { h->err = std::string("md2_muon_step: ") + why; return 2; }
+        if (!h->MU) if (int r = muon_alloc(h)) return r;
+        std::vector<NsMatrices> q;
+        for (const ConvL* c : muon_convs(h)) q.push_back(muon_matrix(h->P + c->w, h->G + c->w, h->MU + c->w, c->coutP, (int64_t)c->taps * c->cinP, y));
+        if (int r = muon_run("md2_muon_step", q, y, h->mu_ws, INT64_MAX, h->stream, &why)) { h->err = std::string("md2_muon_step: ") + why; return r; }
+        h->beta1p *= 0.9; h->beta2p *= 0.999;
+        launch_adam_ranges(h->P, h->G, h->M, h->V, h->mu_ranges, h->mu_nranges, h->mu_n4, (float)(1.0 - h->beta1p), (float)(1.0 - h->beta2p), (float)h->cfg.lr, grad_scale, h->stream);
+        KCHK(); return 0;
+    } catch (const std::exception& e) { h->err = e.what(); return 3; }
+}
+int64_t md2_muon_state_count(md2_handle* h) { return h->MU ? h->n_flux : 0; }
+int32_t md2_muon_state_get(md2_handle* h, float* host, int64_t n) {
+    if (!h->MU) { h->err = "md2_muon_state_get: the handle has no Muon state"; return 2; }
+    try { return get_flat(h, h->MU, host, n); } catch (const std::exception& e) { h->err = e.what(); return 3; }
+}
+int32_t md2_muon_state_set(md2_handle* h, const float* host, int64_t n) {
+    try {
+        if (!host && n == 0) {
+            if (!h->MU) return 0;
+            HIPCHK(hipStreamSynchronize(h->stream));
+            muon_free(h);
+            launch_fill(h->M, h->n_int, 0.f, h->stream); launch_fill(h->V, h->n_int, 0.f, h->stream); h->beta1p = h->beta2p = 1.0;
+            KCHK(); return 0;
+        }
+        if (!host || n != h->n_flux) { h->err = "md2_muon_state_set: wrong parameter count"; return 2; }
+        if (!h->net_ok) { h->err = "md2_muon_state_set: this handle is loss-only"; return 2; }
+        if (!h->MU) if (int r = muon_alloc(h)) return r;
+        std::vector<float> in((size_t)h->n_int), only((size_t)h->n_int, 0.f);
+        convert_params(h, in.data(), const_cast<float*>(host), true);
+        for (const ConvL* c : muon_convs(h)) std::copy(in.begin() + c->w, in.begin() + c->w + c->wn(), only.begin() + c->w);
+        HIPCHK(hipStreamSynchronize(h->stream));
+        HIPCHK(hipMemcpy(h->MU, only.data(), only.size() * sizeof(float), hipMemcpyHostToDevice));
+        return 0;
+    } catch (const std::exception& e) { h->err = e.what(); return 3; }
+}
+
 
 // ---- Flux.testmode! / trainmode!, the BatchNorm running statistics, deterministic mode ------------------------------------------------
 int32_t md2_set_testmode(md2_handle* h, int32_t on) { h->testmode = on != 0; h->have_fwd = false; h->prep_done = false; return 0; }
@@ -1744,7 +1820,7 @@ int32_t md2_comm_allreduce(md2_handle* h, float* dev_buf, int64_t n) {
 int32_t md2_broadcast_state(md2_handle* h, int32_t root) {
     if (!h->comm) { h->err = "md2_broadcast_state: call md2_comm_init first"; return 2; }
     h->have_fwd = false; h->prep_done = false;
-    double bp[2] = {h->beta1p, h->beta2p}; double* dbp = nullptr;
+    double bp[3] = {h->beta1p, h->beta2p, h->MU ? 1.0 : 0.0}; double* dbp = nullptr;
     HIPCHK(hipMalloc((void**)&dbp, sizeof(bp))); HIPCHK(hipMemcpy(dbp, bp, sizeof(bp), hipMemcpyHostToDevice));
     ncclComm_t c = (ncclComm_t)h->comm;
     NCCLCHK(g_rccl.GroupStart());
@@ -1752,11 +1828,15 @@ int32_t md2_broadcast_state(md2_handle* h, int32_t root) {
     NCCLCHK(g_rccl.Broadcast(h->M, h->M, (size_t)h->n_int, ncclFloat, root, c, h->stream));
     NCCLCHK(g_rccl.Broadcast(h->V, h->V, (size_t)h->n_int, ncclFloat, root, c, h->stream));
     NCCLCHK(g_rccl.Broadcast(h->RS, h->RS, (size_t)h->n_rs, ncclFloat, root, c, h->stream));
-    NCCLCHK(g_rccl.Broadcast(dbp, dbp, 2, ncclDouble, root, c, h->stream));
+    NCCLCHK(g_rccl.Broadcast(dbp, dbp, 3, ncclDouble, root, c, h->stream));
     NCCLCHK(g_rccl.GroupEnd());
     HIPCHK(hipStreamSynchronize(h->stream));
     HIPCHK(hipMemcpy(bp, dbp, sizeof(bp), hipMemcpyDeviceToHost)); (void)hipFree(dbp);
     h->beta1p = bp[0]; h->beta2p = bp[1];
+    if (bp[2] == 0.0) { muon_free(h); return 0; }                       // (every rank has the root's answer, so all of them take the same branch)
+    if (!h->MU) if (int r = muon_alloc(h)) return r;
+    NCCLCHK(g_rccl.Broadcast(h->MU, h->MU, (size_t)h->n_int, ncclFloat, root, c, h->stream));
+    HIPCHK(hipStreamSynchronize(h->stream));
     return 0;
 }
 

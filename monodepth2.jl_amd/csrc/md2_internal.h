@@ -285,6 +285,8 @@ void launch_pose_pairs_bwd(const float* dsqcat, float* dsq3, int N, int hw, cons
 void launch_pose_mean_fwd(const View& y, float* rvec, float* tvec, hipStream_t s);
 void launch_pose_mean_bwd(const float* drvec, const float* dtvec, const View& dy, hipStream_t s);
 void launch_adam(float* p, const float* g, float* m, float* v, long n, float c1, float c2, float lr, float gscale, hipStream_t s);
+// ... on n ranges of 16-byte-aligned floats (device table of long2: first float4 | float4s before; entry n: - | n4 in all)
+void launch_adam_ranges(float* p, const float* g, float* m, float* v, const void* ranges, int n, long n4, float c1, float c2, float lr, float gscale, hipStream_t s);
 void launch_fill(float* p, long n, float v, hipStream_t s);
 // dst[i] = bf16(src[i]) (round to nearest even): the per-step bf16 copies of the weights when activations are stored in bf16
 void launch_cast_bf16(const float* src, uint16_t* dst, long n, hipStream_t s);

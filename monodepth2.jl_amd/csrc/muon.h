@@ -20,6 +20,8 @@ struct NsOptions {
     int steps = 5; double coef[3] = {3.4445, -4.7750, 2.0315}, eps = 1e-7;
     double lr = 0, momentum = 0, weight_decay = 0; int nesterov = 1; float grad_scale = 1.f;
 };
+// why these are refused, or null
+const char* ns_check(int steps, const double* coefficients, double eps);
 // bytes of workspace, -1 for sizes that are refused
 int64_t ns_workspace(int kind, int steps, const NsMatrices* q, int count);
 // enqueues on s; 0, or 2 with the reason in *why (nothing was enqueued)

@@ -819,6 +819,11 @@ template <int DT> static void ns_launch(int kind, NsProblem& p, const Layout& L,
 #undef NN
 }
 
+const char* ns_check(int steps, const double* co, double eps) {
+    if (!(eps > 0) || !std::isfinite(eps)) return "eps must be positive";
+    const Plan P = ns_bounds(steps, co, false);
+    return P.ok ? nullptr : P.why;
+}
 int ns_run(int kind, int dtype, const NsMatrices* q, int count, const NsOptions& o, void* wsp, int64_t ws_bytes, hipStream_t s, const char** why) {
     if (!(o.eps > 0) || !std::isfinite(o.eps)) { *why = "eps must be positive"; return 2; }
     const Plan P = ns_bounds(o.steps, o.coef, kind == NS_BACKWARD);

@@ -219,6 +219,17 @@ end
 backward!(h) = check(h, md2_backward(h.ptr), "backward")
 # Flux.Optimise.update!(ADAM(1e-4), θ, ∇), src/Monodepth.jl:170
 adam_step!(h, grad_scale=1f0) = check(h, md2_adam_step(h.ptr, Float32(grad_scale)), "adam_step")
+# Muon for the hidden convolutions, ADAM for the rest (not in the reference)
+function muon_step!(h; eta=0.02, momentum=0.95, nesterov=true, weight_decay=0.0, adjust=:spectral, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7, grad_scale=1f0)
+    co = collect(Float64, coefficients)
+    GC.@preserve co check(h, md2_muon_step(h.ptr, Float64(eta), Float64(momentum), Int32(nesterov), Float64(weight_decay), Int32(adjust === :rms), Int32(steps), pointer(co), Float64(eps), Float32(grad_scale)), "muon_step")
+end
+function muon_state(h)
+    n = md2_muon_state_count(h.ptr); n == 0 && return nothing
+    m = Vector{Float32}(undef, n); GC.@preserve m check(h, md2_muon_state_get(h.ptr, pointer(m), n), "muon_state_get"); m
+end
+muon_state!(h, ::Nothing) = check(h, md2_muon_state_set(h.ptr, C_NULL, Int64(0)), "muon_state_set")
+muon_state!(h, m::Vector{Float32}) = GC.@preserve m check(h, md2_muon_state_set(h.ptr, pointer(m), Int64(length(m))), "muon_state_set")
 # the loop body src/Monodepth.jl:156-176 in one call (with a communicator attached: + all-reduce, ADAM on the mean)
 function train_step!(h, x, auto_loss=nothing; update=true)
     loss = ROCArray{Float32}(undef, 1)

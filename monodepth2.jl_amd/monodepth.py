@@ -351,6 +351,7 @@ class Model:
             raise RuntimeError("a new batch / resolution / Params needs a new handle, but an RCCL communicator is attached: comm_destroy() on every rank first, then comm_init again")
         saved = self.params() if self._h is not None else self._params_host
         state = self._opt_and_bn_state() if self._h is not None else None
+        muon = self.muon_state() if self._h is not None else None
         self.close()
         cfg = _lib.Md2Config(N, Cc, H, W, int(extra["automasking"]), x.device.index or 0, extra["min_depth"], extra["max_depth"], extra["disparity_smoothness"], self.lr,
                              self.encoder.depth, PRECISIONS[self.precision], int(extra["target_id"]), (C.c_int32 * 2)(*extra["source_ids"]),
@@ -362,6 +363,8 @@ class Model:
             self.load_params(saved)
         if state is not None:
             self._restore_opt_and_bn_state(state)
+        if muon is not None:
+            self.load_muon_state(muon)
         if self._testmode:
             _check(_lib.lib().md2_set_testmode(self._h, 1), self._h)
         if cache is not None:
@@ -379,6 +382,22 @@ class Model:
         mm, vv, b1, b2, bn = state; L = _lib.lib()
         _check(L.md2_opt_state_set(self._h, mm.ctypes.data_as(C.c_void_p), vv.ctypes.data_as(C.c_void_p), mm.size, float(b1), float(b2)), self._h, "opt_state_set")
         self.load_bn_state(bn)
+
+    # -- Muon's momentum (None: the handle is ADAM's) ----------------------------------------------------------------------------------
+    def muon_state(self):
+        n = _lib.lib().md2_muon_state_count(_need_handle(self, "muon_state"))
+        if n == 0:
+            return None
+        out = np.empty(n, np.float32)
+        _check(_lib.lib().md2_muon_state_get(self._h, out.ctypes.data_as(C.c_void_p), n), self._h, "muon_state_get"); return out
+
+    def load_muon_state(self, st):
+        """None drops Muon's state: ADAM starts anew."""
+        _need_handle(self, "load_muon_state")
+        st = None if st is None else np.ascontiguousarray(st, np.float32)
+        with torch.cuda.device(self._shape[-1] or 0):
+            _lib.lib().md2_set_stream(self._h, _stream())
+            _check(_lib.lib().md2_muon_state_set(self._h, None if st is None else st.ctypes.data_as(C.c_void_p), 0 if st is None else st.size), self._h, "muon_state_set")
 
     # -- Flux BatchNorm state: running mean / variance per BatchNorm (what `@save model_host` keeps besides the weights) -----------------------
     def bn_state(self):
@@ -510,7 +529,8 @@ def save_checkpoint(m: Model, path):
     n = _lib.lib().md2_params_count(m._h)
     mm = np.empty(n, np.float32); vv = np.empty(n, np.float32); b1 = C.c_double(); b2 = C.c_double()
     _check(_lib.lib().md2_opt_state_get(m._h, mm.ctypes.data_as(C.c_void_p), vv.ctypes.data_as(C.c_void_p), n, C.byref(b1), C.byref(b2)), m._h, "opt_state_get")
-    np.savez(path, params=m.params(), adam_m=mm, adam_v=vv, beta1p=b1.value, beta2p=b2.value, bn_state=m.bn_state(), in_channels=m.encoder.in_channels, encoder_depth=m.encoder.depth, lr=m.lr)
+    muon = m.muon_state()
+    np.savez(path, **({} if muon is None else {"muon_m": muon}), params=m.params(), adam_m=mm, adam_v=vv, beta1p=b1.value, beta2p=b2.value, bn_state=m.bn_state(), in_channels=m.encoder.in_channels, encoder_depth=m.encoder.depth, lr=m.lr)
 
 
 def load_checkpoint(m: Model, path):
@@ -522,6 +542,7 @@ def load_checkpoint(m: Model, path):
     m.load_params(ck["params"])
     if m._h is None:
         raise RuntimeError("load_checkpoint: run the model once (or call model._ensure) before restoring the optimiser state")
+    m.load_muon_state(ck["muon_m"] if "muon_m" in ck else None)             # (before the ADAM state: dropping Muon's clears it)
     mm = np.ascontiguousarray(ck["adam_m"], np.float32); vv = np.ascontiguousarray(ck["adam_v"], np.float32)
     _check(_lib.lib().md2_opt_state_set(m._h, mm.ctypes.data_as(C.c_void_p), vv.ctypes.data_as(C.c_void_p), mm.size, float(ck["beta1p"]), float(ck["beta2p"])), m._h, "opt_state_set")
     if "bn_state" in ck:                  # BatchNorm running statistics: needed to reproduce test-mode inference (eval_image / eval_video, src/Monodepth.jl:209,237)
@@ -637,8 +658,33 @@ class ADAM:
         self.eta = eta
 
 
-def update(optimizer: ADAM, model: Model, grad_scale=1.0):
-    """Flux.Optimise.update!(optimizer, theta, grads) — the step size is the optimiser's eta."""
+@dataclass
+class Muon:
+    """Muon for the hidden convolutions (their updates orthogonalised, see muon_raw), ADAM(adam_eta) for the stem, the output layers, biases and BatchNorm; `update(Muon(...), model)`.
+    The momentum lives in the model's handle.  adjust="spectral": eta is the update's size per singular direction (0.02 and the like); "rms": eta is of an ADAM step's size (1e-4)."""
+    eta: float = 0.02
+    momentum: float = 0.95
+    nesterov: bool = True
+    weight_decay: float = 0.0
+    adjust: str = "spectral"
+    steps: int = 5
+    coefficients: Tuple[float, float, float] = (3.4445, -4.7750, 2.0315)
+    eps: float = 1e-7
+    adam_eta: float = 1e-4
+
+
+def update(optimizer, model: Model, grad_scale=1.0):
+    """Flux.Optimise.update!(optimizer, theta, grads) — the step size is the optimiser's eta (ADAM or Muon)."""
+    if isinstance(optimizer, Muon):
+        o = optimizer; h = _need_handle(model, "update"); st, co, ep = _ns_args(o.steps, o.coefficients, o.eps)
+        if o.adjust not in _MUON_ADJUST:
+            raise ValueError("Muon: adjust must be 'spectral' or 'rms'")
+        if o.adam_eta != model.lr:
+            model.lr = o.adam_eta
+        with torch.cuda.device(model._shape[-1] or 0):
+            _lib.lib().md2_set_stream(h, _stream())
+            _check(_lib.lib().md2_muon_step(h, float(o.eta), float(o.momentum), int(bool(o.nesterov)), float(o.weight_decay), _MUON_ADJUST[o.adjust], st, co, ep, float(grad_scale)), h, "muon_step")
+        return
     _lib.lib().md2_set_stream(model._h, _stream())
     if optimizer is not None and optimizer.eta != model.lr:
         model.lr = optimizer.eta                      # (the property setter calls md2_set_lr)

@@ -88,29 +88,32 @@ class DataParallel:
             flat = self.model.param_buffer(); broadcast_params_(flat, 0, self.group)
             # ADAM moments / BatchNorm statistics travel through the host copies (rare: construction only)
             st = list(self.model._opt_and_bn_state())
-            obj = [st if dist.get_rank(self.group) == 0 else None]
+            obj = [(st, self.model.muon_state()) if dist.get_rank(self.group) == 0 else None]
             dist.broadcast_object_list(obj, src=0, group=self.group)
-            self.model._restore_opt_and_bn_state(tuple(obj[0]))
+            self.model.load_muon_state(obj[0][1])
+            self.model._restore_opt_and_bn_state(tuple(obj[0][0]))
         self._ready = True
 
-    def train_step(self, x, auto_loss, cache, parameters):
+    def train_step(self, x, auto_loss, cache, parameters, optimizer=None):
+        """optimizer: None for ADAM(model.lr), or a Muon (or ADAM)."""
         from . import monodepth as md
         if not self._ready:
             self._setup(x, parameters, cache)
-        if self.comm == "rccl":
+        if self.comm == "rccl" and optimizer is None:
             return md.train_step(self.model, x, auto_loss, cache, parameters, do_update=True)       # all-reduce + ADAM(1/world) inside the library
         loss = md.train_step(self.model, x, auto_loss, cache, parameters, do_update=False)
-        self.allreduce_and_update()
+        self.allreduce_and_update(optimizer)
         return loss
 
-    def allreduce_and_update(self):
-        """After a local `gradient(model)`: sum the gradient buffers over the ranks, then ADAM on the mean."""
+    def allreduce_and_update(self, optimizer=None):
+        """After a local `gradient(model)`: sum the gradient buffers over the ranks, then ADAM (or the given optimiser) on the mean.  Muon's orthogonalisation is deterministic, so the
+        replicas stay identical without exchanging updates."""
         from . import monodepth as md
         if self.comm == "rccl":
             self.model.allreduce_grads()
         else:
             allreduce_sum_(self.model.grad_buffer(), self.group)
-        md.update(md.ADAM(self.model.lr), self.model, grad_scale=1.0 / world_size(self.group))
+        md.update(md.ADAM(self.model.lr) if optimizer is None else optimizer, self.model, grad_scale=1.0 / world_size(self.group))
 
 
 def bucket_plan(batch, channels, height, width, depth=18, scale_levels=(2, 3, 4, 5)):

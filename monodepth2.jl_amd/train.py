@@ -24,8 +24,8 @@ def build_model(in_channels, lr=1e-4, seed=42, depth=18, precision="f32"):
 
 
 def train(datasets, log_dir, save_dir, batch_size=4, n_epochs=20, log_iter=50, save_iter=500, automasking=False,
-          disparity_smoothness=1e-3, lr=1e-4, max_iters=None, seed=0, model=None, quiet=False):
-    """Returns (model, list of per-iteration losses).  `datasets`: list of Depth10k / KittyDataset (same resolution and channels)."""
+          disparity_smoothness=1e-3, lr=1e-4, max_iters=None, seed=0, model=None, quiet=False, optimizer=None):
+    """Returns (model, list of per-iteration losses).  `optimizer`: None for the reference's ADAM(lr), or a Muon(...) (its adam_eta then steps what ADAM keeps, and `lr` is not used).  `datasets`: list of Depth10k / KittyDataset (same resolution and channels)."""
     import torch
     os.makedirs(log_dir, exist_ok=True); os.makedirs(save_dir, exist_ok=True)
     rank, world = (torch.distributed.get_rank(), torch.distributed.get_world_size()) if torch.distributed.is_initialized() else (0, 1)
@@ -40,8 +40,9 @@ def train(datasets, log_dir, save_dir, batch_size=4, n_epochs=20, log_iter=50, s
                           dataset.target_id, list(dataset.source_ids), scales)
     if model is None:
         model = build_model(in_channels, lr=lr)
-    model.lr = lr                                             # ADAM's eta lives in the model's handle configuration: `lr` wins over a passed-in model's
-    optimizer = md.ADAM(lr)
+    if optimizer is None:
+        optimizer = md.ADAM(lr)
+    model.lr = optimizer.adam_eta if isinstance(optimizer, md.Muon) else optimizer.eta      # ADAM's eta lives in the model's handle configuration: it wins over a passed-in model's
     dp = None
     losses, it = [], 0
     for epoch in range(1, n_epochs + 1):
@@ -61,7 +62,7 @@ def train(datasets, log_dir, save_dir, batch_size=4, n_epochs=20, log_iter=50, s
             loss, disparity, warped, _ = md.train_loss(model, x, auto_loss, cache, parameters, do_visualization)
             md.gradient(model)
             if dp is not None:
-                dp.allreduce_and_update()
+                dp.allreduce_and_update(optimizer)
             else:
                 md.update(optimizer, model)
             loss_cpu = float(loss)

@@ -370,3 +370,122 @@ def test_orthogonalised_weight_trains_through_its_pullback():
         w = m.newton_schulz(v); dv = m.newton_schulz_pullback(v, w - t)
         check(w, v); check_back(dv, v, w - t)
         m.muon_raw([v], [dv], [mo], lr=0.05)
+
+
+# ---- the model's own path -------------------------------------------------------------------------------------------------------------
+def make_model(depth=18, N=2, C=1, H=64, W=96, seed=3, lr=1e-4):
+    m = md(); syn = md2amd.synthetic; K, iK = syn.depth10k_intrinsics(W, H)
+    params = m.Params(target_size=(W, H), batch_size=N, automasking=False)
+    cache = m.TrainCache(m.SSIM(), m.Backproject(W, H), m.Project(W, H), K, iK, 2, [1, 3], [0.125, 0.25, 0.5, 1.0])
+    enc = m.ResidualNetwork(depth, in_channels=C); model = m.Model(enc, m.DepthDecoder(list(enc.stages), [2, 3, 4, 5]), m.PoseDecoder(enc.stages[-1]), lr=lr)
+    model.load_params(syn.init_params(C, seed=seed, randomize_affine=True, depth=depth))
+    return model, params, cache, torch.from_numpy(syn.synthetic_triplets(N, C, H, W, seed=5)).cuda()
+
+
+def arrays(flat, depth=18):
+    out, off = {}, 0
+    for name, kind, shape in md2amd.synthetic.param_layout(1, depth):
+        n = int(np.prod(shape)); out[name] = (kind, flat[off:off + n].reshape(shape)); off += n
+    return out
+
+
+def hidden(name, kind):
+    return kind == "W" and name != "enc.stem.W" and not name.startswith("dec.head") and name != "pose.pose3.W"
+
+
+@gpu
+@pytest.mark.parametrize("depth", [18, 50])
+def test_model_update_with_muon(depth):
+    """Two steps of update(Muon, model) against 64 bits from the model's own gradients: the hidden convolutions as matrices, everything else exactly as an ADAM step leaves it."""
+    m = md(); a, params, cache, x = make_model(depth); b = make_model(depth)[0]
+    opt = m.Muon(eta=1e-3, weight_decay=0.1, adjust="rms", adam_eta=2e-4); mom = None
+    for _ in range(2):
+        m.train_step(a, x, None, cache, params, do_update=False); m.train_step(b, x, None, cache, params, do_update=False)
+        p0, g = a.params(), a.grads(); b.param_buffer().copy_(a.param_buffer()); b.grad_buffer().copy_(a.grad_buffer())
+        m.update(opt, a, grad_scale=0.5); m.update(m.ADAM(2e-4), b, grad_scale=0.5)
+        p1, q1 = arrays(a.params(), depth), arrays(b.params(), depth); p0, g = arrays(p0, depth), arrays(g, depth); got = arrays(a.muon_state(), depth)
+        mom = mom or {k: np.zeros_like(v) for k, (_, v) in p0.items()}; count = 0
+        for name, (kind, after) in p1.items():
+            if not hidden(name, kind):
+                assert np.array_equal(after, q1[name][1]), name
+                assert not got[name][1].any(), name
+                continue
+            count += 1; t = [torch.from_numpy(np.ascontiguousarray(v)) for v in (p0[name][1], g[name][1], mom[name])]
+            if t[0].numel() > 1 << 20 and depth == 50:            # (the largest ones: their rows' norms only, to keep the test short)
+                assert np.isfinite(after).all() and not np.array_equal(after, p0[name][1]); mom[name] = got[name][1]; continue
+            ep, em, step = muon_plain(*t, 1e-3, 0.95, True, 0.1, "rms", 0.5)
+            assert float((torch.from_numpy(np.ascontiguousarray(got[name][1])).double() - em).abs().max()) <= 3 * 2.0 ** -24 * float(t[1].abs().max() + t[2].abs().max()), name
+            assert float((torch.from_numpy(np.ascontiguousarray(after)).double() - ep).norm()) <= float(2 * 2.0 ** -24 * (t[0].double().norm() + step.norm()) + 2e-5 * step.norm()), name
+            mom[name] = got[name][1]
+        assert count == {18: 32, 50: 65}[depth]
+
+
+@gpu
+def test_a_muon_handle_refuses_adam_until_its_state_is_dropped():
+    m = md(); model, params, cache, x = make_model(); L = md2amd._lib.lib()
+    with pytest.raises(RuntimeError, match="no device handle"):
+        m.update(m.Muon(), model)
+    m.train_step(model, x, None, cache, params); assert model.muon_state() is None
+    for bad in (dict(eta=-1.0), dict(momentum=1.0), dict(weight_decay=-1.0), dict(steps=0), dict(eps=0.0), dict(coefficients=(9.0, 0.0, 0.0))):
+        with pytest.raises(RuntimeError, match="muon_step"):
+            m.update(m.Muon(**bad), model)
+    with pytest.raises(ValueError):
+        m.update(m.Muon(adjust="x"), model)
+    assert model.muon_state() is None                                     # a refused call leaves the handle ADAM's
+    m.update(m.Muon(), model); p = model.params(); assert np.abs(model.muon_state()).max() > 0
+    with pytest.raises(RuntimeError, match="stepped by Muon"):
+        m.update(m.ADAM(1e-4), model)
+    with pytest.raises(RuntimeError, match="stepped by Muon"):
+        m.train_step(model, x, None, cache, params)
+    assert np.array_equal(model.params(), p)
+    assert L.md2_muon_state_set(model._h, p.ctypes.data_as(ctypes.c_void_p), 7) == 2 and L.md2_muon_state_set(model._h, None, 7) == 2
+    model.load_params(p); assert model.muon_state() is None                # new parameters: the optimiser starts anew
+    m.update(m.Muon(), model); p = model.params(); model.load_muon_state(None); st = model._opt_and_bn_state()
+    assert model.muon_state() is None and not st[0].any() and not st[1].any() and st[2:4] == (1.0, 1.0)
+    m.train_step(model, x, None, cache, params); assert not np.array_equal(model.params(), p)
+
+
+@gpu
+def test_muon_state_survives_a_handle_rebuild_and_a_checkpoint(tmp_path):
+    m = md(); model, params, cache, x = make_model(); opt = m.Muon(eta=1e-3)
+    for _ in range(2):
+        m.train_step(model, x, None, cache, params, do_update=False); m.update(opt, model)
+    st, adam = model.muon_state(), model._opt_and_bn_state()
+    m.save_checkpoint(model, str(tmp_path / "c.npz"))
+    m.train_loss(model, x[:1].contiguous(), None, cache, m.Params(target_size=(96, 64), batch_size=1, automasking=False))      # another batch size: a new handle
+    assert np.array_equal(model.muon_state(), st) and np.array_equal(model._opt_and_bn_state()[0], adam[0])
+    other, _, _, _ = make_model(seed=9); m.train_step(other, x, None, cache, params, do_update=False); m.load_checkpoint(other, str(tmp_path / "c.npz"))
+    assert np.array_equal(other.muon_state(), st) and np.array_equal(other._opt_and_bn_state()[1], adam[1]) and other._opt_and_bn_state()[2] == adam[2]
+    plain, _, _, _ = make_model(seed=9); m.train_step(plain, x, None, cache, params); m.save_checkpoint(plain, str(tmp_path / "d.npz"))
+    m.load_checkpoint(other, str(tmp_path / "d.npz")); assert other.muon_state() is None and np.array_equal(other._opt_and_bn_state()[0], plain._opt_and_bn_state()[0])
+
+
+@gpu
+def test_muon_step_beside_the_training_step_and_in_one_process_data_parallel():
+    """Training steps with Muon, the two-stream step around it, equal one after the other and through DataParallel (one rank)."""
+    m = md(); opt = m.Muon(eta=1e-3); m.set_deterministic(True)
+    try:
+        runs = []
+        for way in range(2):
+            model, params, cache, x = make_model(); dp = md2amd.parallel.DataParallel(model, comm="torch"); losses = []
+            for _ in range(3):
+                if way:
+                    losses.append(float(dp.train_step(x, None, cache, params, optimizer=opt)))
+                else:
+                    loss = m.train_loss(model, x, None, cache, params)[0]; m.gradient(model); m.update(opt, model); losses.append(float(loss))
+            runs.append((losses, model.params(), model.muon_state()))
+        assert runs[0][0] == runs[1][0] and np.array_equal(runs[0][1], runs[1][1]) and np.array_equal(runs[0][2], runs[1][2]) and all(np.isfinite(runs[0][0]))
+    finally:
+        m.set_deterministic(False)
+
+
+@gpu
+def test_train_takes_the_optimizer(tmp_path):
+    class Frames:                                                         # what train() reads of a dataset
+        resolution, target_id, source_ids = (96, 64), 2, (1, 3); K, invK = md2amd.synthetic.depth10k_intrinsics(96, 64)
+        x = md2amd.synthetic.synthetic_triplets(4, 1, 64, 96, seed=7)
+        def __len__(self): return 4
+        def __getitem__(self, i): return self.x[i]
+    model, losses = md2amd.train.train([Frames()], str(tmp_path / "l"), str(tmp_path / "s"), batch_size=2, n_epochs=2, log_iter=100, save_iter=2, quiet=True, optimizer=md().Muon(eta=1e-3, adam_eta=5e-5))
+    assert len(losses) == 4 and np.isfinite(losses).all() and model.lr == 5e-5 and np.abs(model.muon_state()).max() > 0
+    assert any("muon_m" in np.load(f) for f in (tmp_path / "s").glob("*.npz"))
