@@ -39,6 +39,7 @@ constexpr int PART = 64 * 64 * 4;         // unit of the split products' partial
 // where one weight (or batch of equal matrices) has its part of a product's lists
 struct Use { int32_t first, red, part; };                        // first item, first reduction item, first partial sum
 struct Cut { int32_t tile, chunk; };                             // a product's tile side, and at most how many K blocks an item has: the same for every weight of a call
+constexpr double SX = 8192.0, SA = 2048.0, SB = 512.0;            // scales of X (norm <= 4), A (<= 16) and B (<= 60): below 2^15, and f16 ends at 65504
 // what the host passes per weight, by value
 struct Desc {
     const void* x; const void* d; void* y;                    // matrix | dout | result;  Muon: momentum | gradient | weight
@@ -633,6 +634,200 @@ template <int DT> __global__ __launch_bounds__(256) void ns_back_finish_kernel(W
     }
 }
 
+// ---- small matrices: a workgroup each, everything in LDS --------------------------------------------------------------------
+// A call whose matrices all fit (short side MP = 32 or 64, pairs of X and A within 160 KB) is one launch: eight waves keep X in LDS from the first read to the result.  The launches of the
+// tiled path cost 5 - 6 us each whatever the size; its 18 for a 64 x 64 matrix took 106 us.
+// LDS rows are an odd multiple of 64 bytes off a multiple of 256, and swizzled as the ring's, so that the products' row reads meet every bank.
+template <int MT> struct Small {
+    static constexpr int MP = MT * 32, TILES = MT * MT, KS = MT == 1 ? 4 : 2, AROW = 320, AB = MT == 1 ? 12288 : MP * AROW, LDS = 163840;      // KS: waves that share a Gram tile's K axis
+    __host__ __device__ static int blocks(int n) { return cdiv(n, 32) * 2; }                            // 16-column blocks of a row
+    __host__ __device__ static int row(int n) { const int b = blocks(n); return (b + (5 - b % 4) % 4) * 64; }      // bytes of a row
+    __host__ static bool fits(int m, int n) { return m <= MP && (int64_t)MP * row(n) + AB + 256 <= LDS; }
+};
+struct SmallArgs { int steps; float gram, poly, poly_e, apply, apply_e, last, last_e, decay; double eps, grow; MuonArgs mu; int dt_bytes; };
+template <int N> struct SmallPack { Desc d[N]; };
+__device__ inline void unpack4(const f16x4 h, const f16x4 l, float v[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = (float)h[e] + (float)l[e];
+}
+// four neighbouring columns (j a multiple of 4) of a swizzled LDS row
+__device__ inline char* small_at(char* rows, int stride, int i, int j, int lo) { return rows + i * stride + (j >> 4) * 64 + (((((j & 15) >> 3) + lo * 2) ^ row_swizzle(i)) << 4) + (j & 4) * 2; }
+__device__ inline f16x8 small_row(const char* rows, int stride, int i, int block, int chunk) { return *reinterpret_cast<const f16x8*>(rows + i * stride + block * 64 + ((chunk ^ row_swizzle(i)) << 4)); }
+
+template <int MT, int DT, int MUON, int N> __global__ __launch_bounds__(512) void ns_small_kernel(SmallPack<N> dp, Strides st, SmallArgs a) {
+    using C = Small<MT>;
+    __shared__ __attribute__((aligned(16))) char lds[C::LDS];
+    const Desc& D = dp.d[N == 1 ? 0 : blockIdx.x]; const int b = N == 1 ? blockIdx.x : 0, m = D.m, n = D.n, nb = C::blocks(n), S = C::row(n);
+    const int t = threadIdx.x, lane = t & 63, wv = t >> 6, lr = lane & 31, lk = lane >> 5;
+    char *X = lds, *A = lds + C::MP * S; double* red = reinterpret_cast<double*>(lds + C::LDS - 256);
+    const int64_t ys = D.tall ? 1 : n, yl = D.tall ? m : 1, ss = N == 1 ? st.xs : ys, sl = N == 1 ? st.xl : yl;
+    const char* src = (const char*)D.x + (N == 1 ? st.xb * b * a.dt_bytes : 0); char* y = (char*)D.y + (int64_t)m * n * b * a.dt_bytes;
+    const bool along = !(ss == 1 && sl != 1);                    // neighbouring lanes along the long side
+    // X as fp32, each block of 16 columns where its pairs will be, and the norm
+    double sum = 0; const int cols = nb * 16, all = C::MP * cols;
+    for (int q0 = 0; q0 < all; q0 += 8 * 512) {
+        float x[8], g[8]; int at[8]; int64_t o[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int q = q0 + u * 512 + t, i = along ? q / cols : q % C::MP, j = along ? q % cols : q / C::MP;
+            at[u] = q < all ? i * S + j * 4 : -1; o[u] = q < all && i < m && j < n ? i * ss + j * sl : -1;      // (16 columns of fp32 take the 64 bytes of their block)
+            x[u] = o[u] >= 0 ? ld_el<DT>(src, o[u]) : 0.f;
+            if constexpr (MUON) g[u] = o[u] >= 0 ? reinterpret_cast<const float*>(D.d)[o[u]] : 0.f;
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            if constexpr (MUON) {
+                x[u] = momentum_step(x[u], g[u], a.mu);
+                if (o[u] >= 0) reinterpret_cast<float*>(const_cast<char*>(src))[o[u]] = x[u];
+                x[u] = muon_u(x[u], g[u], a.mu);
+            }
+            if (at[u] >= 0) *reinterpret_cast<float*>(X + at[u]) = x[u];
+            sum += (double)x[u] * (double)x[u];
+        }
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+    if (lane == 0) red[wv] = sum;
+    __syncthreads();
+    const double norm = sqrt(((red[0] + red[1]) + (red[2] + red[3])) + ((red[4] + red[5]) + (red[6] + red[7])));
+    int fq = 0;
+    if (norm <= a.eps && norm > 0) { const double room = 4.0 * a.eps / (norm * a.grow); if (room >= 2.0) fq = ilogb(room); }      // (as in ns_pack_kernel)
+    const float inv2 = (float)ldexp(1.0, -2 * fq); int fe; const float f = (float)frexp(ldexp(SX, fq) / (norm <= a.eps ? a.eps : norm), &fe);
+    for (int q = t; q < C::MP * nb; q += 512) {                  // a block of 16 columns a thread
+        const int i = q / nb, blk = q % nb; char* p = X + i * S + blk * 64; f32x4 r[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) r[k] = *reinterpret_cast<const f32x4*>(p + k * 16);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            float w[4]; f16x4 hi, lo;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = ldexpf(r[k][e], fe) * f;
+            split4(w, hi, lo);
+            *reinterpret_cast<f16x4*>(small_at(X, S, i, blk * 16 + k * 4, 0)) = hi; *reinterpret_cast<f16x4*>(small_at(X, S, i, blk * 16 + k * 4, 1)) = lo;
+        }
+    }
+    __syncthreads();
+    const int tile = wv % C::TILES, ks = wv / C::TILES, i0 = tile / MT * 32, j0 = tile % MT * 32;
+    for (int step = 0; step < a.steps; ++step) {
+        const bool last = step == a.steps - 1;
+        // A = X X^T: a 32 x 32 tile and a share of K a wave, three sums that do not wait for each other
+        f32x16 c[3] = {};
+        if (ks < C::KS) {
+            for (int k = ks; k < nb; k += C::KS) {
+                const f16x8 ah = small_row(X, S, i0 + lr, k, lk), al = small_row(X, S, i0 + lr, k, lk + 2), bh = small_row(X, S, j0 + lr, k, lk), bl = small_row(X, S, j0 + lr, k, lk + 2);
+                c[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, c[0], 0, 0, 0); c[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh, c[1], 0, 0, 0); c[2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl, c[2], 0, 0, 0);
+            }
+            c[0] += c[1] + c[2];
+            if (ks > 0)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    f32x4 w;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[e] = c[0][g * 4 + e];
+                    *reinterpret_cast<f32x4*>(A + (((ks - 1) * C::TILES + tile) * 256 + g * 64 + lane) * 16) = w;
+                }
+        }
+        __syncthreads();
+        if (ks == 0)
+#pragma unroll
+            for (int r = 1; r < C::KS; ++r)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const f32x4 w = *reinterpret_cast<const f32x4*>(A + (((r - 1) * C::TILES + tile) * 256 + g * 64 + lane) * 16);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) c[0][g * 4 + e] += w[e];
+                }
+        __syncthreads();
+        auto write = [&](const f32x16& v) {                      // lane: row j0 + lr, registers: four neighbouring columns from i0 (A and B are symmetric)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const float w[4] = {v[g * 4], v[g * 4 + 1], v[g * 4 + 2], v[g * 4 + 3]}; f16x4 hi, lo; split4(w, hi, lo); const int i = i0 + g * 8 + lk * 4;
+                *reinterpret_cast<f16x4*>(small_at(A, C::AROW, j0 + lr, i, 0)) = hi; *reinterpret_cast<f16x4*>(small_at(A, C::AROW, j0 + lr, i, 1)) = lo;
+            }
+        };
+        if (ks == 0) { c[0] *= a.gram; write(c[0]); }
+        __syncthreads();
+        // B = b A + c A A, in A's place
+        f32x16 p[3] = {}; float E[16];
+        if (ks == 0) {
+#pragma unroll
+            for (int k = 0; k < C::MP / 16; ++k) {
+                const f16x8 ah = small_row(A, C::AROW, i0 + lr, k, lk), al = small_row(A, C::AROW, i0 + lr, k, lk + 2), bh = small_row(A, C::AROW, j0 + lr, k, lk), bl = small_row(A, C::AROW, j0 + lr, k, lk + 2);
+                p[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, p[0], 0, 0, 0); p[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh, p[1], 0, 0, 0); p[2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl, p[2], 0, 0, 0);
+            }
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int i = i0 + g * 8 + lk * 4;
+                unpack4(*reinterpret_cast<const f16x4*>(small_at(A, C::AROW, j0 + lr, i, 0)), *reinterpret_cast<const f16x4*>(small_at(A, C::AROW, j0 + lr, i, 1)), E + g * 4);
+            }
+            p[0] += p[1] + p[2]; const float facc = a.poly * inv2;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) p[0][e] = facc * p[0][e] + a.poly_e * E[e];
+        }
+        __syncthreads();
+        if (ks == 0) write(p[0]);
+        __syncthreads();
+        // X <- a X + B X, 32 columns a wave at a time, in place; the last step leaves fp32
+        const float facc = (last ? a.last : a.apply) * inv2, fe_ = last ? a.last_e : a.apply_e;
+        for (int cg = wv; cg < nb / 2; cg += 8) {
+            f16x8 xh[C::MP / 16], xl[C::MP / 16];
+            const int s = lane & 15, g4 = lane >> 4, blk = cg * 2 + (g4 & 1), chunk = (s & 3) >> 1;
+#pragma unroll
+            for (int k = 0; k < C::MP / 16; ++k) {
+                typedef __attribute__((address_space(3))) s16x4* p4; typedef short s16x8 __attribute__((ext_vector_type(8)));
+                s16x4 v[4];
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {                    // rows 0..3 and 4..7 of the lane's eight; hi, lo
+                    const int row = k * 16 + (g4 >> 1) * 8 + (h & 1) * 4 + (s >> 2);
+                    v[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p4)(X + row * S + blk * 64 + (((chunk + (h >> 1) * 2) ^ row_swizzle(row)) << 4) + (s & 1) * 8));
+                }
+                xh[k] = __builtin_bit_cast(f16x8, (s16x8)__builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7)); xl[k] = __builtin_bit_cast(f16x8, (s16x8)__builtin_shufflevector(v[2], v[3], 0, 1, 2, 3, 4, 5, 6, 7));
+            }
+#pragma unroll
+            for (int r = 0; r < MT; ++r) {
+                const int i = r * 32 + lr; f32x16 d[3] = {};
+#pragma unroll
+                for (int k = 0; k < C::MP / 16; ++k) {
+                    const f16x8 bh = small_row(A, C::AROW, i, k, lk), bl = small_row(A, C::AROW, i, k, lk + 2);
+                    d[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xh[k], bh, d[0], 0, 0, 0); d[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xl[k], bh, d[1], 0, 0, 0); d[2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xh[k], bl, d[2], 0, 0, 0);
+                }
+                d[0] += d[1] + d[2];
+                float e4[16];
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int j = cg * 32 + g * 8 + lk * 4;
+                    unpack4(*reinterpret_cast<const f16x4*>(small_at(X, S, i, j, 0)), *reinterpret_cast<const f16x4*>(small_at(X, S, i, j, 1)), e4 + g * 4);
+                }
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int j = cg * 32 + g * 8 + lk * 4; float w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[e] = facc * d[0][g * 4 + e] + fe_ * e4[g * 4 + e];
+                    if (last) *reinterpret_cast<f32x4*>(X + i * S + j * 4) = f32x4{w[0], w[1], w[2], w[3]};
+                    else { f16x4 hi, lo; split4(w, hi, lo); *reinterpret_cast<f16x4*>(small_at(X, S, i, j, 0)) = hi; *reinterpret_cast<f16x4*>(small_at(X, S, i, j, 1)) = lo; }
+                }
+            }
+        }
+        __syncthreads();
+    }
+    const bool turn = D.tall != 0;
+    for (int q0 = 0; q0 < m * n; q0 += 8 * 512) {
+        float old[8]; int64_t o[8]; int at[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int q = q0 + u * 512 + t, i = turn ? q % m : q / n, j = turn ? q / m : q % n;
+            o[u] = q < m * n ? i * ys + j * yl : -1; at[u] = i * S + j * 4;
+            if constexpr (MUON) old[u] = o[u] >= 0 ? reinterpret_cast<const float*>(y)[o[u]] : 0.f;
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (o[u] >= 0) {
+                const float v = ldexpf(*reinterpret_cast<const float*>(X + at[u]), -fq);
+                if constexpr (MUON) reinterpret_cast<float*>(y)[o[u]] = a.decay * old[u] - D.alpha * v; else st_el<DT>(y, o[u], v);
+            }
+    }
+}
+
 // ---- host -------------------------------------------------------------------------------------------------------------------
 // Bounds of what the iteration can meet, from the scalar polynomial on [0, s]: the iterates' singular values, B's, and by how much a step of the pullback can grow G
 struct Plan { bool ok = false; const char* why = ""; double grow = 1, growth[MD2_NS_MAX_STEPS + 1] = {}, s[MD2_NS_MAX_STEPS + 1] = {}, vgain[MD2_NS_MAX_STEPS] = {}; };
@@ -641,17 +836,21 @@ Plan ns_bounds(int steps, const double* co, bool back) {
     if (steps < 1 || steps > MD2_NS_MAX_STEPS) { P.why = "steps must be in 1..16"; return P; }
     const double a = co[0], b = co[1], c = co[2];
     if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) { P.why = "the coefficients must be finite"; return P; }
+    // with u = s^2 everything is a quadratic in u: its largest magnitude on [0, U] is at an end or at the vertex; the iterate's, s (a + b u + c u^2), where a + 3 b u + 5 c u^2 = 0
+    auto most = [](double k0, double k1, double k2, double U) {
+        double r = std::max(std::fabs(k0), std::fabs(k0 + U * (k1 + U * k2))); const double v = k2 != 0 ? -k1 / (2 * k2) : -1;
+        return v > 0 && v < U ? std::max(r, std::fabs(k0 + v * (k1 + v * k2))) : r;
+    };
     double lip[MD2_NS_MAX_STEPS]; P.s[0] = 1.0;
     for (int k = 0; k < steps; ++k) {
-        double top = 0, bm = 0, L = 0, up = 0; const int N = 4096;
-        for (int i = 0; i <= N; ++i) {
-            const double s = P.s[k] * i / N, s2 = s * s, q = b * s2 + c * s2 * s2;
-            top = std::max(top, std::fabs(s * (a + q))); up = std::max(up, std::fabs(a + q)); bm = std::max(bm, std::fabs(q));
-            L = std::max(L, std::max(std::fabs(a + q), std::fabs(a + 3 * b * s2 + 5 * c * s2 * s2)));
-        }
-        P.s[k + 1] = top * 1.01; lip[k] = L * 1.01; P.vgain[k] = std::fabs(b) + 2 * std::fabs(c) * P.s[k] * P.s[k];
+        const double U = P.s[k] * P.s[k]; auto at = [&](double u) { return std::fabs(std::sqrt(u) * (a + u * (b + u * c))); };
+        double top = at(U); const double disc = 9 * b * b - 20 * a * c, den = 10 * c;
+        for (const double u : {den != 0 && disc >= 0 ? (-3 * b + std::sqrt(disc)) / den : -1.0, den != 0 && disc >= 0 ? (-3 * b - std::sqrt(disc)) / den : (b != 0 ? -a / (3 * b) : -1.0)})
+            if (u > 0 && u < U) top = std::max(top, at(u));
+        const double bm = most(0, b, c, U), up = most(a, b, c, U), L = std::max(up, most(a, 3 * b, 5 * c, U));
+        P.s[k + 1] = top * 1.001; lip[k] = L * 1.001; P.vgain[k] = std::fabs(b) + 2 * std::fabs(c) * U;
         if (!(P.s[k + 1] <= 4.0) || !(bm <= 60.0)) { P.why = "these coefficients let a singular value grow past 4 (or b s^2 + c s^4 past 60)"; return P; }
-        P.grow *= std::max(up, 1.0) * 1.01;
+        P.grow *= std::max(up, 1.0) * 1.001;
     }
     P.growth[steps] = 1.0;
     for (int k = steps - 1; k >= 0; --k) P.growth[k] = P.growth[k + 1] * std::max(lip[k], 1.0);
@@ -659,7 +858,6 @@ Plan ns_bounds(int steps, const double* co, bool back) {
     P.ok = true; return P;
 }
 double pow2_below(double v) { return std::exp2(std::floor(std::log2(v))); }
-constexpr double SX = 8192.0, SA = 2048.0, SB = 512.0;            // scales of X (norm <= 4), A (<= 16) and B (<= 60): below 2^15, and f16 ends at 65504
 
 int64_t up(int64_t v, int64_t q) { return (v + q - 1) / q * q; }
 struct Layout { int64_t mats, sym[SYMS], red[SYMS], nn, pk, fac, part, split, buf, total; int64_t n_mats, n_sym[SYMS], n_red[SYMS], n_nn, n_pk; };
@@ -736,10 +934,27 @@ static void slots_of(int kind, int steps, NsProblem& p) {
     if (kind == NS_BACKWARD) { nX = steps + 2; nA = 2 * steps + 2; }      // every iterate and two G | every A, every B, S, V
     else { nX = 2; nA = 2; }                                             // X twice | A, B
 }
+// 1 or 2: every matrix of a forward or Muon call fits Small<1> or Small<2>; 0: the tiled path
+static int ns_small(int kind, const std::vector<Desc>& d) {
+    if (kind == NS_BACKWARD) return 0;
+    bool one = true, two = true;
+    for (const Desc& q : d) { one = one && Small<1>::fits(q.m, q.n); two = two && Small<2>::fits(q.m, q.n); }
+    return one ? 1 : two ? 2 : 0;
+}
+template <int MT, int DT> static void small_launch(int kind, const NsProblem& p, const SmallArgs& a, hipStream_t s) {
+    if (kind == NS_MUON)
+        for (size_t i = 0; i < p.d.size(); i += MUON_DESCS) {
+            SmallPack<MUON_DESCS> dp; const int n = (int)std::min<size_t>(MUON_DESCS, p.d.size() - i);
+            for (int k = 0; k < n; ++k) dp.d[k] = p.d[i + k];
+            hipLaunchKernelGGL((ns_small_kernel<MT, NS_F32, 1, MUON_DESCS>), dim3(n), dim3(512), 0, s, dp, p.st, a);
+        }
+    else { SmallPack<1> dp; dp.d[0] = p.d[0]; hipLaunchKernelGGL((ns_small_kernel<MT, DT, 0, 1>), dim3(p.d[0].batch), dim3(512), 0, s, dp, p.st, a); }
+}
 int64_t ns_workspace(int kind, int steps, const NsMatrices* q, int count) {
     if (steps < 1 || steps > MD2_NS_MAX_STEPS) return -1;
     NsProblem p; slots_of(kind, steps, p);
     for (int i = 0; i < count; ++i) { if (!fits(q[i].batch, q[i].rows, q[i].cols)) return -1; p.d.push_back(make_desc(q[i])); }
+    if (ns_small(kind, p.d)) return 256;                         // (none is used; a caller's buffer is never empty)
     std::stable_sort(p.d.begin(), p.d.end(), [](const Desc& a, const Desc& b) { return a.m > b.m; });
     return check_total(ns_layout(p));
 }
@@ -747,6 +962,13 @@ int64_t ns_workspace(int kind, int steps, const NsMatrices* q, int count) {
 template <int DT> static void ns_launch(int kind, NsProblem& p, const Layout& L, char* base, const NsOptions& o, const Plan& P, hipStream_t s) {
     Ws ws; ws.mats = (Mat*)(base + L.mats); for (int k = 0; k < SYMS; ++k) { ws.sym[k] = (Item*)(base + L.sym[k]); ws.red[k] = (Item*)(base + L.red[k]); } ws.nn = (Item*)(base + L.nn); ws.pk = (Item*)(base + L.pk); ws.fac = (Fac*)(base + L.fac); ws.part = (double*)(base + L.part); ws.split = base + L.split; ws.buf = base + L.buf;
     const int bytes = DT == NS_F32 ? 4 : 2, steps = o.steps;
+    if (const int mt = ns_small(kind, p.d)) {
+        const double a = o.coef[0], b = o.coef[1], c = o.coef[2];
+        SmallArgs q{steps, (float)(SA / (SX * SX)), (float)(c * SB / (SA * SA)), (float)(b * SB / SA), (float)(1.0 / SB), (float)a, (float)(1.0 / (SB * SX)), (float)(a / SX), (float)(1.0 - o.lr * o.weight_decay),
+                    o.eps, P.grow, MuonArgs{(float)o.momentum, o.grad_scale, o.nesterov}, bytes};
+        if (mt == 1) small_launch<1, DT>(kind, p, q, s); else small_launch<2, DT>(kind, p, q, s);
+        return;
+    }
     if (kind == NS_MUON)
         for (size_t i = 0; i < p.d.size(); i += MUON_DESCS) {
             DescPack<MUON_DESCS, 2> dp; const int n = (int)std::min<size_t>(MUON_DESCS, p.d.size() - i);
@@ -840,8 +1062,8 @@ int ns_run(int kind, int dtype, const NsMatrices* q, int count, const NsOptions&
     }
     if (kind != NS_MUON) { const bool tall = p.d[0].tall; const int64_t *x = q[0].xs, *d = q[0].ds; p.st = Strides{x[0], x[tall ? 2 : 1], x[tall ? 1 : 2], d[0], d[tall ? 2 : 1], d[tall ? 1 : 2]}; }
     std::stable_sort(p.d.begin(), p.d.end(), [](const Desc& a, const Desc& b) { return a.m > b.m; });      // the longest work items first
-    const Layout L = ns_layout(p);
-    if (check_total(L) < 0) { *why = "too many matrices"; return 2; }
+    Layout L{}; L.total = 256;
+    if (!ns_small(kind, p.d)) { L = ns_layout(p); if (check_total(L) < 0) { *why = "too many matrices"; return 2; } }
     if (!wsp || (uintptr_t)wsp % 256 || ws_bytes < L.total) { *why = "the workspace is missing, too small or not aligned to 256 bytes"; return 2; }
     if (dtype == NS_F32) ns_launch<NS_F32>(kind, p, L, (char*)wsp, o, P, s);
     else if (dtype == NS_BF16) ns_launch<NS_BF16>(kind, p, L, (char*)wsp, o, P, s);

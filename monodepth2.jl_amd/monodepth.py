@@ -10,7 +10,9 @@ float32 tensors whose shape is the REVERSE of the Julia shape (same bytes): Juli
 torch is used only for device memory, streams and torch.distributed; every computation is a HIP kernel
 of libmd2hip.so.  There is no CPU path: without the library / a GPU every call raises.
 """
+import contextlib
 import ctypes as C
+import math
 from dataclasses import dataclass, field
 from typing import List, Optional, Tuple
 
@@ -834,7 +836,8 @@ def _ns_matrices(x, what):
     """-> (x as (batch, rows, cols), a view where its strides allow one, dtype code)."""
     if not (torch.is_tensor(x) and x.is_cuda and x.dtype in _NS_DTYPES and x.dim() >= 2):
         raise ValueError("%s: expected a CUDA tensor (..., rows, cols) of float32, bfloat16 or float16 (the product path has no CPU fallback)" % what)
-    return x.detach().reshape((int(np.prod(x.shape[:-2], dtype=np.int64)),) + tuple(x.shape[-2:])), _NS_DTYPES[x.dtype]
+    s = x.shape
+    return (x if x.dim() == 3 else x.unsqueeze(0) if x.dim() == 2 else x.detach().reshape(math.prod(s[:-2]), s[-2], s[-1])), _NS_DTYPES[x.dtype]
 
 
 def _ns_workspace(nbytes, device, what):
@@ -843,11 +846,22 @@ def _ns_workspace(nbytes, device, what):
     return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
+_F64x3, _I64x3 = C.c_double * 3, C.c_int64 * 3
+_NS_DEFAULT = _F64x3(*NS_COEFFICIENTS)
+
+
 def _ns_args(steps, coefficients, eps):
+    if coefficients == NS_COEFFICIENTS:
+        return int(steps), _NS_DEFAULT, float(eps)
     co = tuple(float(c) for c in coefficients)
     if len(co) != 3:
         raise ValueError("coefficients: expected (a, b, c)")
-    return int(steps), (C.c_double * 3)(*co), float(eps)
+    return int(steps), _F64x3(*co), float(eps)
+
+
+def _on(device):
+    """The context in which `device` is the current one (nothing to do where it is)."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def newton_schulz(x, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7):
@@ -857,9 +871,9 @@ def newton_schulz(x, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7):
     if y.numel() == 0:
         return y
     B, R, K = x3.shape; L = _lib.lib()
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         ws = _ns_workspace(L.md2_newton_schulz_workspace(B, R, K, st, 0), x.device, "newton_schulz")
-        _check(L.md2_newton_schulz(x3.data_ptr(), y.data_ptr(), B, R, K, (C.c_int64 * 3)(*x3.stride()), dt, st, co, ep, ws.data_ptr(), ws.numel(), _stream()), None, "newton_schulz")
+        _check(L.md2_newton_schulz(x3.data_ptr(), y.data_ptr(), B, R, K, _I64x3(*x3.stride()), dt, st, co, ep, ws.data_ptr(), ws.numel(), _stream()), None, "newton_schulz")
     return y
 
 
@@ -872,9 +886,9 @@ def newton_schulz_pullback(x, dout, steps=5, coefficients=NS_COEFFICIENTS, eps=1
     if dx.numel() == 0:
         return dx
     B, R, K = x3.shape; L = _lib.lib()
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         ws = _ns_workspace(L.md2_newton_schulz_workspace(B, R, K, st, 1), x.device, "newton_schulz_pullback")
-        _check(L.md2_newton_schulz_bwd(x3.data_ptr(), d3.data_ptr(), dx.data_ptr(), B, R, K, (C.c_int64 * 3)(*x3.stride()), (C.c_int64 * 3)(*d3.stride()), dt, st, co, ep, ws.data_ptr(), ws.numel(),
+        _check(L.md2_newton_schulz_bwd(x3.data_ptr(), d3.data_ptr(), dx.data_ptr(), B, R, K, _I64x3(*x3.stride()), _I64x3(*d3.stride()), dt, st, co, ep, ws.data_ptr(), ws.numel(),
                                        _stream()), None, "newton_schulz_bwd")
     return dx
 
@@ -888,20 +902,22 @@ def muon_raw(params, grads, momenta, lr=0.02, momentum=0.95, nesterov=True, weig
         raise ValueError("muon_raw: params, grads and momenta must be lists of one length")
     if adjust not in _MUON_ADJUST:
         raise ValueError("muon_raw: adjust must be 'spectral' or 'rms'")
-    st, co, ep = _ns_args(steps, coefficients, eps); keep = []
+    st, co, ep = _ns_args(steps, coefficients, eps); keep = []; dev = params[0].device if n else None
     for p, g, m in zip(params, grads, momenta):
         for t in (p, g, m):
-            _dev(t)
+            if not (t.is_cuda and t.dtype == torch.float32 and t.is_contiguous()):
+                _dev(t)                                       # (raises)
         if p.dim() < 2 or g.shape != p.shape or m.shape != p.shape:
             raise ValueError("muon_raw: a weight needs two or more dimensions, and a gradient and a momentum of its shape (got %s, %s, %s)" % (tuple(p.shape), tuple(g.shape), tuple(m.shape)))
-        if not (p.device == g.device == m.device == params[0].device):
+        if not (p.device == dev and g.device == dev and m.device == dev):
             raise ValueError("muon_raw: every tensor must be on one device")
-        if p.numel():
-            keep.append((p.data_ptr(), g.data_ptr(), m.data_ptr(), p.shape[0], p.numel() // p.shape[0]))
+        k = p.numel()
+        if k:
+            keep.append((p.data_ptr(), g.data_ptr(), m.data_ptr(), p.shape[0], k // p.shape[0]))
     if not keep:
         return
-    n = len(keep); P, G, M, R, K = zip(*keep); R, K = (C.c_int64 * n)(*R), (C.c_int64 * n)(*K); L = _lib.lib(); dev = params[0].device
-    with torch.cuda.device(dev):
+    n = len(keep); P, G, M, R, K = zip(*keep); R, K = (C.c_int64 * n)(*R), (C.c_int64 * n)(*K); L = _lib.lib()
+    with _on(dev):
         ws = _ns_workspace(L.md2_muon_workspace(R, K, n, st), dev, "muon_raw")
         _check(L.md2_muon_raw((C.c_void_p * n)(*P), (C.c_void_p * n)(*G), (C.c_void_p * n)(*M), R, K, n, float(lr), float(momentum), int(bool(nesterov)), float(weight_decay),
                               _MUON_ADJUST[adjust], float(grad_scale), st, co, ep, ws.data_ptr(), ws.numel(), _stream()), None, "muon_raw")

@@ -126,7 +126,8 @@ def test_two_weights_may_share_a_gradient():
 
 
 # ---- newton_schulz ------------------------------------------------------------------------------------------------------------
-SHAPES = [(1, 1), (1, 7), (9, 1), (2, 2), (16, 16), (31, 33), (64, 64), (65, 64), (64, 576), (127, 130), (128, 128), (129, 129), (200, 77), (33, 1000), (130, 300), (257, 96), (256, 640), (385, 514)]
+SHAPES = [(1, 1), (1, 7), (9, 1), (2, 2), (16, 16), (31, 33), (64, 64), (65, 64), (64, 576), (127, 130), (128, 128), (129, 129), (200, 77), (33, 1000), (130, 300), (257, 96), (256, 640), (385, 514),
+          (32, 1152), (32, 1153), (1153, 20), (64, 512), (513, 64), (61, 511), (5, 1000), (700, 130), (1000, 1100)]      # (the first six: both sides of what a workgroup keeps in LDS)
 
 
 def check(y, x, steps=5, coef=COEF, eps=1e-7, name=""):
@@ -308,15 +309,24 @@ def test_muon_raw(kw):
 
 
 @gpu
-def test_muon_raw_list_order_and_company_do_not_matter():
-    m = md(); shapes = [(70, 90), (16, 40), (130, 64), (200, 200)] * 9                   # 36 weights: more than one argument block of the set-up kernel
+def test_muon_raw_list_order_and_company():
+    """A list in another order gives the same bits.  Alone, a weight may take other tiles (sums in another order): both results are within 2e-5 of the step of the exact one (as above)."""
+    m = md(); shapes = [(70, 90), (16, 40), (130, 64), (200, 200)] * 11                  # 44 weights: more than one argument block of the set-up kernel
     def make():
         return [[gradient_like(s, i + 100 * k).float().cuda() for i, s in enumerate(shapes)] for k in range(3)]
-    a, b = make(), make()
+    a, b, c = make(), make(), make(); start = [p.clone() for p in a[0]]
     m.muon_raw(*a)
-    for i in reversed(range(len(shapes))):
-        m.muon_raw([b[0][i]], [b[1][i]], [b[2][i]])
+    m.muon_raw(b[0][::-1], b[1][::-1], b[2][::-1])
     assert all(torch.equal(x, y) for k in (0, 2) for x, y in zip(a[k], b[k]))
+    for i in range(len(shapes)):
+        m.muon_raw([c[0][i]], [c[1][i]], [c[2][i]])
+        step = float((a[0][i] - start[i]).norm())
+        assert torch.equal(a[2][i], c[2][i]) and float((a[0][i].double() - c[0][i].double()).norm()) <= 4 * 2.0 ** -24 * (float(start[i].norm()) + step) + 4e-5 * step
+    small = [[gradient_like((17, 5 + i), i + 100 * k).float().cuda() for i in range(80)] for k in range(3)]; one = [[t.clone() for t in l] for l in small]
+    m.muon_raw(*small)                                                                   # 80 weights that fit a workgroup each: three launches
+    for i in range(80):
+        m.muon_raw([one[0][i]], [one[1][i]], [one[2][i]])
+    assert all(torch.equal(x, y) for k in (0, 2) for x, y in zip(small[k], one[k]))
     m.muon_raw([], [], [])
     with pytest.raises(ValueError):
         m.muon_raw([a[0][0].t()], [a[1][0].t()], [a[2][0].t()])
