@@ -68,7 +68,7 @@ struct Ws { Mat* mats; Item *sym[SYMS], *red[SYMS], *nn, *pk; Fac* fac; double* 
 __host__ __device__ inline int cdiv(int a, int b) { return (a + b - 1) / b; }
 __host__ __device__ inline int kblocks(int kind, int m, int n) { return (kind >= SYM_S ? 2 : 1) * cdiv(kind == GRAM || kind == SYM_S ? n : m, 16); }
 
-struct Cuts { Cut sym[SYMS]; int32_t nn_tile; };
+struct Cuts { Cut sym[SYMS]; int32_t nn_tile, fuse; };           // fuse: every short side is at most 64 (sym_whole): 64-tiles throughout, GRAM and SYM_S do POLY's and SYM_V's work
 // Workgroup b runs on XCD b % 8, each with an L2 of its own.  Of `groups` groups of `size` items, the items of one share an operand: eight groups at a time are dealt to the XCDs, a group
 // to one.  -> the place of item `i` of group `g` (the last groups, fewer than eight, are dealt among themselves)
 __device__ inline int dealt(int g, int i, int groups, int size) {
@@ -433,7 +433,15 @@ __device__ inline void store_pair8(char* p, const float v[8]) {
     *reinterpret_cast<f16x8*>(p) = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7); *reinterpret_cast<f16x8*>(p + LO) = __builtin_shufflevector(l[0], l[1], 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-struct SymArgs { Slot l[2], r[2], e, out; int kind, nseg, have_e; float acc, ecoef; };      // out = acc * (sum of l r^T) + ecoef * e, in the buffers' own scales (with e: a factor A too many)
+__device__ inline void unpack4(const f16x4 h, const f16x4 l, float v[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = (float)h[e] + (float)l[e];
+}
+// four neighbouring columns (j a multiple of 4) of a swizzled LDS row
+__device__ inline char* small_at(char* rows, int stride, int i, int j, int lo) { return rows + i * stride + (((j >> 4) ^ (i & 3)) << 6) + (((((j & 15) >> 3) + lo * 2) ^ row_swizzle(i)) << 4) + (j & 4) * 2; }
+__device__ inline f16x8 small_row(const char* rows, int stride, int i, int block, int chunk) { return *reinterpret_cast<const f16x8*>(rows + i * stride + ((block ^ (i & 3)) << 6) + ((chunk ^ row_swizzle(i)) << 4)); }
+
+struct SymArgs { Slot l[2], r[2], e, out; int kind, nseg, have_e; float acc, ecoef; Slot with, then; int fuse; float acc2, ecoef2; };      // out = acc * (sum of l r^T) + ecoef * e, in the buffers' own scales (with e: a factor A too many)
 __device__ inline void unpack8(const f16x8 h, const f16x8 l, float v[8]) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = (float)h[e] + (float)l[e];
@@ -471,6 +479,44 @@ template <int T, int R> __device__ inline void sym_finish(const Item& it, const 
         }
     }
 }
+// Short sides of at most 64: the workgroup that has all of A goes on to B = b A + c A A (and from S to V = b S + c (S A + A S), `with` being A), which saves a launch.  lds: 32 KB
+__device__ inline void sym_whole(char* lds, const Item& it, const SymArgs& a, const Fac* facs, const float* tile, int planes) {
+    const int t = threadIdx.x, lane = t & 63, lr = lane & 31, lk = lane >> 5, i0 = (t >> 7) * 32, j0 = ((t >> 6) & 1) * 32; const Dims d = dims(it);
+    char *first = lds, *second = a.kind == SYM_S ? lds + 16384 : first, *out = slot(it, d, a.out), *then = slot(it, d, a.then); const char* with = slot(it, d, a.with); const float inv2 = facs[it.mat].inv2;
+#pragma unroll
+    for (int z = 0; z < 2; ++z) {
+        const int r = z * 32 + t / 8, c = t % 8 * 8; const int64_t o = pair_off(d.arb, r, c); float v[8];
+        if (a.kind == SYM_S) { *reinterpret_cast<f16x8*>(small_at(second, 256, r, c, 0)) = *reinterpret_cast<const f16x8*>(with + o); *reinterpret_cast<f16x8*>(small_at(second, 256, r, c, 1)) = *reinterpret_cast<const f16x8*>(with + o + LO); }
+        tile_row8<64>(tile, planes, r, c, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= a.acc;
+        f16x4 h[2], l[2]; split4(v, h[0], l[0]); split4(v + 4, h[1], l[1]);
+        const f16x8 hi = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7), lo = __builtin_shufflevector(l[0], l[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        *reinterpret_cast<f16x8*>(small_at(first, 256, r, c, 0)) = hi; *reinterpret_cast<f16x8*>(small_at(first, 256, r, c, 1)) = lo;
+        if (a.kind == GRAM) { *reinterpret_cast<f16x8*>(out + o) = hi; *reinterpret_cast<f16x8*>(out + o + LO) = lo; }      // (the pullback reads A again; S goes no further)
+    }
+    __syncthreads();
+    f32x16 c[3] = {};
+    auto add = [&](const char* L, const char* R) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const f16x8 ah = small_row(L, 256, i0 + lr, k, lk), al = small_row(L, 256, i0 + lr, k, lk + 2), bh = small_row(R, 256, j0 + lr, k, lk), bl = small_row(R, 256, j0 + lr, k, lk + 2);
+            c[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, c[0], 0, 0, 0); c[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh, c[1], 0, 0, 0); c[2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl, c[2], 0, 0, 0);
+        }
+    };
+    add(first, second);
+    if (a.kind == SYM_S) add(second, first);
+    c[0] += c[1] + c[2];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {                                // lane: row j0 + lr, registers: four neighbouring columns (the result is symmetric)
+        const int i = i0 + g * 8 + lk * 4, j = j0 + lr; const int64_t o = pair_off(d.arb, j, i); float x[4], v[4]; f16x4 hi, lo;
+        unpack4(*reinterpret_cast<const f16x4*>(small_at(first, 256, j, i, 0)), *reinterpret_cast<const f16x4*>(small_at(first, 256, j, i, 1)), x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = a.acc2 * inv2 * c[0][g * 4 + e] + a.ecoef2 * x[e];
+        split4(v, hi, lo);
+        *reinterpret_cast<f16x4*>(then + o) = hi; *reinterpret_cast<f16x4*>(then + o + LO) = lo;
+    }
+}
 template <int T> __device__ inline void sym_tile(char* lds, const Item& it, const Ws& ws, const SymArgs& a) {
     const Dims d = dims(it); const bool kn = a.kind == GRAM || a.kind == SYM_S; const int64_t rb = kn ? d.xrb : d.arb;
     Seg seg[2];
@@ -479,7 +525,8 @@ template <int T> __device__ inline void sym_tile(char* lds, const Item& it, cons
     f32x16 c[2][2] = {};
     product<T, false>(lds, seg, a.nseg == 2 ? cdiv(kn ? it.n : it.m, 16) : 1 << 30, it.k0, it.k1, 1.f, c);
     float* tile = reinterpret_cast<float*>(lds); tile_store<T>(tile, c);
-    if (it.part < 0) sym_finish<T, T>(it, a, ws.fac, tile, 4, 0);
+    if (T == 64 && it.part < 0 && a.fuse) sym_whole(lds + 65536, it, a, ws.fac, tile, 4);
+    else if (it.part < 0) sym_finish<T, T>(it, a, ws.fac, tile, 4, 0);
     else {
         constexpr int PER = T / 8; float* out = reinterpret_cast<float*>(ws.split + (int64_t)it.part * PART);
 #pragma unroll 2
@@ -495,11 +542,11 @@ template <int T> __global__ __launch_bounds__(256, T == 128 ? 2 : 1) void ns_sym
     const Item it = ws.sym[a.kind][blockIdx.x];
     sym_tile<T>(lds, it, ws, a);
 }
-// the shares of a tile, summed in order: 32 rows of it a workgroup
+// the shares of a tile, summed in order: 16 rows of a 128-tile or 32 of a 64-tile a workgroup (8 KB of each share)
 template <int T> __device__ inline void reduce_tile(float* tile, const Item& it, const Ws& ws, const SymArgs& a, int r0) {
-    constexpr int N = 32 * T / 8 / 256; const float* in = reinterpret_cast<const float*>(ws.split + (int64_t)it.part * PART) + r0 * T + threadIdx.x * 8;
+    constexpr int R = 2048 / T, N = 1; const float* in = reinterpret_cast<const float*>(ws.split + (int64_t)it.part * PART) + r0 * T + threadIdx.x * 8;
     f32x4 v[N][2] = {};
-#pragma unroll 4
+#pragma unroll 8
     for (int k = 0; k < it.k1; ++k)
 #pragma unroll
         for (int z = 0; z < N; ++z)
@@ -510,12 +557,31 @@ template <int T> __device__ inline void reduce_tile(float* tile, const Item& it,
 #pragma unroll
         for (int h = 0; h < 2; ++h) *reinterpret_cast<f32x4*>(tile + tile_at<T>((z * 256 + threadIdx.x) / (T / 8), threadIdx.x % (T / 8) * 8 + h * 4)) = v[z][h];
     __syncthreads();
-    sym_finish<T, 32>(it, a, ws.fac, tile, 1, r0);
+    sym_finish<T, R>(it, a, ws.fac, tile, 1, r0);
 }
 template <int T> __global__ __launch_bounds__(256) void ns_reduce_kernel(Ws ws, SymArgs a) {
-    __shared__ __attribute__((aligned(16))) float tile[32 * T];
-    const Item it = ws.red[a.kind][blockIdx.x / (T / 32)];
-    reduce_tile<T>(tile, it, ws, a, blockIdx.x % (T / 32) * 32);
+    __shared__ __attribute__((aligned(16))) float tile[2048]; constexpr int SLABS = T * T / 2048;
+    const Item it = ws.red[a.kind][blockIdx.x / SLABS];
+    reduce_tile<T>(tile, it, ws, a, blockIdx.x % SLABS * (2048 / T));
+}
+
+// the shares of a whole short side (at most 64), and on to the product with it
+__global__ __launch_bounds__(256) void ns_reduce_whole_kernel(Ws ws, SymArgs a) {
+    __shared__ __attribute__((aligned(16))) char lds[16384 + 32768];
+    const Item it = ws.red[a.kind][blockIdx.x]; float* tile = reinterpret_cast<float*>(lds); const float* in = reinterpret_cast<const float*>(ws.split + (int64_t)it.part * PART) + threadIdx.x * 8;
+    f32x4 v[2][2] = {};
+#pragma unroll 4
+    for (int k = 0; k < it.k1; ++k)
+#pragma unroll
+        for (int z = 0; z < 2; ++z)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) v[z][h] += *reinterpret_cast<const f32x4*>(in + (int64_t)k * 4096 + z * 2048 + h * 4);
+#pragma unroll
+    for (int z = 0; z < 2; ++z)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) *reinterpret_cast<f32x4*>(tile + tile_at<64>(z * 32 + threadIdx.x / 8, threadIdx.x % 8 * 8 + h * 4)) = v[z][h];
+    __syncthreads();
+    sym_whole(lds + 16384, it, a, ws.fac, tile, 1);
 }
 
 enum { OUT_PAIR = 0, OUT_Y = 1, OUT_MUON = 2, OUT_BACK = 3 };
@@ -554,7 +620,7 @@ template <int T, int DT, int OUT> __device__ inline void nn_tile(char* lds, doub
         else if constexpr (OUT == OUT_BACK) {                    // G in fp32, and this tile's share of <X0, G>
             unpack8(xh[z], xl[z], x);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) dot += (double)x[e] * (double)v[e];
+            for (int e = 0; e < 8; ++e) dot += i < it.m ? (double)x[e] * (double)v[e] : 0.0;      // (rows behind the last may hold anything: 64-tiles of B and V do not cover 128)
             float* w = reinterpret_cast<float*>(slot(it, d, a.out) + i * d.xrb + (int64_t)j * 4);
             *reinterpret_cast<f32x4*>(w) = f32x4{v[0], v[1], v[2], v[3]}; *reinterpret_cast<f32x4*>(w + 4) = f32x4{v[4], v[5], v[6], v[7]};
         } else if (OUT == OUT_MUON && rows) {
@@ -637,29 +703,21 @@ template <int DT> __global__ __launch_bounds__(256) void ns_back_finish_kernel(W
 // ---- small matrices: a workgroup each, everything in LDS --------------------------------------------------------------------
 // A call whose matrices all fit (short side MP = 32 or 64, pairs of X and A within 160 KB) is one launch: eight waves keep X in LDS from the first read to the result.  The launches of the
 // tiled path cost 5 - 6 us each whatever the size; its 18 for a 64 x 64 matrix took 106 us.
-// LDS rows are an odd multiple of 64 bytes off a multiple of 256, and swizzled as the ring's, so that the products' row reads meet every bank.
+// LDS rows are multiples of 256 bytes; row i's blocks of 64 are stored at block ^ (i & 3) and their chunks swizzled as the ring's, so that the products' row reads meet every bank.
 template <int MT> struct Small {
-    static constexpr int MP = MT * 32, TILES = MT * MT, KS = MT == 1 ? 4 : 2, AROW = 320, AB = MT == 1 ? 12288 : MP * AROW, LDS = 163840;      // KS: waves that share a Gram tile's K axis
+    static constexpr int MP = MT * 32, TILES = MT * MT, KS = MT == 1 ? 4 : 2, AROW = MT == 1 ? 256 : MP * 4, AB = MT == 1 ? 12288 : MP * AROW, LDS = 163840;      // KS: waves that share a Gram tile's K axis
     __host__ __device__ static int blocks(int n) { return cdiv(n, 32) * 2; }                            // 16-column blocks of a row
-    __host__ __device__ static int row(int n) { const int b = blocks(n); return (b + (5 - b % 4) % 4) * 64; }      // bytes of a row
-    __host__ static bool fits(int m, int n) { return m <= MP && (int64_t)MP * row(n) + AB + 256 <= LDS; }
+    __host__ __device__ static int row(int n) { return cdiv(n, 64) * 256; }      // bytes of a row
+    __host__ static bool fits(int m, int n) { return m <= MP && (int64_t)MP * row(n) + AB <= LDS; }
 };
 struct SmallArgs { int steps; float gram, poly, poly_e, apply, apply_e, last, last_e, decay; double eps, grow; MuonArgs mu; int dt_bytes; };
 template <int N> struct SmallPack { Desc d[N]; };
-__device__ inline void unpack4(const f16x4 h, const f16x4 l, float v[4]) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = (float)h[e] + (float)l[e];
-}
-// four neighbouring columns (j a multiple of 4) of a swizzled LDS row
-__device__ inline char* small_at(char* rows, int stride, int i, int j, int lo) { return rows + i * stride + (j >> 4) * 64 + (((((j & 15) >> 3) + lo * 2) ^ row_swizzle(i)) << 4) + (j & 4) * 2; }
-__device__ inline f16x8 small_row(const char* rows, int stride, int i, int block, int chunk) { return *reinterpret_cast<const f16x8*>(rows + i * stride + block * 64 + ((chunk ^ row_swizzle(i)) << 4)); }
-
 template <int MT, int DT, int MUON, int N> __global__ __launch_bounds__(512) void ns_small_kernel(SmallPack<N> dp, Strides st, SmallArgs a) {
     using C = Small<MT>;
     __shared__ __attribute__((aligned(16))) char lds[C::LDS];
     const Desc& D = dp.d[N == 1 ? 0 : blockIdx.x]; const int b = N == 1 ? blockIdx.x : 0, m = D.m, n = D.n, nb = C::blocks(n), S = C::row(n);
     const int t = threadIdx.x, lane = t & 63, wv = t >> 6, lr = lane & 31, lk = lane >> 5;
-    char *X = lds, *A = lds + C::MP * S; double* red = reinterpret_cast<double*>(lds + C::LDS - 256);
+    char *X = lds, *A = lds + C::MP * S; double* red = reinterpret_cast<double*>(A);
     const int64_t ys = D.tall ? 1 : n, yl = D.tall ? m : 1, ss = N == 1 ? st.xs : ys, sl = N == 1 ? st.xl : yl;
     const char* src = (const char*)D.x + (N == 1 ? st.xb * b * a.dt_bytes : 0); char* y = (char*)D.y + (int64_t)m * n * b * a.dt_bytes;
     const bool along = !(ss == 1 && sl != 1);                    // neighbouring lanes along the long side
@@ -670,7 +728,7 @@ template <int MT, int DT, int MUON, int N> __global__ __launch_bounds__(512) voi
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
             const int q = q0 + u * 512 + t, i = along ? q / cols : q % C::MP, j = along ? q % cols : q / C::MP;
-            at[u] = q < all ? i * S + j * 4 : -1; o[u] = q < all && i < m && j < n ? i * ss + j * sl : -1;      // (16 columns of fp32 take the 64 bytes of their block)
+            at[u] = q < all ? i * S + (((j >> 4) ^ (i & 3)) << 6) + (j & 15) * 4 : -1; o[u] = q < all && i < m && j < n ? i * ss + j * sl : -1;      // (16 columns of fp32 take the 64 bytes of their block)
             x[u] = o[u] >= 0 ? ld_el<DT>(src, o[u]) : 0.f;
             if constexpr (MUON) g[u] = o[u] >= 0 ? reinterpret_cast<const float*>(D.d)[o[u]] : 0.f;
         }
@@ -694,7 +752,7 @@ template <int MT, int DT, int MUON, int N> __global__ __launch_bounds__(512) voi
     if (norm <= a.eps && norm > 0) { const double room = 4.0 * a.eps / (norm * a.grow); if (room >= 2.0) fq = ilogb(room); }      // (as in ns_pack_kernel)
     const float inv2 = (float)ldexp(1.0, -2 * fq); int fe; const float f = (float)frexp(ldexp(SX, fq) / (norm <= a.eps ? a.eps : norm), &fe);
     for (int q = t; q < C::MP * nb; q += 512) {                  // a block of 16 columns a thread
-        const int i = q / nb, blk = q % nb; char* p = X + i * S + blk * 64; f32x4 r[4];
+        const int i = q / nb, blk = q % nb; char* p = X + i * S + ((blk ^ (i & 3)) << 6); f32x4 r[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) r[k] = *reinterpret_cast<const f32x4*>(p + k * 16);
 #pragma unroll
@@ -779,7 +837,7 @@ template <int MT, int DT, int MUON, int N> __global__ __launch_bounds__(512) voi
 #pragma unroll
                 for (int h = 0; h < 4; ++h) {                    // rows 0..3 and 4..7 of the lane's eight; hi, lo
                     const int row = k * 16 + (g4 >> 1) * 8 + (h & 1) * 4 + (s >> 2);
-                    v[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p4)(X + row * S + blk * 64 + (((chunk + (h >> 1) * 2) ^ row_swizzle(row)) << 4) + (s & 1) * 8));
+                    v[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p4)(X + row * S + ((blk ^ (row & 3)) << 6) + (((chunk + (h >> 1) * 2) ^ row_swizzle(row)) << 4) + (s & 1) * 8));
                 }
                 xh[k] = __builtin_bit_cast(f16x8, (s16x8)__builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7)); xl[k] = __builtin_bit_cast(f16x8, (s16x8)__builtin_shufflevector(v[2], v[3], 0, 1, 2, 3, 4, 5, 6, 7));
             }
@@ -803,7 +861,7 @@ template <int MT, int DT, int MUON, int N> __global__ __launch_bounds__(512) voi
                     const int j = cg * 32 + g * 8 + lk * 4; float w[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) w[e] = facc * d[0][g * 4 + e] + fe_ * e4[g * 4 + e];
-                    if (last) *reinterpret_cast<f32x4*>(X + i * S + j * 4) = f32x4{w[0], w[1], w[2], w[3]};
+                    if (last) *reinterpret_cast<f32x4*>(X + i * S + (((j >> 4) ^ (i & 3)) << 6) + (j & 15) * 4) = f32x4{w[0], w[1], w[2], w[3]};
                     else { f16x4 hi, lo; split4(w, hi, lo); *reinterpret_cast<f16x4*>(small_at(X, S, i, j, 0)) = hi; *reinterpret_cast<f16x4*>(small_at(X, S, i, j, 1)) = lo; }
                 }
             }
@@ -816,7 +874,7 @@ template <int MT, int DT, int MUON, int N> __global__ __launch_bounds__(512) voi
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
             const int q = q0 + u * 512 + t, i = turn ? q % m : q / n, j = turn ? q / m : q % n;
-            o[u] = q < m * n ? i * ys + j * yl : -1; at[u] = i * S + j * 4;
+            o[u] = q < m * n ? i * ys + j * yl : -1; at[u] = i * S + (((j >> 4) ^ (i & 3)) << 6) + (j & 15) * 4;
             if constexpr (MUON) old[u] = o[u] >= 0 ? reinterpret_cast<const float*>(y)[o[u]] : 0.f;
         }
 #pragma unroll
@@ -866,28 +924,38 @@ struct Layout { int64_t mats, sym[SYMS], red[SYMS], nn, pk, fac, part, split, bu
 
 struct NsProblem { std::vector<Desc> d; std::vector<Use> u; Strides st{}; int nX, nA, kinds; Cuts cuts{}; };      // u: [weight][kinds]
 
-// Tiles and splits of a call's products, from its sizes alone.
-// 128-tiles share a staged row between two waves (half the loads of 64-tiles, whose four waves split K instead), so they are taken wherever they occupy half the CUs, counting a long K axis
-// as pieces of MIN128 blocks of 16.  The K axis is cut where that makes the launch shorter by this model: a CU has its share of the workgroups, a step of one costs STEP us (the rate of two a CU), and
-// a cut K axis costs a second launch and its partial sums' way to memory and back.
-static constexpr int CUS = 256, MIN128 = 16, MIN64 = 64;
-static constexpr double STEP = 0.4, LAUNCH = 6.0, PART_US = 64.0 * 1024 * 2 / 3.0e6;      // us; a 64 KB partial sum written and read at 3 TB/s
+// Tiles and splits of a call's products, from its sizes alone, by a model of a launch.
+// 128-tiles share a staged row between two waves (half the loads of 64-tiles, whose four waves split K instead) and are the faster ones where they fill the chip; a call with few tiles is over
+// sooner in 64-tiles, and sooner still with its K axis cut.  Measured: a block of 16 K takes a 128-tile 0.4 us at two workgroups a CU and 0.5 alone, a 64-tile 0.14 (a step of its waves,
+// 0.55, is four blocks) and 0.22 where the chip is full of them (their loads); a workgroup's way in and out is 4 us, which two 128-tiles a CU hide from each other; a cut K axis costs a launch of 5 us and its partial sums' way through memory.
+// (512 x 4608, X X^T: 180 128-tile pieces 13 us and 6 to join them, 36 64-tiles uncut 32; B X: 144 128-tiles 19.5, 576 64-tiles 23.  512 x 2304, B X: 72 128-tiles 20, 288 64-tiles 15.)
+static constexpr int CUS = 256, MIN128 = 16, MIN64 = 16;
+static constexpr double LAUNCH = 5.0, PART_US = 64.0 * 1024 * 2 / 5.0e6;
+static double launch_us(int tile, int64_t items, int64_t work, int64_t longest, bool equal) {      // items, their K blocks in all, the longest one's; equal: they come in whole rounds
+    const double rounds = (double)items / CUS, whole = equal && items > CUS ? std::ceil(rounds) : rounds;
+    if (tile == 64) return std::max(std::max(longest * 0.14 + 4.0, equal ? std::ceil(rounds) * (longest * 0.14 + 4.0) : rounds * 4.0 + work * 0.14 / CUS), work * 0.22 / CUS + 4.0);
+    return std::max(longest * (items <= CUS ? 0.5 : 0.8) + 4.0, (work * 0.4 / CUS + rounds * 2.0) * (rounds > 0 ? whole / rounds : 1.0));      // (0.8: beside another one)
+}
 static int64_t tri(int64_t m, int tile) { const int64_t t = (m + tile - 1) / tile; return t * (t + 1) / 2; }
 static Layout ns_layout(NsProblem& p) {
     Layout L{}; p.u.assign(p.d.size() * p.kinds, Use{});
-    int64_t buf = 0, split_max = 0;
+    int64_t buf = 0, split_max = 0; int widest = 0;
+    for (const Desc& d : p.d) widest = std::max(widest, d.m);
+    p.cuts.fuse = widest <= 64;
     for (int kind = 0; kind < p.kinds; ++kind) {
-        int64_t pieces = 0, part = 0; int most = 1;
-        for (const Desc& d : p.d) { const int kb = kblocks(kind, d.m, d.n); pieces += d.batch * tri(d.m, 128) * cdiv(kb, MIN128); most = std::max(most, kb); }
-        const int tile = pieces >= CUS / 2 ? 128 : 64, least = tile == 128 ? MIN128 : MIN64;
-        int chunk = most; double best = 1e30;
-        for (int c = most;; c = std::max(least, std::min(c - 1, c * 7 / 8))) {
-            int64_t items = 0, parts = 0; 
-            for (const Desc& d : p.d) { const int64_t t = d.batch * tri(d.m, tile), sp = cdiv(kblocks(kind, d.m, d.n), c); items += t * sp; if (sp > 1) parts += t * sp; }
-            const double us = (double)((items + CUS - 1) / CUS) * std::min(c, most) * STEP / (tile == 128 ? 1 : 4) + (parts ? LAUNCH : 0) + parts * PART_US / (tile == 128 ? 1 : 4);
-            if (us < best) { best = us; chunk = c; }
-            if (c <= least) break;
-        }
+        int64_t part = 0; int most = 1, tile = 64, chunk = 1; double best = 1e30; const bool equal = p.d.size() == 1;
+        for (const Desc& d : p.d) most = std::max(most, kblocks(kind, d.m, d.n));
+        for (const int T : {128, 64})
+            for (int c = most; T == 64 || !p.cuts.fuse; c = std::max(T == 128 ? MIN128 : MIN64, std::min(c - 1, c * 7 / 8))) {
+                int64_t items = 0, parts = 0, work = 0, longest = 0;
+                for (const Desc& d : p.d) {
+                    const int kb = kblocks(kind, d.m, d.n), sp = cdiv(kb, c); const int64_t t = d.batch * tri(d.m, T);
+                    items += t * sp; work += t * kb; longest = std::max<int64_t>(longest, cdiv(kb, sp)); if (sp > 1) parts += t * sp;
+                }
+                const double us = launch_us(T, items, work, longest, equal) + (parts ? LAUNCH : 0) + parts * PART_US / (T == 128 ? 1 : 4);
+                if (us < best) { best = us; tile = T; chunk = c; }
+                if (c <= (T == 128 ? MIN128 : MIN64)) break;
+            }
         p.cuts.sym[kind] = Cut{tile, chunk};
         for (size_t i = 0; i < p.d.size(); ++i) {
             const Desc& d = p.d[i]; Use& u = p.u[i * p.kinds + kind]; const int kb = kblocks(kind, d.m, d.n), split = cdiv(kb, cdiv(kb, cdiv(kb, chunk))); const int64_t tiles = d.batch * tri(d.m, tile);
@@ -897,9 +965,13 @@ static Layout ns_layout(NsProblem& p) {
         }
         split_max = std::max(split_max, part);
     }
-    int64_t nn128 = 0;
-    for (const Desc& d : p.d) nn128 += (int64_t)d.batch * cdiv(d.m, 128) * cdiv(d.n, 128);
-    p.cuts.nn_tile = nn128 >= CUS / 2 ? 128 : 64;
+    double nn[2];
+    for (const int T : {128, 64}) {
+        int64_t items = 0, work = 0, longest = 0; const int seg = p.kinds == SYMS ? 2 : 1;
+        for (const Desc& d : p.d) { const int64_t t = (int64_t)d.batch * cdiv(d.m, T) * cdiv(d.n, T), kb = seg * cdiv(d.m, 16); items += t; work += t * kb; longest = std::max(longest, kb); }
+        nn[T == 64] = launch_us(T, items, work, longest, p.d.size() == 1);
+    }
+    p.cuts.nn_tile = !p.cuts.fuse && nn[0] <= nn[1] ? 128 : 64;
     for (Desc& d : p.d) {
         const int64_t mt = cdiv(d.m, PAD), nt = cdiv(d.n, PAD);
         d.first = (int)L.n_mats; d.nn0 = (int)L.n_nn; d.pk0 = (int)L.n_pk;
@@ -987,7 +1059,8 @@ template <int DT> static void ns_launch(int kind, NsProblem& p, const Layout& L,
         if (p.cuts.sym[a.kind].tile == 128) hipLaunchKernelGGL((ns_sym_kernel<128>), dim3((unsigned)L.n_sym[a.kind]), blk, 0, s, ws, a);
         else hipLaunchKernelGGL((ns_sym_kernel<64>), dim3((unsigned)L.n_sym[a.kind]), blk, 0, s, ws, a);
         if (!L.n_red[a.kind]) return;
-        if (p.cuts.sym[a.kind].tile == 128) hipLaunchKernelGGL((ns_reduce_kernel<128>), dim3((unsigned)L.n_red[a.kind] * 4), blk, 0, s, ws, a);
+        if (a.fuse) { hipLaunchKernelGGL(ns_reduce_whole_kernel, dim3((unsigned)L.n_red[a.kind]), blk, 0, s, ws, a); return; }
+        if (p.cuts.sym[a.kind].tile == 128) hipLaunchKernelGGL((ns_reduce_kernel<128>), dim3((unsigned)L.n_red[a.kind] * 8), blk, 0, s, ws, a);
         else hipLaunchKernelGGL((ns_reduce_kernel<64>), dim3((unsigned)L.n_red[a.kind] * 2), blk, 0, s, ws, a);
     };
     const MuonArgs mu{(float)o.momentum, o.grad_scale, o.nesterov};
@@ -1007,9 +1080,10 @@ template <int DT> static void ns_launch(int kind, NsProblem& p, const Layout& L,
     auto B = [&](int k) { return Slot{nX, back ? 2 * k + 1 : 1}; };
     for (int k = 0; k < steps; ++k) {
         SymArgs g{}; g.l[0] = g.r[0] = X(k); g.e = g.out = A(k); g.nseg = 1; g.kind = GRAM; g.acc = (float)(SA / (SX * SX));
+        g.fuse = p.cuts.fuse; g.then = B(k); g.acc2 = (float)(c * SB / (SA * SA)); g.ecoef2 = (float)(b * SB / SA);
         sym(g);
         SymArgs q{}; q.l[0] = q.r[0] = q.e = A(k); q.out = B(k); q.nseg = 1; q.kind = POLY; q.have_e = 1; q.acc = (float)(c * SB / (SA * SA)); q.ecoef = (float)(b * SB / SA);
-        sym(q);
+        if (!p.cuts.fuse) sym(q);
         if (back && k == steps - 1) break;
         NnArgs f{}; f.l[0] = B(k); f.r[0] = f.e = X(k); f.out = X(k + 1); f.nseg = 1;
         if (k < steps - 1) { f.acc = (float)(1.0 / SB); f.ecoef = (float)a; NN(NS_F32, OUT_PAIR); }
@@ -1029,9 +1103,10 @@ template <int DT> static void ns_launch(int kind, NsProblem& p, const Layout& L,
         const double gin = sg(k + 1), gout = sg(k), sbound = 2 * P.growth[k + 1] * P.s[k];
         const double ss = pow2_below(16384.0 / sbound), sv = pow2_below(16384.0 / (sbound * P.vgain[k]));
         SymArgs q{}; q.l[0] = G[cur]; q.r[0] = X(k); q.l[1] = X(k); q.r[1] = G[cur]; q.e = q.out = S; q.nseg = 2; q.kind = SYM_S; q.acc = (float)(ss / (gin * SX));
+        q.fuse = p.cuts.fuse; q.with = A(k); q.then = V; q.acc2 = (float)(c * sv / (ss * SA)); q.ecoef2 = (float)(b * sv / ss);
         sym(q);
         SymArgs v{}; v.l[0] = S; v.r[0] = A(k); v.l[1] = A(k); v.r[1] = S; v.e = S; v.out = V; v.nseg = 2; v.kind = SYM_V; v.have_e = 1; v.acc = (float)(c * sv / (ss * SA)); v.ecoef = (float)(b * sv / ss);
-        sym(v);
+        if (!p.cuts.fuse) sym(v);
         NnArgs f{}; f.l[0] = B(k); f.r[0] = f.e = G[cur]; f.l[1] = V; f.r[1] = X(k); f.out = G[cur ^ 1]; f.x0 = X(0); f.nseg = 2;
         f.mid = (float)(sv * SX / (SB * gin)); f.acc = (float)(gout / (sv * SX)); f.ecoef = (float)(a * gout / gin);
         if (k > 0) NN(NS_F32, OUT_PAIR);

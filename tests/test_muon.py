@@ -127,7 +127,7 @@ def test_two_weights_may_share_a_gradient():
 
 # ---- newton_schulz ------------------------------------------------------------------------------------------------------------
 SHAPES = [(1, 1), (1, 7), (9, 1), (2, 2), (16, 16), (31, 33), (64, 64), (65, 64), (64, 576), (127, 130), (128, 128), (129, 129), (200, 77), (33, 1000), (130, 300), (257, 96), (256, 640), (385, 514),
-          (32, 1152), (32, 1153), (1153, 20), (64, 512), (513, 64), (61, 511), (5, 1000), (700, 130), (1000, 1100)]      # (the first six: both sides of what a workgroup keeps in LDS)
+          (32, 1152), (32, 1153), (1153, 20), (64, 512), (513, 64), (61, 575), (577, 64), (32, 1185), (5, 1000), (700, 130), (1000, 1100), (64, 3000), (4000, 50)]      # (the first eight: both sides of what a workgroup keeps in LDS)
 
 
 def check(y, x, steps=5, coef=COEF, eps=1e-7, name=""):
@@ -219,7 +219,7 @@ def check_back(dx, x, dout, steps=5, coef=COEF, eps=1e-7):
 
 @gpu
 @pytest.mark.parametrize("dtype", list(HALF))
-@pytest.mark.parametrize("shape", [(1, 7), (9, 1), (2, 3), (31, 33), (64, 64), (65, 64), (64, 576), (129, 131), (200, 77), (130, 300), (3, 40, 60), (2, 150, 37)])
+@pytest.mark.parametrize("shape", [(1, 7), (9, 1), (2, 3), (31, 33), (64, 64), (65, 64), (64, 576), (129, 131), (200, 77), (130, 300), (3, 40, 60), (2, 150, 37), (64, 2000), (20, 3000), (5, 33, 500)])
 def test_newton_schulz_pullback(shape, dtype):
     x = gradient_like(shape, sum(shape)).to(dtype).cuda(); d = torch.randn(shape, generator=torch.Generator().manual_seed(2), dtype=torch.float64).to(dtype).cuda()
     keep = x.clone(), d.clone(); dx = md().newton_schulz_pullback(x, d)
@@ -336,6 +336,21 @@ def test_muon_raw_list_order_and_company():
         m.muon_raw([a[0][0]], [a[1][1]], [a[2][0]])
     with pytest.raises(RuntimeError, match="overlaps"):
         m.muon_raw([a[0][0], a[0][0]], [a[1][0], a[1][0]], [a[2][0], a[2][4]])
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(64, 64), (40, 1500), (130, 200), (3, 70, 90), (300, 600), (17, 60, 700), (150, 1000)])
+def test_nothing_depends_on_what_the_workspace_held(shape):
+    """Rows and columns behind a matrix's last in the workspace may hold anything, NaN too: the same bits after the allocator's memory was filled with NaN and with zeros."""
+    m = md(); x = gradient_like(shape, 3).float().cuda(); d = torch.randn(shape, generator=torch.Generator().manual_seed(4)).cuda(); got = []
+    for fill in (math.nan, 0.0):
+        out = []
+        for f in (lambda: m.newton_schulz(x), lambda: m.newton_schulz_pullback(x, d)):
+            torch.cuda.empty_cache(); junk = torch.full((1 << 27,), fill, device="cuda"); torch.cuda.synchronize(); del junk      # 512 MB: the next workspace is cut from it
+            out.append(f())
+        p, mo = x.reshape(-1, shape[-1]).clone(), torch.zeros(x.numel() // shape[-1], shape[-1], device="cuda"); junk = torch.full((1 << 27,), fill, device="cuda"); del junk
+        m.muon_raw([p], [x.reshape(-1, shape[-1])], [mo]); got.append(out + [p, mo])
+    assert all(torch.equal(a, b) and torch.isfinite(a).all() for a, b in zip(*got))
 
 
 # ---- streams, graphs, repeatability ---------------------------------------------------------------------------------------------------
