@@ -851,12 +851,10 @@ _NS_DEFAULT = _F64x3(*NS_COEFFICIENTS)
 
 
 def _ns_args(steps, coefficients, eps):
-    if coefficients == NS_COEFFICIENTS:
-        return int(steps), _NS_DEFAULT, float(eps)
-    co = tuple(float(c) for c in coefficients)
+    co = tuple(coefficients)
     if len(co) != 3:
         raise ValueError("coefficients: expected (a, b, c)")
-    return int(steps), _F64x3(*co), float(eps)
+    return int(steps), _NS_DEFAULT if co == NS_COEFFICIENTS else _F64x3(*(float(c) for c in co)), float(eps)
 
 
 def _on(device):
