@@ -765,13 +765,14 @@ template <int MT, int DT, int MUON, int N> __global__ __launch_bounds__(512) voi
         }
     }
     __syncthreads();
+    const int shares = nb >= 8 ? C::KS : 1;                      // (fewer blocks: joining shares costs more than it saves)
     const int tile = wv % C::TILES, ks = wv / C::TILES, i0 = tile / MT * 32, j0 = tile % MT * 32;
     for (int step = 0; step < a.steps; ++step) {
         const bool last = step == a.steps - 1;
         // A = X X^T: a 32 x 32 tile and a share of K a wave, three sums that do not wait for each other
         f32x16 c[3] = {};
-        if (ks < C::KS) {
-            for (int k = ks; k < nb; k += C::KS) {
+        if (ks < shares) {
+            for (int k = ks; k < nb; k += shares) {
                 const f16x8 ah = small_row(X, S, i0 + lr, k, lk), al = small_row(X, S, i0 + lr, k, lk + 2), bh = small_row(X, S, j0 + lr, k, lk), bl = small_row(X, S, j0 + lr, k, lk + 2);
                 c[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, c[0], 0, 0, 0); c[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh, c[1], 0, 0, 0); c[2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl, c[2], 0, 0, 0);
             }
@@ -785,17 +786,19 @@ template <int MT, int DT, int MUON, int N> __global__ __launch_bounds__(512) voi
                     *reinterpret_cast<f32x4*>(A + (((ks - 1) * C::TILES + tile) * 256 + g * 64 + lane) * 16) = w;
                 }
         }
-        __syncthreads();
-        if (ks == 0)
+        if (shares > 1) {
+            __syncthreads();
+            if (ks == 0)
 #pragma unroll
-            for (int r = 1; r < C::KS; ++r)
+                for (int r = 1; r < C::KS; ++r)
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const f32x4 w = *reinterpret_cast<const f32x4*>(A + (((r - 1) * C::TILES + tile) * 256 + g * 64 + lane) * 16);
+                    for (int g = 0; g < 4; ++g) {
+                        const f32x4 w = *reinterpret_cast<const f32x4*>(A + (((r - 1) * C::TILES + tile) * 256 + g * 64 + lane) * 16);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) c[0][g * 4 + e] += w[e];
-                }
-        __syncthreads();
+                        for (int e = 0; e < 4; ++e) c[0][g * 4 + e] += w[e];
+                    }
+            __syncthreads();
+        }
         auto write = [&](const f32x16& v) {                      // lane: row j0 + lr, registers: four neighbouring columns from i0 (A and B are symmetric)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
@@ -825,37 +828,39 @@ template <int MT, int DT, int MUON, int N> __global__ __launch_bounds__(512) voi
         __syncthreads();
         if (ks == 0) write(p[0]);
         __syncthreads();
-        // X <- a X + B X, 32 columns a wave at a time, in place; the last step leaves fp32
+        // X <- a X + B X, a 32 x 32 tile a wave at a time, in place: a round's eight waves have read their columns before any of them writes; the last step leaves fp32
         const float facc = (last ? a.last : a.apply) * inv2, fe_ = last ? a.last_e : a.apply_e;
-        for (int cg = wv; cg < nb / 2; cg += 8) {
-            f16x8 xh[C::MP / 16], xl[C::MP / 16];
-            const int s = lane & 15, g4 = lane >> 4, blk = cg * 2 + (g4 & 1), chunk = (s & 3) >> 1;
+        for (int at = wv; at - wv < nb / 2 * MT; at += 8) {
+            const bool mine = at < nb / 2 * MT; const int cg = at / MT, i = at % MT * 32 + lr;
+            f16x8 xh[C::MP / 16], xl[C::MP / 16]; float e4[16];
+            if (mine) {
+                const int s = lane & 15, g4 = lane >> 4, blk = cg * 2 + (g4 & 1), chunk = (s & 3) >> 1;
 #pragma unroll
-            for (int k = 0; k < C::MP / 16; ++k) {
-                typedef __attribute__((address_space(3))) s16x4* p4; typedef short s16x8 __attribute__((ext_vector_type(8)));
-                s16x4 v[4];
+                for (int k = 0; k < C::MP / 16; ++k) {
+                    typedef __attribute__((address_space(3))) s16x4* p4; typedef short s16x8 __attribute__((ext_vector_type(8)));
+                    s16x4 v[4];
 #pragma unroll
-                for (int h = 0; h < 4; ++h) {                    // rows 0..3 and 4..7 of the lane's eight; hi, lo
-                    const int row = k * 16 + (g4 >> 1) * 8 + (h & 1) * 4 + (s >> 2);
-                    v[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p4)(X + row * S + ((blk ^ (row & 3)) << 6) + (((chunk + (h >> 1) * 2) ^ row_swizzle(row)) << 4) + (s & 1) * 8));
+                    for (int h = 0; h < 4; ++h) {                // rows 0..3 and 4..7 of the lane's eight; hi, lo
+                        const int row = k * 16 + (g4 >> 1) * 8 + (h & 1) * 4 + (s >> 2);
+                        v[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p4)(X + row * S + ((blk ^ (row & 3)) << 6) + (((chunk + (h >> 1) * 2) ^ row_swizzle(row)) << 4) + (s & 1) * 8));
+                    }
+                    xh[k] = __builtin_bit_cast(f16x8, (s16x8)__builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7)); xl[k] = __builtin_bit_cast(f16x8, (s16x8)__builtin_shufflevector(v[2], v[3], 0, 1, 2, 3, 4, 5, 6, 7));
                 }
-                xh[k] = __builtin_bit_cast(f16x8, (s16x8)__builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7)); xl[k] = __builtin_bit_cast(f16x8, (s16x8)__builtin_shufflevector(v[2], v[3], 0, 1, 2, 3, 4, 5, 6, 7));
-            }
 #pragma unroll
-            for (int r = 0; r < MT; ++r) {
-                const int i = r * 32 + lr; f32x16 d[3] = {};
+                for (int g = 0; g < 4; ++g) {
+                    const int j = cg * 32 + g * 8 + lk * 4;
+                    unpack4(*reinterpret_cast<const f16x4*>(small_at(X, S, i, j, 0)), *reinterpret_cast<const f16x4*>(small_at(X, S, i, j, 1)), e4 + g * 4);
+                }
+            }
+            __syncthreads();
+            if (mine) {
+                f32x16 d[3] = {};
 #pragma unroll
                 for (int k = 0; k < C::MP / 16; ++k) {
                     const f16x8 bh = small_row(A, C::AROW, i, k, lk), bl = small_row(A, C::AROW, i, k, lk + 2);
                     d[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xh[k], bh, d[0], 0, 0, 0); d[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xl[k], bh, d[1], 0, 0, 0); d[2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xh[k], bl, d[2], 0, 0, 0);
                 }
                 d[0] += d[1] + d[2];
-                float e4[16];
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const int j = cg * 32 + g * 8 + lk * 4;
-                    unpack4(*reinterpret_cast<const f16x4*>(small_at(X, S, i, j, 0)), *reinterpret_cast<const f16x4*>(small_at(X, S, i, j, 1)), e4 + g * 4);
-                }
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
                     const int j = cg * 32 + g * 8 + lk * 4; float w[4];
