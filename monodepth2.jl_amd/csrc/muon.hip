@@ -242,7 +242,7 @@ template <int DT, int SRC> __global__ __launch_bounds__(256) void ns_pack_kernel
         if (it.ti == 0 && it.tj == 0 && threadIdx.x == 0) ws.fac[it.mat] = Fac{(float)ldexp(1.0, -2 * q), q};
         scale = ldexp(scale, q);
     }
-    const double fd = norm <= eps ? (eps > 0 ? scale / eps : 0.0) : scale / norm;      // (a NaN norm stays one; eps = 0, dout: 0 for a zero dout)
+    const double fd = norm <= eps ? (norm > 0 ? scale / eps : 0.0) : scale / norm;     // (a NaN norm stays one; zeros stay zeros, however small eps is)
     int fe; const float f = (float)frexp(fd, &fe);               // mantissa and exponent apart: 1 / norm may lie outside fp32's range where the product does not
     float v[8][4]; load_tile<DT, SRC, false>(M, it, mu, v, lds);
     char* out = M.buf + x_slot * M.xbytes; const int64_t rb = (int64_t)M.np * 4;
@@ -750,7 +750,7 @@ template <int MT, int DT, int MUON, int N> __global__ __launch_bounds__(512) voi
     const double norm = sqrt(((red[0] + red[1]) + (red[2] + red[3])) + ((red[4] + red[5]) + (red[6] + red[7])));
     int fq = 0;
     if (norm <= a.eps && norm > 0) { const double room = 4.0 * a.eps / (norm * a.grow); if (room >= 2.0) fq = ilogb(room); }      // (as in ns_pack_kernel)
-    const float inv2 = (float)ldexp(1.0, -2 * fq); int fe; const float f = (float)frexp(ldexp(SX, fq) / (norm <= a.eps ? a.eps : norm), &fe);
+    const float inv2 = (float)ldexp(1.0, -2 * fq); int fe; const float f = (float)frexp(norm > 0 || norm != norm ? ldexp(SX, fq) / (norm <= a.eps ? a.eps : norm) : 0.0, &fe);
     for (int q = t; q < C::MP * nb; q += 512) {                  // a block of 16 columns a thread
         const int i = q / nb, blk = q % nb; char* p = X + i * S + ((blk ^ (i & 3)) << 6); f32x4 r[4];
 #pragma unroll
@@ -1121,13 +1121,16 @@ template <int DT> static void ns_launch(int kind, NsProblem& p, const Layout& L,
 #undef NN
 }
 
+// (any fp32 norm over any fp32 eps, and the carry of a clamped matrix, stay far inside the range of doubles)
+static const char* const kEps = "eps must be positive and at most 3.4e38";
+static bool eps_ok(double eps) { return eps > 0 && eps <= 3.4e38; }
 const char* ns_check(int steps, const double* co, double eps) {
-    if (!(eps > 0) || !std::isfinite(eps)) return "eps must be positive";
+    if (!eps_ok(eps)) return kEps;
     const Plan P = ns_bounds(steps, co, false);
     return P.ok ? nullptr : P.why;
 }
 int ns_run(int kind, int dtype, const NsMatrices* q, int count, const NsOptions& o, void* wsp, int64_t ws_bytes, hipStream_t s, const char** why) {
-    if (!(o.eps > 0) || !std::isfinite(o.eps)) { *why = "eps must be positive"; return 2; }
+    if (!eps_ok(o.eps)) { *why = kEps; return 2; }
     const Plan P = ns_bounds(o.steps, o.coef, kind == NS_BACKWARD);
     if (!P.ok) { *why = P.why; return 2; }
     const int el = dtype == NS_F32 ? 4 : 2;

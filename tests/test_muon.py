@@ -514,3 +514,23 @@ def test_train_takes_the_optimizer(tmp_path):
     model, losses = md2amd.train.train([Frames()], str(tmp_path / "l"), str(tmp_path / "s"), batch_size=2, n_epochs=2, log_iter=100, save_iter=2, quiet=True, optimizer=md().Muon(eta=1e-3, adam_eta=5e-5))
     assert len(losses) == 4 and np.isfinite(losses).all() and model.lr == 5e-5 and np.abs(model.muon_state()).max() > 0
     assert any("muon_m" in np.load(f) for f in (tmp_path / "s").glob("*.npz"))
+
+
+# ---- arguments at the ends of their ranges ----------------------------------------------------------------------------------------------
+def test_an_eps_past_the_largest_float_is_refused():
+    for eps in (3.5e38, 1e308):
+        assert ns_c(eps=eps) == 2 and "eps" in last_error()
+        assert muon_c(eps=eps) == 2 and "eps" in last_error()
+    assert ns_c(eps=3.4e38) == 2 and "workspace" in last_error()
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(48, 80), (90, 150)])
+def test_the_smallest_and_largest_eps(shape):
+    """Zeros over an eps whose reciprocal no double holds are zeros; a matrix far below a huge eps is only scaled and grown."""
+    m = md()
+    assert torch.equal(m.newton_schulz(torch.zeros(shape, device="cuda"), eps=1e-320), torch.zeros(shape, device="cuda"))
+    x = gradient_like(shape, 8, scale=1.0)
+    check(m.newton_schulz(x.float().cuda(), eps=1e-320), x.float())
+    check(m.newton_schulz(x.float().cuda(), eps=1e30), x.float(), eps=1e30)
+    check(m.newton_schulz((x * 1e30).float().cuda(), eps=1e38), (x * 1e30).float(), eps=1e38)
