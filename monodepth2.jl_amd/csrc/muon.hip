@@ -920,7 +920,7 @@ Plan ns_bounds(int steps, const double* co, bool back) {
     if (back && !(P.growth[0] <= 8192.0)) { P.why = "the pullback of this many steps can grow a gradient past 8192 times its norm"; return P; }
     P.ok = true; return P;
 }
-double pow2_below(double v) { return std::exp2(std::floor(std::log2(v))); }
+double pow2_below(double v) { return std::exp2(std::min(std::floor(std::log2(v)), 40.0)); }      // (a scale; its bound is 0 where coefficients are)
 
 int64_t up(int64_t v, int64_t q) { return (v + q - 1) / q * q; }
 struct Layout { int64_t mats, sym[SYMS], red[SYMS], nn, pk, fac, part, split, buf, total; int64_t n_mats, n_sym[SYMS], n_red[SYMS], n_nn, n_pk; };

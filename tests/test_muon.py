@@ -534,3 +534,17 @@ def test_the_smallest_and_largest_eps(shape):
     check(m.newton_schulz(x.float().cuda(), eps=1e-320), x.float())
     check(m.newton_schulz(x.float().cuda(), eps=1e30), x.float(), eps=1e30)
     check(m.newton_schulz((x * 1e30).float().cuda(), eps=1e38), (x * 1e30).float(), eps=1e38)
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(24, 40), (70, 90), (130, 200)])
+@pytest.mark.parametrize("coef", [(1.0, 0.0, 0.0), (1.5, -0.5, 0.0), (0.75, 0.0, -0.25), (0.0, 1.0, 0.0), (0.0, 0.0, 0.0)])
+def test_coefficients_that_are_zero(shape, coef):
+    m = md(); x = gradient_like(shape, 14, noise=1.0).float().cuda(); d = torch.randn(shape, generator=torch.Generator().manual_seed(9)).cuda()
+    y, dx = m.newton_schulz(x, steps=1, coefficients=coef), m.newton_schulz_pullback(x, d, steps=1, coefficients=coef)
+    if not any(coef):
+        assert not y.any() and not dx.any()
+        return
+    check(y, x, 1, coef); check_back(dx, x, d, 1, coef)
+    if coef[0]:
+        check(m.newton_schulz(x, steps=3, coefficients=coef), x, 3, coef); check_back(m.newton_schulz_pullback(x, d, steps=3, coefficients=coef), x, d, 3, coef)
