@@ -1129,6 +1129,12 @@ const char* ns_check(int steps, const double* co, double eps) {
     const Plan P = ns_bounds(steps, co, false);
     return P.ok ? nullptr : P.why;
 }
+// does the contiguous result share memory with what `st` reaches from p?
+static bool overlaps(const NsMatrices& q, const void* p, const int64_t st[3], int el) {
+    const __int128 y0 = (__int128)(uintptr_t)q.y, y1 = y0 + (__int128)q.batch * q.rows * q.cols * el, p0 = (__int128)(uintptr_t)p;
+    const __int128 p1 = p0 + ((__int128)(q.batch - 1) * st[0] + (__int128)(q.rows - 1) * st[1] + (__int128)(q.cols - 1) * st[2] + 1) * el;
+    return y0 < p1 && p0 < y1;
+}
 int ns_run(int kind, int dtype, const NsMatrices* q, int count, const NsOptions& o, void* wsp, int64_t ws_bytes, hipStream_t s, const char** why) {
     if (!eps_ok(o.eps)) { *why = kEps; return 2; }
     const Plan P = ns_bounds(o.steps, o.coef, kind == NS_BACKWARD);
@@ -1141,6 +1147,8 @@ int ns_run(int kind, int dtype, const NsMatrices* q, int count, const NsOptions&
         if (!fits(m.batch, m.rows, m.cols)) { *why = "sizes must be positive, a side at most 2^20, a matrix at most 2^31 elements, a batch at most 2^20"; return 2; }
         if (((uintptr_t)m.x | (uintptr_t)m.d | (uintptr_t)m.y) % el) { *why = "a pointer is not aligned to its elements"; return 2; }
         for (int k = 0; k < 3; ++k) if (m.xs[k] < 0 || m.ds[k] < 0) { *why = "negative stride"; return 2; }
+        // (one matrix may be written before another is read)
+        if (kind != NS_MUON && (overlaps(m, m.x, m.xs, el) || (kind == NS_BACKWARD && overlaps(m, m.d, m.ds, el)))) { *why = "the result overlaps an input"; return 2; }
         p.d.push_back(make_desc(m));
     }
     if (kind != NS_MUON) { const bool tall = p.d[0].tall; const int64_t *x = q[0].xs, *d = q[0].ds; p.st = Strides{x[0], x[tall ? 2 : 1], x[tall ? 1 : 2], d[0], d[tall ? 2 : 1], d[tall ? 1 : 2]}; }

@@ -548,3 +548,13 @@ def test_coefficients_that_are_zero(shape, coef):
     check(y, x, 1, coef); check_back(dx, x, d, 1, coef)
     if coef[0]:
         check(m.newton_schulz(x, steps=3, coefficients=coef), x, 3, coef); check_back(m.newton_schulz_pullback(x, d, steps=3, coefficients=coef), x, d, 3, coef)
+
+
+@pytest.mark.parametrize("kw,refused", [(dict(y=4096), True), (dict(y=4096 + 252), True), (dict(y=4096 - 252), True), (dict(y=4096 + 256), False), (dict(y=4096 - 256), False),
+                                        (dict(batch=2, strides=(1024, 8, 1), y=4096 + 2048), True), (dict(batch=2, strides=(0, 0, 0), y=4096 + 4), False), (dict(strides=(1 << 62, 1 << 62, 1 << 62)), True)])
+def test_a_result_that_overlaps_an_input_is_refused(kw, refused):
+    """8 x 8 fp32 matrices of 256 bytes at 4096 (a call that is not refused for it is for its workspace)."""
+    assert ns_c(**kw) == 2 and ("overlaps" if refused else "workspace") in last_error(), last_error()
+    if set(kw) == {"y"}:
+        L = md2amd._lib.lib(); st = (ctypes.c_int64 * 3)(64, 8, 1); co = (ctypes.c_double * 3)(*COEF)
+        assert L.md2_newton_schulz_bwd(65536, 4096, kw["y"], 1, 8, 8, st, st, 0, 5, co, 1e-7, 4096, 0, None) == 2 and ("overlaps" if refused else "workspace") in last_error()
