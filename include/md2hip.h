@@ -144,7 +144,7 @@ int32_t md2_opt_state_get(md2_handle* h, float* host_m, float* host_v, int64_t n
 int32_t md2_opt_state_set(md2_handle* h, const float* host_m, const float* host_v, int64_t n, double beta1p, double beta2p);
 /* Muon instead of ADAM for the matrices: the hidden convolutions (every one but the stem, the disparity heads and the pose decoder's last) take md2_muon_raw's update, Cout x Cin k k
  * each, all other parameters the ADAM step of md2_adam_step (its eta, its moments).  Arguments as for md2_muon_raw; grads scaled by grad_scale first.  The first call allocates the
- * momentum and a workspace (so it cannot be captured into a graph; later ones can) and makes the handle Muon's: md2_adam_step and md2_train_step's update then return an error, because the
+ * momentum and a workspace (no call can be captured into a graph: ADAM's bias corrections change with every step) and makes the handle Muon's: md2_adam_step and md2_train_step's update then return an error, because the
  * hidden convolutions' ADAM moments are no longer kept, until md2_muon_state_set(h, NULL, 0). */
 int32_t md2_muon_step(md2_handle* h, double lr, double momentum, int32_t nesterov, double weight_decay, int32_t adjust, int32_t steps, const double* host_coefficients, double eps, float grad_scale);
 /* Muon's momentum (Flux parameter layout, host; 0 where ADAM steps): count = md2_params_count(h) once the handle has it, 0 before.  set gives the handle Muon state (a resumed run);

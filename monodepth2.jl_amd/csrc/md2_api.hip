@@ -1601,7 +1601,7 @@ static int muon_alloc(md2_handle* h) {
                     && hipMalloc((void**)&h->mu_ranges, r.size() * sizeof(long)) == hipSuccess && hipMemcpy(h->mu_ranges, r.data(), r.size() * sizeof(long), hipMemcpyHostToDevice) == hipSuccess;
     h->MU = mu;
     if (ok) launch_fill(h->MU, h->n_int, 0.f, h->stream);
-    else { muon_free(h); h->err = "md2_muon_step: no device memory for the momentum and the workspace (the first call cannot be captured into a graph)"; (void)hipGetLastError(); }
+    else { muon_free(h); h->err = "md2_muon_step: no device memory for the momentum and the workspace"; (void)hipGetLastError(); }
     (void)hipSetDevice(dev);
     return ok ? 0 : 3;
 }
@@ -1610,6 +1610,10 @@ int32_t md2_muon_step(md2_handle* h, double lr, double momentum, int32_t nestero
         if (!h->net_ok) { h->err = "this handle is loss-only (height/width below 64 or not multiples of 32): the model entry points are unavailable"; return 2; }
         const MuonHyper y{lr, momentum, nesterov, weight_decay, adjust, grad_scale, steps, co, eps}; const char* why = "";
         if ((why = muon_check(y)) || (why = co ? ns_check(steps, co, eps) : "null coefficients")) { h->err = std::string("md2_muon_step: ") + why; return 2; }
+        // (a replay would repeat the captured step's bias corrections, which are ADAM's arguments)
+        hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
+        if (hipStreamIsCapturing(h->stream, &capturing) != hipSuccess) (void)hipGetLastError();
+        if (capturing != hipStreamCaptureStatusNone) { h->err = "md2_muon_step cannot be captured into a graph: the ADAM part's bias corrections change with every step (md2_muon_raw can)"; return 2; }
         if (!h->MU) if (int r = muon_alloc(h)) return r;
         std::vector<NsMatrices> q;
         for (const ConvL* c : muon_convs(h)) q.push_back(muon_matrix(h->P + c->w, h->G + c->w, h->MU + c->w, c->coutP, (int64_t)c->taps * c->cinP, y));

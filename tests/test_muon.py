@@ -558,3 +558,18 @@ def test_a_result_that_overlaps_an_input_is_refused(kw, refused):
     if set(kw) == {"y"}:
         L = md2amd._lib.lib(); st = (ctypes.c_int64 * 3)(64, 8, 1); co = (ctypes.c_double * 3)(*COEF)
         assert L.md2_newton_schulz_bwd(65536, 4096, kw["y"], 1, 8, 8, st, st, 0, 5, co, 1e-7, 4096, 0, None) == 2 and ("overlaps" if refused else "workspace") in last_error()
+
+
+@gpu
+def test_a_model_step_cannot_be_captured():
+    """The ADAM part's bias corrections are arguments of its launch: a replayed step would repeat them, so the call is refused and nothing is recorded or changed."""
+    m = md(); model, params, cache, x = make_model(); m.train_step(model, x, None, cache, params, do_update=False); p = model.params()
+    for first in (True, False):
+        side = torch.zeros(4, device="cuda"); torch.cuda.synchronize(); graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            side.add_(1)
+            with pytest.raises(RuntimeError, match="captured"):
+                m.update(m.Muon(), model)
+        graph.replay(); torch.cuda.synchronize()
+        assert (side == 1).all() and np.array_equal(model.params(), p) and (model.muon_state() is None) == first
+        m.update(m.Muon(), model); q = model.params(); assert not np.array_equal(p, q); p = q
