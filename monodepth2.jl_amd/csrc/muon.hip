@@ -267,7 +267,6 @@ __device__ inline Dims dims(const Item& it) {
 }
 __device__ inline char* slot(const Item& it, const Dims& d, Slot s) { return it.buf + s.x * d.xbytes + s.a * d.abytes; }
 
-typedef const __attribute__((address_space(1))) void* glb_t;
 typedef __attribute__((address_space(3))) void* lds_t;
 // LDS of a product: RING stages of 16 K of both operands.  128-tiles: shared by the workgroup, 16 KB each, so that two workgroups share a CU; 64-tiles: each wave's own, 8 KB each
 template <int T> struct Ring { static constexpr int N = T == 128 ? 5 : 4, STAGE = T == 128 ? 16384 : 8192, THREADS = T == 128 ? 256 : 64, LOADS = STAGE / THREADS / 32, BYTES = T == 128 ? N * STAGE : 4 * N * STAGE; };      // LOADS: a wave's instructions per stage and operand
@@ -995,9 +994,9 @@ static Layout ns_layout(NsProblem& p) {
 static bool fits(int64_t batch, int64_t rows, int64_t cols) {      // sizes whose work items and element counts stay far inside 31 bits
     return rows > 0 && cols > 0 && batch > 0 && rows <= (1 << 20) && cols <= (1 << 20) && rows * cols <= (1ll << 31) && batch <= (1 << 20);
 }
-static int64_t check_total(const Layout& L) {
-    for (int k = 0; k < SYMS; ++k) if (L.n_sym[k] >= (1ll << 28)) return -1;
-    return (L.n_nn < (1ll << 28) && L.n_pk < (1ll << 28) && L.n_mats < (1ll << 24)) ? L.total : -1;
+static int64_t check_total(const Layout& L) {      // (a launch has fewer than 2^32 threads: 2^24 workgroups of 256)
+    for (int k = 0; k < SYMS; ++k) if (L.n_sym[k] >= (1ll << 24) || L.n_red[k] * 8 >= (1ll << 24)) return -1;
+    return (L.n_nn < (1ll << 24) && L.n_pk < (1ll << 24) && L.n_mats < (1ll << 24)) ? L.total : -1;
 }
 
 static Desc make_desc(const NsMatrices& q) {

@@ -573,3 +573,9 @@ def test_a_model_step_cannot_be_captured():
         graph.replay(); torch.cuda.synchronize()
         assert (side == 1).all() and np.array_equal(model.params(), p) and (model.muon_state() is None) == first
         m.update(m.Muon(), model); q = model.params(); assert not np.array_equal(p, q); p = q
+
+
+def test_more_work_than_a_launch_can_hold_is_refused():
+    """(such a call's workspace would be 16 TB and more)"""
+    L = md2amd._lib.lib()
+    assert L.md2_newton_schulz_workspace(1 << 20, 1000, 2000, 5, 0) == -1 and L.md2_newton_schulz_workspace(1 << 20, 100, 200, 5, 0) > 0
