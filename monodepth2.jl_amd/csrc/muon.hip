@@ -210,18 +210,19 @@ template <int DT, int SRC, bool UPDATE> __device__ inline void load_tile(const M
         for (int e = 0; e < 4; ++e) v[p][e] = lds[(p * 8 + (t >> 5)) * (PK_COLS + 1) + (t & 31) * 4 + e];
 }
 
-// sum of squares of every tile (Muon: after moving the momentum on)
-template <int DT, int SRC> __global__ __launch_bounds__(256) void ns_norm_kernel(Ws ws, double* part, MuonArgs mu) {
+// sum of squares of every tile (Muon: after moving the momentum on); the pullback's second half of the grid: of dout's
+template <int DT, int SRC> __global__ __launch_bounds__(256) void ns_norm_kernel(Ws ws, MuonArgs mu) {
     __shared__ float lds[PK_ROWS * (PK_COLS + 1)]; __shared__ double red[4];
     const Item it = ws.pk[blockIdx.x]; const Mat M = ws.mats[it.mat];
-    float v[8][4]; load_tile<DT, SRC, true>(M, it, mu, v, lds);
+    float v[8][4];
+    if (SRC == SRC_X && blockIdx.y) load_tile<DT, SRC_DOUT, false>(M, it, mu, v, lds); else load_tile<DT, SRC, true>(M, it, mu, v, lds);
     double s = 0;
 #pragma unroll
     for (int p = 0; p < 8; ++p)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s += (double)v[p][e] * (double)v[p][e];
     s = block_sum(s, red);
-    if (threadIdx.x == 0) part[blockIdx.x] = s;
+    if (threadIdx.x == 0) ws.part[blockIdx.y * gridDim.x + blockIdx.x] = s;
 }
 // |.|_F of a matrix from its tiles' sums, in a fixed order
 __device__ inline double norm_of(const Mat& M, const double* part, double* red) {
@@ -229,14 +230,15 @@ __device__ inline double norm_of(const Mat& M, const double* part, double* red) 
     for (int q = threadIdx.x; q < M.pkn; q += 256) s += part[M.pk0 + q];
     return sqrt(block_sum(s, red));
 }
-// scale * source / max(norm, eps) as pairs.
+// scale * source / max(norm, eps) as pairs; the pullback's second half of the grid: d_scale * dout / |dout| into d_slot.
 // Where the norm r = |X| / eps is clamped, X0 may be too small for f16: it is carried 2^q larger, 2^q r grow <= 4 (grow: by how much all steps can grow a singular value), so A, B, S and V
 // are 2^2q, 2^2q, 2^q and 2^q larger, and what has one factor of A too many (A A, S A, B X, V X) is multiplied by 2^-2q.  q = 0 for every other matrix.
-template <int DT, int SRC> __global__ __launch_bounds__(256) void ns_pack_kernel(Ws ws, const double* part, MuonArgs mu, int x_slot, double scale, double eps, double grow) {
+template <int DT, int SRC> __global__ __launch_bounds__(256) void ns_pack_kernel(Ws ws, MuonArgs mu, double scale, double eps, double grow, int d_slot, double d_scale) {
     __shared__ float lds[PK_ROWS * (PK_COLS + 1)]; __shared__ double red[4];
-    const Item it = ws.pk[blockIdx.x]; const Mat M = ws.mats[it.mat];
-    const double norm = norm_of(M, part, red);
-    if constexpr (SRC != SRC_DOUT) {
+    const Item it = ws.pk[blockIdx.x]; const Mat M = ws.mats[it.mat]; const bool dout = SRC == SRC_X && blockIdx.y;
+    const double norm = norm_of(M, ws.part + (dout ? gridDim.x : 0), red);
+    if (dout) { scale = d_scale; eps = 0; }
+    else {
         int q = 0;
         if (norm <= eps && norm > 0) { const double room = 4.0 * eps / (norm * grow); if (room >= 2.0) q = ilogb(room); }
         if (it.ti == 0 && it.tj == 0 && threadIdx.x == 0) ws.fac[it.mat] = Fac{(float)ldexp(1.0, -2 * q), q};
@@ -244,8 +246,9 @@ template <int DT, int SRC> __global__ __launch_bounds__(256) void ns_pack_kernel
     }
     const double fd = norm <= eps ? (norm > 0 ? scale / eps : 0.0) : scale / norm;     // (a NaN norm stays one; zeros stay zeros, however small eps is)
     int fe; const float f = (float)frexp(fd, &fe);               // mantissa and exponent apart: 1 / norm may lie outside fp32's range where the product does not
-    float v[8][4]; load_tile<DT, SRC, false>(M, it, mu, v, lds);
-    char* out = M.buf + x_slot * M.xbytes; const int64_t rb = (int64_t)M.np * 4;
+    float v[8][4];
+    if (dout) load_tile<DT, SRC_DOUT, false>(M, it, mu, v, lds); else load_tile<DT, SRC, false>(M, it, mu, v, lds);
+    char* out = M.buf + (dout ? d_slot : 0) * M.xbytes; const int64_t rb = (int64_t)M.np * 4;
 #pragma unroll
     for (int p = 0; p < 8; ++p) {
         float w[4]; f16x4 hi, lo;
@@ -1068,16 +1071,18 @@ template <int DT> static void ns_launch(int kind, NsProblem& p, const Layout& L,
         else hipLaunchKernelGGL((ns_reduce_kernel<64>), dim3((unsigned)L.n_red[a.kind] * 2), blk, 0, s, ws, a);
     };
     const MuonArgs mu{(float)o.momentum, o.grad_scale, o.nesterov};
-    double *xpart = ws.part, *dpart = ws.part + L.n_pk, *dots = ws.part + 2 * L.n_pk;
-    if (kind == NS_MUON) {
-        hipLaunchKernelGGL((ns_norm_kernel<NS_F32, SRC_MUON>), pk, blk, 0, s, ws, xpart, mu);
-        hipLaunchKernelGGL((ns_pack_kernel<NS_F32, SRC_MUON>), pk, blk, 0, s, ws, xpart, mu, 0, SX, o.eps, P.grow);
-    } else {
-        hipLaunchKernelGGL((ns_norm_kernel<DT, SRC_X>), pk, blk, 0, s, ws, xpart, mu);
-        hipLaunchKernelGGL((ns_pack_kernel<DT, SRC_X>), pk, blk, 0, s, ws, xpart, mu, 0, SX, o.eps, P.grow);
-    }
     const double a = o.coef[0], b = o.coef[1], c = o.coef[2];
     const bool back = kind == NS_BACKWARD;
+    double *xpart = ws.part, *dpart = ws.part + L.n_pk, *dots = ws.part + 2 * L.n_pk;
+    auto sg = [&](int k) { return pow2_below(16384.0 / P.growth[k]); };                 // scale of dL/dX_k (of dout / |dout|: at most growth[k])
+    if (kind == NS_MUON) {
+        hipLaunchKernelGGL((ns_norm_kernel<NS_F32, SRC_MUON>), pk, blk, 0, s, ws, mu);
+        hipLaunchKernelGGL((ns_pack_kernel<NS_F32, SRC_MUON>), pk, blk, 0, s, ws, mu, SX, o.eps, P.grow, 0, 0.0);
+    } else {
+        const dim3 both(pk.x, back ? 2 : 1);
+        hipLaunchKernelGGL((ns_norm_kernel<DT, SRC_X>), both, blk, 0, s, ws, mu);
+        hipLaunchKernelGGL((ns_pack_kernel<DT, SRC_X>), both, blk, 0, s, ws, mu, SX, o.eps, P.grow, steps, back ? sg(steps) : 0.0);
+    }
     const int nX = p.nX;
     auto X = [&](int k) { return Slot{back ? k : (k & 1), 0}; };
     auto A = [&](int k) { return Slot{nX, back ? 2 * k : 0}; };
@@ -1098,11 +1103,8 @@ template <int DT> static void ns_launch(int kind, NsProblem& p, const Layout& L,
         }
     }
     if (!back) return;
-    hipLaunchKernelGGL((ns_norm_kernel<DT, SRC_DOUT>), pk, blk, 0, s, ws, dpart, mu);
-    auto sg = [&](int k) { return pow2_below(16384.0 / P.growth[k]); };                 // scale of dL/dX_k (of dout / |dout|: at most growth[k])
     const Slot G[2] = {Slot{steps, 0}, Slot{steps + 1, 0}}; const Slot S{nX, 2 * steps}, V{nX, 2 * steps + 1};
     int cur = 0;
-    hipLaunchKernelGGL((ns_pack_kernel<DT, SRC_DOUT>), pk, blk, 0, s, ws, dpart, mu, G[cur].x, sg(steps), 0.0, 1.0);
     for (int k = steps - 1; k >= 0; --k, cur ^= 1) {
         const double gin = sg(k + 1), gout = sg(k), sbound = 2 * P.growth[k + 1] * P.s[k];
         const double ss = pow2_below(16384.0 / sbound), sv = pow2_below(16384.0 / (sbound * P.vgain[k]));
