@@ -49,7 +49,7 @@ struct Desc {
 };
 struct Strides { int64_t xb, xs, xl, db, ds, dl; };              // in elements: batch, along the short side, along the long side
 template <int N, int KINDS> struct DescPack { Desc d[N]; Use u[N][KINDS]; };
-constexpr int MUON_DESCS = 38;            // 38 * (72 + 2 * 12) bytes: a set-up launch's arguments stay below 4 KB
+constexpr int MUON_DESCS = 38;            // 38 * (72 + 2 * 12) bytes: a first launch's arguments stay below 4 KB
 
 // the same per matrix, on the device
 struct Mat {
@@ -75,24 +75,27 @@ __device__ inline int dealt(int g, int i, int groups, int size) {
     const int full = groups / 8 * 8, r = groups - full;
     return g < full ? g / 8 * 8 * size + i * 8 + g % 8 : full * size + i * r + (g - full);
 }
-// the tables and work lists of a call, from its weights' descriptions.  N = 1: a batch with strides of its own (and the pullback's products); else contiguous weights
-template <int N, int KINDS> __global__ __launch_bounds__(256) void ns_setup_kernel(DescPack<N, KINDS> dp, Strides st, Cuts cuts, int dt_bytes, Ws ws) {
-    const Desc& D = dp.d[N == 1 ? 0 : blockIdx.y];
+// matrix b of a weight (or of a batch with strides of its own, N = 1)
+template <int N> __device__ inline Mat make_mat(const Desc& D, const Strides& st, const Cuts& cuts, int dt_bytes, char* base, int b) {
+    const int mp = cdiv(D.m, PAD) * PAD, np = cdiv(D.n, PAD) * PAD, npk = mp / PK_ROWS * (np / PK_COLS), nnn = cdiv(D.m, cuts.nn_tile) * cdiv(D.n, cuts.nn_tile);
+    const int64_t ss = D.tall ? 1 : D.n, sl = D.tall ? D.m : 1;      // a contiguous matrix's strides
+    Mat M;
+    M.x = (const char*)D.x + (N == 1 ? st.xb * b * dt_bytes : 0); M.d = (const char*)D.d + (N == 1 ? st.db * b * dt_bytes : 0); M.y = (char*)D.y + (int64_t)D.m * D.n * b * dt_bytes;
+    M.xs = N == 1 ? st.xs : ss; M.xl = N == 1 ? st.xl : sl; M.ds = N == 1 ? st.ds : ss; M.dl = N == 1 ? st.dl : sl; M.ys = ss; M.yl = sl;
+    M.buf = base + D.ws0 + D.ws1 * b; M.m = D.m; M.n = D.n; M.mp = mp; M.np = np;
+    M.xbytes = (int64_t)mp * np * 4; M.abytes = (int64_t)mp * mp * 4;
+    M.pk0 = D.pk0 + npk * b; M.pkn = npk; M.nn0 = D.nn0 + nnn * b; M.nnn = nnn; M.alpha = D.alpha;
+    return M;
+}
+// the tables and work lists of a weight's matrices first, first + by, ...
+template <int N, int KINDS> __device__ inline void set_up(const Desc& D, const Use* use, const Strides& st, const Cuts& cuts, int dt_bytes, const Ws& ws, int first, int by) {
     const int mp = cdiv(D.m, PAD) * PAD, np = cdiv(D.n, PAD) * PAD, npk = mp / PK_ROWS * (np / PK_COLS), pr = mp / PK_ROWS, nr = cdiv(D.m, cuts.nn_tile), nnn = nr * cdiv(D.n, cuts.nn_tile);
-    for (int b = blockIdx.x; b < D.batch; b += gridDim.x) {
-        const int id = D.first + b; char* buf = ws.buf + D.ws0 + D.ws1 * b; const int64_t ss = D.tall ? 1 : D.n, sl = D.tall ? D.m : 1;      // a contiguous matrix's strides
-        if (threadIdx.x == 0) {
-            Mat M;
-            M.x = (const char*)D.x + (N == 1 ? st.xb * b * dt_bytes : 0); M.d = (const char*)D.d + (N == 1 ? st.db * b * dt_bytes : 0); M.y = (char*)D.y + (int64_t)D.m * D.n * b * dt_bytes;
-            M.xs = N == 1 ? st.xs : ss; M.xl = N == 1 ? st.xl : sl; M.ds = N == 1 ? st.ds : ss; M.dl = N == 1 ? st.dl : sl; M.ys = ss; M.yl = sl;
-            M.buf = buf; M.m = D.m; M.n = D.n; M.mp = mp; M.np = np;
-            M.xbytes = (int64_t)mp * np * 4; M.abytes = (int64_t)mp * mp * 4;
-            M.pk0 = D.pk0 + npk * b; M.pkn = npk; M.nn0 = D.nn0 + nnn * b; M.nnn = nnn; M.alpha = D.alpha;
-            ws.mats[id] = M;
-        }
+    for (int b = first; b < D.batch; b += by) {
+        const int id = D.first + b; char* buf = ws.buf + D.ws0 + D.ws1 * b;
+        if (threadIdx.x == 0) ws.mats[id] = make_mat<N>(D, st, cuts, dt_bytes, ws.buf, b);
 #pragma unroll
         for (int kind = 0; kind < KINDS; ++kind) {
-            const Use& u = dp.u[N == 1 ? 0 : blockIdx.y][kind]; const Cut cut = cuts.sym[kind];
+            const Use& u = use[kind]; const Cut cut = cuts.sym[kind];
             const int mt = cdiv(D.m, cut.tile), tri = mt * (mt + 1) / 2, kb = kblocks(kind, D.m, D.n), per = cut.tile * cut.tile * 4 / PART, chunk = cdiv(kb, cdiv(kb, cut.chunk)), split = cdiv(kb, chunk);
             for (int q = threadIdx.x; q < mt * mt; q += 256) {
                 const int i = q / mt, j = q % mt;
@@ -210,10 +213,19 @@ template <int DT, int SRC, bool UPDATE> __device__ inline void load_tile(const M
         for (int e = 0; e < 4; ++e) v[p][e] = lds[(p * 8 + (t >> 5)) * (PK_COLS + 1) + (t & 31) * 4 + e];
 }
 
-// sum of squares of every tile (Muon: after moving the momentum on); the pullback's second half of the grid: of dout's
-template <int DT, int SRC> __global__ __launch_bounds__(256) void ns_norm_kernel(Ws ws, MuonArgs mu) {
-    __shared__ float lds[PK_ROWS * (PK_COLS + 1)]; __shared__ double red[4];
-    const Item it = ws.pk[blockIdx.x]; const Mat M = ws.mats[it.mat];
+// A call's first launch: the tables and work lists of the later ones (the first `tables` workgroups), and the sum of squares of every tile (Muon: after moving the momentum on; the
+// pullback's second half of the grid: of dout's), which work their tiles out themselves.  As launches of their own the tables cost 5 - 13 us, which now pass beside the sums.
+template <int DT, int SRC, int N, int KINDS> __global__ __launch_bounds__(256) void ns_start_kernel(DescPack<N, KINDS> dp, int weights, int tables, int tiles, Strides st, Cuts cuts, Ws ws, MuonArgs mu) {
+    __shared__ float lds[PK_ROWS * (PK_COLS + 1)]; __shared__ double red[4]; constexpr int BYTES = DT == NS_F32 ? 4 : 2;
+    if (blockIdx.x < tables) {
+        const int w = N == 1 ? 0 : blockIdx.x;
+        if (blockIdx.y == 0) set_up<N, KINDS>(dp.d[w], dp.u[w], st, cuts, BYTES, ws, N == 1 ? blockIdx.x : 0, N == 1 ? tables : 1);
+        return;
+    }
+    const int id = dp.d[0].pk0 + blockIdx.x - tables; int w = 0;
+    if constexpr (N > 1) for (int hi = weights - 1; w < hi;) { const int q = (w + hi + 1) / 2; if (dp.d[q].pk0 <= id) w = q; else hi = q - 1; }
+    const Desc& D = dp.d[w]; const int pr = cdiv(D.m, PAD) * PAD / PK_ROWS, npk = pr * cdiv(D.n, PAD) * (PAD / PK_COLS), b = (id - D.pk0) / npk, q = (id - D.pk0) % npk;
+    const Mat M = make_mat<N>(D, st, cuts, BYTES, ws.buf, b); Item it{}; it.ti = q % pr; it.tj = q / pr;
     float v[8][4];
     if (SRC == SRC_X && blockIdx.y) load_tile<DT, SRC_DOUT, false>(M, it, mu, v, lds); else load_tile<DT, SRC, true>(M, it, mu, v, lds);
     double s = 0;
@@ -222,7 +234,7 @@ template <int DT, int SRC> __global__ __launch_bounds__(256) void ns_norm_kernel
 #pragma unroll
         for (int e = 0; e < 4; ++e) s += (double)v[p][e] * (double)v[p][e];
     s = block_sum(s, red);
-    if (threadIdx.x == 0) ws.part[blockIdx.y * gridDim.x + blockIdx.x] = s;
+    if (threadIdx.x == 0) ws.part[blockIdx.y * tiles + id] = s;
 }
 // |.|_F of a matrix from its tiles' sums, in a fixed order
 __device__ inline double norm_of(const Mat& M, const double* part, double* red) {
@@ -999,7 +1011,7 @@ static bool fits(int64_t batch, int64_t rows, int64_t cols) {      // sizes whos
 }
 static int64_t check_total(const Layout& L) {      // (a launch has fewer than 2^32 threads: 2^24 workgroups of 256)
     for (int k = 0; k < SYMS; ++k) if (L.n_sym[k] >= (1ll << 24) || L.n_red[k] * 8 >= (1ll << 24)) return -1;
-    return (L.n_nn < (1ll << 24) && L.n_pk < (1ll << 24) && L.n_mats < (1ll << 24)) ? L.total : -1;
+    return (L.n_nn < (1ll << 24) && L.n_pk < (1ll << 24) - 1024 && L.n_mats < (1ll << 24)) ? L.total : -1;
 }
 
 static Desc make_desc(const NsMatrices& q) {
@@ -1040,24 +1052,13 @@ int64_t ns_workspace(int kind, int steps, const NsMatrices* q, int count) {
 
 template <int DT> static void ns_launch(int kind, NsProblem& p, const Layout& L, char* base, const NsOptions& o, const Plan& P, hipStream_t s) {
     Ws ws; ws.mats = (Mat*)(base + L.mats); for (int k = 0; k < SYMS; ++k) { ws.sym[k] = (Item*)(base + L.sym[k]); ws.red[k] = (Item*)(base + L.red[k]); } ws.nn = (Item*)(base + L.nn); ws.pk = (Item*)(base + L.pk); ws.fac = (Fac*)(base + L.fac); ws.part = (double*)(base + L.part); ws.split = base + L.split; ws.buf = base + L.buf;
-    const int bytes = DT == NS_F32 ? 4 : 2, steps = o.steps;
+    const int steps = o.steps;
     if (const int mt = ns_small(kind, p.d)) {
         const double a = o.coef[0], b = o.coef[1], c = o.coef[2];
         SmallArgs q{steps, (float)(SA / (SX * SX)), (float)(c * SB / (SA * SA)), (float)(b * SB / SA), (float)(1.0 / SB), (float)a, (float)(1.0 / (SB * SX)), (float)(a / SX), (float)(1.0 - o.lr * o.weight_decay),
-                    o.eps, P.grow, MuonArgs{(float)o.momentum, o.grad_scale, o.nesterov}, bytes};
+                    o.eps, P.grow, MuonArgs{(float)o.momentum, o.grad_scale, o.nesterov}, DT == NS_F32 ? 4 : 2};
         if (mt == 1) small_launch<1, DT>(kind, p, q, s); else small_launch<2, DT>(kind, p, q, s);
         return;
-    }
-    if (kind == NS_MUON)
-        for (size_t i = 0; i < p.d.size(); i += MUON_DESCS) {
-            DescPack<MUON_DESCS, 2> dp; const int n = (int)std::min<size_t>(MUON_DESCS, p.d.size() - i);
-            for (int k = 0; k < n; ++k) { dp.d[k] = p.d[i + k]; for (int u = 0; u < 2; ++u) dp.u[k][u] = p.u[(i + k) * 2 + u]; }
-            hipLaunchKernelGGL((ns_setup_kernel<MUON_DESCS, 2>), dim3(1, n), dim3(256), 0, s, dp, p.st, p.cuts, bytes, ws);
-        }
-    else {
-        const dim3 grid(std::min(p.d[0].batch, 1024));
-        if (kind == NS_BACKWARD) { DescPack<1, 4> dp; dp.d[0] = p.d[0]; for (int u = 0; u < 4; ++u) dp.u[0][u] = p.u[u]; hipLaunchKernelGGL((ns_setup_kernel<1, 4>), grid, dim3(256), 0, s, dp, p.st, p.cuts, bytes, ws); }
-        else { DescPack<1, 2> dp; dp.d[0] = p.d[0]; for (int u = 0; u < 2; ++u) dp.u[0][u] = p.u[u]; hipLaunchKernelGGL((ns_setup_kernel<1, 2>), grid, dim3(256), 0, s, dp, p.st, p.cuts, bytes, ws); }
     }
     const dim3 blk(256), pk((unsigned)L.n_pk), nn((unsigned)L.n_nn);
 #define NN(dt, out) do { if (p.cuts.nn_tile == 128) hipLaunchKernelGGL((ns_nn_kernel<128, dt, out>), nn, blk, 0, s, ws, f, dots); \
@@ -1076,11 +1077,16 @@ template <int DT> static void ns_launch(int kind, NsProblem& p, const Layout& L,
     double *xpart = ws.part, *dpart = ws.part + L.n_pk, *dots = ws.part + 2 * L.n_pk;
     auto sg = [&](int k) { return pow2_below(16384.0 / P.growth[k]); };                 // scale of dL/dX_k (of dout / |dout|: at most growth[k])
     if (kind == NS_MUON) {
-        hipLaunchKernelGGL((ns_norm_kernel<NS_F32, SRC_MUON>), pk, blk, 0, s, ws, mu);
+        for (size_t i = 0; i < p.d.size(); i += MUON_DESCS) {
+            DescPack<MUON_DESCS, 2> dp; const int n = (int)std::min<size_t>(MUON_DESCS, p.d.size() - i); const int64_t next = i + n < p.d.size() ? p.d[i + n].pk0 : L.n_pk;
+            for (int k = 0; k < n; ++k) { dp.d[k] = p.d[i + k]; for (int u = 0; u < 2; ++u) dp.u[k][u] = p.u[(i + k) * 2 + u]; }
+            hipLaunchKernelGGL((ns_start_kernel<NS_F32, SRC_MUON, MUON_DESCS, 2>), dim3((unsigned)(n + next - p.d[i].pk0)), blk, 0, s, dp, n, n, (int)L.n_pk, p.st, p.cuts, ws, mu);
+        }
         hipLaunchKernelGGL((ns_pack_kernel<NS_F32, SRC_MUON>), pk, blk, 0, s, ws, mu, SX, o.eps, P.grow, 0, 0.0);
     } else {
-        const dim3 both(pk.x, back ? 2 : 1);
-        hipLaunchKernelGGL((ns_norm_kernel<DT, SRC_X>), both, blk, 0, s, ws, mu);
+        const int tables = std::min(p.d[0].batch, 1024); const dim3 both(pk.x, back ? 2 : 1), start(pk.x + tables, both.y);
+        if (back) { DescPack<1, 4> dp; dp.d[0] = p.d[0]; for (int u = 0; u < 4; ++u) dp.u[0][u] = p.u[u]; hipLaunchKernelGGL((ns_start_kernel<DT, SRC_X, 1, 4>), start, blk, 0, s, dp, 1, tables, (int)L.n_pk, p.st, p.cuts, ws, mu); }
+        else { DescPack<1, 2> dp; dp.d[0] = p.d[0]; for (int u = 0; u < 2; ++u) dp.u[0][u] = p.u[u]; hipLaunchKernelGGL((ns_start_kernel<DT, SRC_X, 1, 2>), start, blk, 0, s, dp, 1, tables, (int)L.n_pk, p.st, p.cuts, ws, mu); }
         hipLaunchKernelGGL((ns_pack_kernel<DT, SRC_X>), both, blk, 0, s, ws, mu, SX, o.eps, P.grow, steps, back ? sg(steps) : 0.0);
     }
     const int nX = p.nX;
