@@ -186,7 +186,7 @@ template <int DT, int SRC, bool UPDATE> __device__ inline void load_tile(const M
         return;
     }
     const bool turn = ss == 1 && sl != 1;
-#pragma unroll 1
+#pragma unroll (SRC == SRC_MUON ? 1 : 2)
     for (int h = 0; h < 2; ++h) {
         float x[16], g[16];
         auto at = [&](int q, int& i, int& j) { const int id = h * 4096 + q * 256 + t; i = turn ? id & 63 : id >> 7; j = turn ? id >> 6 : id & 127; };
@@ -248,6 +248,8 @@ __device__ inline double norm_of(const Mat& M, const double* part, double* red) 
 template <int DT, int SRC> __global__ __launch_bounds__(256) void ns_pack_kernel(Ws ws, MuonArgs mu, double scale, double eps, double grow, int d_slot, double d_scale) {
     __shared__ float lds[PK_ROWS * (PK_COLS + 1)]; __shared__ double red[4];
     const Item it = ws.pk[blockIdx.x]; const Mat M = ws.mats[it.mat]; const bool dout = SRC == SRC_X && blockIdx.y;
+    float v[8][4];                                               // (before the norm: its sums wait for memory too)
+    if (dout) load_tile<DT, SRC_DOUT, false>(M, it, mu, v, lds); else load_tile<DT, SRC, false>(M, it, mu, v, lds);
     const double norm = norm_of(M, ws.part + (dout ? gridDim.x : 0), red);
     if (dout) { scale = d_scale; eps = 0; }
     else {
@@ -258,8 +260,6 @@ template <int DT, int SRC> __global__ __launch_bounds__(256) void ns_pack_kernel
     }
     const double fd = norm <= eps ? (norm > 0 ? scale / eps : 0.0) : scale / norm;     // (a NaN norm stays one; zeros stay zeros, however small eps is)
     int fe; const float f = (float)frexp(fd, &fe);               // mantissa and exponent apart: 1 / norm may lie outside fp32's range where the product does not
-    float v[8][4];
-    if (dout) load_tile<DT, SRC_DOUT, false>(M, it, mu, v, lds); else load_tile<DT, SRC, false>(M, it, mu, v, lds);
     char* out = M.buf + (dout ? d_slot : 0) * M.xbytes; const int64_t rb = (int64_t)M.np * 4;
 #pragma unroll
     for (int p = 0; p < 8; ++p) {
@@ -686,21 +686,25 @@ template <int T, int DT, int OUT> __global__ __launch_bounds__(256, T == 128 ? 2
 template <int DT> __global__ __launch_bounds__(256) void ns_back_finish_kernel(Ws ws, const double* xpart, const double* dpart, const double* dots, Slot g, Slot x0, double gscale, double xscale, double eps) {
     __shared__ float lds[PK_ROWS * (PK_COLS + 1)]; __shared__ double red[4];
     const Item it = ws.pk[blockIdx.x]; const Mat M = ws.mats[it.mat];
+    const int64_t xrb = (int64_t)M.np * 4; const int t = threadIdx.x; const bool turn = M.ys == 1 && M.yl != 1;
+    f32x4 G[8]; f16x4 xh[8], xl[8];                              // (before the sums, which wait for memory too)
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+        const int i = it.ti * PK_ROWS + p * 8 + (t >> 5), j = it.tj * PK_COLS + (t & 31) * 4; const char* X0 = slot(M, x0) + pair_off(xrb, i, j);
+        G[p] = *reinterpret_cast<const f32x4*>(slot(M, g) + i * xrb + (int64_t)j * 4); xh[p] = *reinterpret_cast<const f16x4*>(X0); xl[p] = *reinterpret_cast<const f16x4*>(X0 + LO);
+    }
     const double norm = norm_of(M, xpart, red), dnorm = norm_of(M, dpart, red);
     double along = 0;
     for (int q = threadIdx.x; q < M.nnn; q += 256) along += dots[M.nn0 + q];
     along = block_sum(along, red) / xscale;
     const bool clamped = norm <= eps;
     const float fg = (float)(dnorm / gscale / (clamped ? eps : norm)), fx = clamped ? 0.f : (float)(along * (dnorm / gscale) / norm / xscale);
-    const int64_t xrb = (int64_t)M.np * 4; const int t = threadIdx.x; const bool turn = M.ys == 1 && M.yl != 1;
 #pragma unroll
     for (int p = 0; p < 8; ++p) {
         const int li = p * 8 + (t >> 5), lj = (t & 31) * 4, i = it.ti * PK_ROWS + li, j = it.tj * PK_COLS + lj;
-        const f32x4 G = *reinterpret_cast<const f32x4*>(slot(M, g) + i * xrb + (int64_t)j * 4);
-        const char* X0 = slot(M, x0) + pair_off(xrb, i, j); const f16x4 xh = *reinterpret_cast<const f16x4*>(X0), xl = *reinterpret_cast<const f16x4*>(X0 + LO);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float v = clamped ? G[e] * fg : G[e] * fg - ((float)xh[e] + (float)xl[e]) * fx;
+            const float v = clamped ? G[p][e] * fg : G[p][e] * fg - ((float)xh[p][e] + (float)xl[p][e]) * fx;
             if (turn) lds[li * (PK_COLS + 1) + lj + e] = v;
             else if (i < M.m && j + e < M.n) st_el<DT>(M.y, i * M.ys + (j + e) * M.yl, v);
         }
