@@ -158,7 +158,8 @@ __device__ inline float momentum_step(float m, float g, const MuonArgs& mu) { re
 __device__ inline float muon_u(float m, float g, const MuonArgs& mu) { return mu.nesterov ? mu.beta * m + (1.f - mu.beta) * (mu.gscale * g) : m; }
 // One 64 x 128 tile of the source, 8 values of each of the thread's four columns: v[p][e] = element (p * 8 + t / 32, (t % 32) * 4 + e).
 // Rows whose long side is contiguous and aligned are read as vectors; any other source element by element along its contiguous side (neighbouring lanes, neighbouring addresses) and
-// through LDS.  All of a thread's loads are issued before the first is used.  UPDATE: the momentum moves on and is written back.
+// through LDS.  All of a thread's loads are issued before the first is used: what lies outside reads the first row or element instead and is dropped (behind a branch each 16-bit load
+// waited for its conversion: 10 - 12 us a launch against 6).  UPDATE: the momentum moves on and is written back.
 template <int DT, int SRC, bool UPDATE> __device__ inline void load_tile(const Mat& M, const Item& it, const MuonArgs& mu, float v[8][4], float* lds) {
     const int t = threadIdx.x, i0 = it.ti * PK_ROWS, j0 = it.tj * PK_COLS; constexpr int EL = DT == NS_F32 ? 4 : 2;
     const char* src = SRC == SRC_DOUT ? M.d : M.x; const int64_t ss = SRC == SRC_DOUT ? M.ds : M.xs, sl = SRC == SRC_DOUT ? M.dl : M.xl;
@@ -168,10 +169,12 @@ template <int DT, int SRC, bool UPDATE> __device__ inline void load_tile(const M
         f32x4 x[8], g[8]; const int j = j0 + (t & 31) * 4;
 #pragma unroll
         for (int p = 0; p < 8; ++p) {
-            const int i = i0 + p * 8 + (t >> 5); const int64_t o = i * ss + j;
-            x[p] = i < M.m ? ld_el4<DT>(src, o) : f32x4{0, 0, 0, 0};
-            if constexpr (SRC == SRC_MUON) g[p] = i < M.m ? *reinterpret_cast<const f32x4*>(M.d + o * 4) : f32x4{0, 0, 0, 0};
+            const int i = i0 + p * 8 + (t >> 5); const int64_t o = (i < M.m ? i * ss : 0) + j;
+            x[p] = ld_el4<DT>(src, o);
+            if constexpr (SRC == SRC_MUON) g[p] = *reinterpret_cast<const f32x4*>(M.d + o * 4);
         }
+#pragma unroll
+        for (int p = 0; p < 8; ++p) if (i0 + p * 8 + (t >> 5) >= M.m) { x[p] = f32x4{0, 0, 0, 0}; if constexpr (SRC == SRC_MUON) g[p] = f32x4{0, 0, 0, 0}; }
 #pragma unroll
         for (int p = 0; p < 8; ++p) {
             const int i = i0 + p * 8 + (t >> 5);
@@ -192,9 +195,11 @@ template <int DT, int SRC, bool UPDATE> __device__ inline void load_tile(const M
         auto at = [&](int q, int& i, int& j) { const int id = h * 4096 + q * 256 + t; i = turn ? id & 63 : id >> 7; j = turn ? id >> 6 : id & 127; };
 #pragma unroll
         for (int q = 0; q < 16; ++q) {
-            int i, j; at(q, i, j); const bool in = i0 + i < M.m && j0 + j < M.n; const int64_t o = (i0 + i) * ss + (j0 + j) * sl;
-            x[q] = in ? ld_el<DT>(src, o) : 0.f;
-            if constexpr (SRC == SRC_MUON) g[q] = in ? reinterpret_cast<const float*>(M.d)[o] : 0.f;
+            int i, j; at(q, i, j); const bool in = i0 + i < M.m && j0 + j < M.n; const int64_t o = in ? (i0 + i) * ss + (j0 + j) * sl : 0;
+            x[q] = ld_el<DT>(src, o);
+            if constexpr (SRC == SRC_MUON) g[q] = reinterpret_cast<const float*>(M.d)[o];
+            x[q] = in ? x[q] : 0.f;
+            if constexpr (SRC == SRC_MUON) g[q] = in ? g[q] : 0.f;
         }
 #pragma unroll
         for (int q = 0; q < 16; ++q) {
@@ -747,8 +752,8 @@ template <int MT, int DT, int MUON, int N> __global__ __launch_bounds__(512) voi
         for (int u = 0; u < 8; ++u) {
             const int q = q0 + u * 512 + t, i = along ? q / cols : q % C::MP, j = along ? q % cols : q / C::MP;
             at[u] = q < all ? i * S + (((j >> 4) ^ (i & 3)) << 6) + (j & 15) * 4 : -1; o[u] = q < all && i < m && j < n ? i * ss + j * sl : -1;      // (16 columns of fp32 take the 64 bytes of their block)
-            x[u] = o[u] >= 0 ? ld_el<DT>(src, o[u]) : 0.f;
-            if constexpr (MUON) g[u] = o[u] >= 0 ? reinterpret_cast<const float*>(D.d)[o[u]] : 0.f;
+            x[u] = ld_el<DT>(src, o[u] >= 0 ? o[u] : 0); x[u] = o[u] >= 0 ? x[u] : 0.f;      // (no branch around a load, as in load_tile)
+            if constexpr (MUON) { g[u] = reinterpret_cast<const float*>(D.d)[o[u] >= 0 ? o[u] : 0]; g[u] = o[u] >= 0 ? g[u] : 0.f; }
         }
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
