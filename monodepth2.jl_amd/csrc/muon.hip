@@ -248,7 +248,7 @@ __device__ inline double norm_of(const Mat& M, const double* part, double* red) 
     return sqrt(block_sum(s, red));
 }
 // scale * source / max(norm, eps) as pairs; the pullback's second half of the grid: d_scale * dout / |dout| into d_slot.
-// Where the norm r = |X| / eps is clamped, X0 may be too small for f16: it is carried 2^q larger, 2^q r grow <= 4 (grow: by how much all steps can grow a singular value), so A, B, S and V
+// Where the norm r = |X| / eps is clamped, X0 may be too small for f16: it is carried 2^q larger, 2^q r grow <= 4 (grow: by how much all steps can grow a singular value; the pullback: Plan::carry), so A, B, S and V
 // are 2^2q, 2^2q, 2^q and 2^q larger, and what has one factor of A too many (A A, S A, B X, V X) is multiplied by 2^-2q.  q = 0 for every other matrix.
 template <int DT, int SRC> __global__ __launch_bounds__(256) void ns_pack_kernel(Ws ws, MuonArgs mu, double scale, double eps, double grow, int d_slot, double d_scale) {
     __shared__ float lds[PK_ROWS * (PK_COLS + 1)]; __shared__ double red[4];
@@ -916,7 +916,8 @@ template <int MT, int DT, int MUON, int N> __global__ __launch_bounds__(512) voi
 
 // ---- host -------------------------------------------------------------------------------------------------------------------
 // Bounds of what the iteration can meet, from the scalar polynomial on [0, s]: the iterates' singular values, B's, and by how much a step of the pullback can grow G
-struct Plan { bool ok = false; const char* why = ""; double grow = 1, growth[MD2_NS_MAX_STEPS + 1] = {}, s[MD2_NS_MAX_STEPS + 1] = {}, vgain[MD2_NS_MAX_STEPS] = {}; };
+// grow, carry: a clamped matrix is carried at most 4 / (r grow) larger, the pullback's at most 4 / (r carry) (ns_pack_kernel)
+struct Plan { bool ok = false; const char* why = ""; double grow = 1, carry = 1, growth[MD2_NS_MAX_STEPS + 1] = {}, s[MD2_NS_MAX_STEPS + 1] = {}, vgain[MD2_NS_MAX_STEPS] = {}; };
 Plan ns_bounds(int steps, const double* co, bool back) {
     Plan P;
     if (steps < 1 || steps > MD2_NS_MAX_STEPS) { P.why = "steps must be in 1..16"; return P; }
@@ -927,7 +928,7 @@ Plan ns_bounds(int steps, const double* co, bool back) {
         double r = std::max(std::fabs(k0), std::fabs(k0 + U * (k1 + U * k2))); const double v = k2 != 0 ? -k1 / (2 * k2) : -1;
         return v > 0 && v < U ? std::max(r, std::fabs(k0 + v * (k1 + v * k2))) : r;
     };
-    double lip[MD2_NS_MAX_STEPS]; P.s[0] = 1.0;
+    double lip[MD2_NS_MAX_STEPS], gain = 1.0, carry = 0.0; P.s[0] = 1.0;      // gain: how much larger than r = |X0| the iterate can be
     for (int k = 0; k < steps; ++k) {
         const double U = P.s[k] * P.s[k]; auto at = [&](double u) { return std::fabs(std::sqrt(u) * (a + u * (b + u * c))); };
         double top = at(U); const double disc = 9 * b * b - 20 * a * c, den = 10 * c;
@@ -937,7 +938,12 @@ Plan ns_bounds(int steps, const double* co, bool back) {
         P.s[k + 1] = top * 1.001; lip[k] = L * 1.001; P.vgain[k] = std::fabs(b) + 2 * std::fabs(c) * U;
         if (!(P.s[k + 1] <= 4.0) || !(bm <= 60.0)) { P.why = "these coefficients let a singular value grow past 4 (or b s^2 + c s^4 past 60)"; return P; }
         P.grow *= std::max(up, 1.0) * 1.001;
+        if (gain > 0 && P.s[k] > 0) carry = std::max(carry, 4.0 * gain / P.s[k]);
+        gain *= up * 1.001;
     }
+    // The forward products hold a carried iterate of up to 4, whatever s[k] is; the pullback's S and V are scaled by s[k], so there a carried iterate, 2^q r gain, stays below s[k] as well.
+    // (With coefficients that shrink singular values s[k] falls below 4 gain / grow, and S would pass f16's range.  With the default ones it does not: carry = grow.)
+    P.carry = std::max(P.grow, carry);
     P.growth[steps] = 1.0;
     for (int k = steps - 1; k >= 0; --k) P.growth[k] = P.growth[k + 1] * std::max(lip[k], 1.0);
     if (back && !(P.growth[0] <= 8192.0)) { P.why = "the pullback of this many steps can grow a gradient past 8192 times its norm"; return P; }
@@ -1096,7 +1102,7 @@ template <int DT> static void ns_launch(int kind, NsProblem& p, const Layout& L,
         const int tables = std::min(p.d[0].batch, 1024); const dim3 both(pk.x, back ? 2 : 1), start(pk.x + tables, both.y);
         if (back) { DescPack<1, 4> dp; dp.d[0] = p.d[0]; for (int u = 0; u < 4; ++u) dp.u[0][u] = p.u[u]; hipLaunchKernelGGL((ns_start_kernel<DT, SRC_X, 1, 4>), start, blk, 0, s, dp, 1, tables, (int)L.n_pk, p.st, p.cuts, ws, mu); }
         else { DescPack<1, 2> dp; dp.d[0] = p.d[0]; for (int u = 0; u < 2; ++u) dp.u[0][u] = p.u[u]; hipLaunchKernelGGL((ns_start_kernel<DT, SRC_X, 1, 2>), start, blk, 0, s, dp, 1, tables, (int)L.n_pk, p.st, p.cuts, ws, mu); }
-        hipLaunchKernelGGL((ns_pack_kernel<DT, SRC_X>), both, blk, 0, s, ws, mu, SX, o.eps, P.grow, steps, back ? sg(steps) : 0.0);
+        hipLaunchKernelGGL((ns_pack_kernel<DT, SRC_X>), both, blk, 0, s, ws, mu, SX, o.eps, back ? P.carry : P.grow, steps, back ? sg(steps) : 0.0);
     }
     const int nX = p.nX;
     auto X = [&](int k) { return Slot{back ? k : (k & 1), 0}; };

@@ -579,3 +579,16 @@ def test_more_work_than_a_launch_can_hold_is_refused():
     """(such a call's workspace would be 16 TB and more)"""
     L = md2amd._lib.lib()
     assert L.md2_newton_schulz_workspace(1 << 20, 1000, 2000, 5, 0) == -1 and L.md2_newton_schulz_workspace(1 << 20, 100, 200, 5, 0) > 0
+
+
+# ---- ranges of the numbers inside --------------------------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("shape", [(1, 1), (20, 30), (70, 90), (200, 130)])
+@pytest.mark.parametrize("coef,steps", [((1.0, -1.0, 0.0), 2), ((0.75, 0.0, -0.25), 3), ((0.5, 0.0, 0.0), 6)])
+def test_pullback_of_a_clamped_matrix_with_coefficients_that_shrink(shape, coef, steps):
+    """A matrix below eps is carried larger; where the coefficients let singular values shrink, an iterate must not be carried past the bound by which G X^T is scaled (its pairs would be
+    infinite, the next product NaN).  One entry holds nearly all of x and dout, so that entries come as near to the norms' bounds as they can."""
+    g = torch.Generator().manual_seed(3); z = 1e-3 * torch.randn(shape, generator=g, dtype=torch.float64) / max(shape); z[shape[0] // 2, shape[1] // 3] = 1.0; z /= z.norm()
+    for r in (0.01, 0.03, 0.06, 0.1, 0.2, 0.3, 0.45, 0.7):
+        x, d = (z * r * 1e-7).float().cuda(), z.float().cuda()
+        check_back(md().newton_schulz_pullback(x, d, steps=steps, coefficients=coef), x, d, steps, coef)
