@@ -702,14 +702,15 @@ template <int DT> __global__ __launch_bounds__(256) void ns_back_finish_kernel(W
     double along = 0;
     for (int q = threadIdx.x; q < M.nnn; q += 256) along += dots[M.nn0 + q];
     along = block_sum(along, red) / xscale;
-    const bool clamped = norm <= eps;
-    const float fg = (float)(dnorm / gscale / (clamped ? eps : norm)), fx = clamped ? 0.f : (float)(along * (dnorm / gscale) / norm / xscale);
+    // |dout| / (gscale |x|) as a factor in [1/2, 2) and a power of two: by itself it leaves fp32's range before dx does (G may be 2^14), and would turn zeros into NaN beyond it
+    const bool clamped = norm <= eps; int ed, en; const double md = frexp(dnorm / gscale, &ed), mn = frexp(clamped ? eps : norm, &en);
+    const float fg = (float)(md / mn), fx = clamped ? 0.f : (float)(along * (md / mn) / xscale); const int fe = ed - en;
 #pragma unroll
     for (int p = 0; p < 8; ++p) {
         const int li = p * 8 + (t >> 5), lj = (t & 31) * 4, i = it.ti * PK_ROWS + li, j = it.tj * PK_COLS + lj;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float v = clamped ? G[p][e] * fg : G[p][e] * fg - ((float)xh[p][e] + (float)xl[p][e]) * fx;
+            const float v = ldexpf(clamped ? G[p][e] * fg : G[p][e] * fg - ((float)xh[p][e] + (float)xl[p][e]) * fx, fe);
             if (turn) lds[li * (PK_COLS + 1) + lj + e] = v;
             else if (i < M.m && j + e < M.n) st_el<DT>(M.y, i * M.ys + (j + e) * M.yl, v);
         }

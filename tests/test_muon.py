@@ -592,3 +592,19 @@ def test_pullback_of_a_clamped_matrix_with_coefficients_that_shrink(shape, coef,
     for r in (0.01, 0.03, 0.06, 0.1, 0.2, 0.3, 0.45, 0.7):
         x, d = (z * r * 1e-7).float().cuda(), z.float().cuda()
         check_back(md().newton_schulz_pullback(x, d, steps=steps, coefficients=coef), x, d, steps, coef)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(3, 5), (70, 90)])
+def test_pullback_of_the_smallest_and_largest_gradients(shape, dtype):
+    """dx = (dout - X0 <X0, dout>) / |x| for coefficients (1, 0, 0).  Powers of two scale x and dout until |dout| / |x| is subnormal times 2^14: the normal dx has the bits of the unscaled
+    call's, moved by the exponent.  Where dx passes fp32's range it is infinite, and its zeros stay zeros."""
+    m = md(); x = gradient_like(shape, 51, noise=1.0, scale=1.0); x[0, 0] = 9 * x.norm(); d = torch.randn(shape, generator=torch.Generator().manual_seed(52), dtype=torch.float64)
+    x, d = (x / x.norm()).to(dtype).cuda(), d.to(dtype).cuda(); ref = m.newton_schulz_pullback(x, d, steps=1, coefficients=(1.0, 0.0, 0.0)).double()
+    for sx, sd in ((2.0 ** 60, 2.0 ** -63), (2.0 ** 30, 2.0 ** -94), (2.0 ** 62, 2.0 ** -60), (2.0 ** -40, 2.0 ** 80)):
+        got = m.newton_schulz_pullback(x * sx, d * sd, steps=1, coefficients=(1.0, 0.0, 0.0), eps=1e-30).double(); want = ref * (sd / sx); normal = want.abs() >= 2.0 ** -125
+        assert normal.sum() >= want.numel() // 4 and torch.equal(got[normal], want[normal]), (sx, sd)
+    for eps in (1e-12, 1e-320):                                  # a^5 / eps dout, past 3.4e38 everywhere but where dout is 0
+        z = d * 1e30; z[1:] = 0; got = m.newton_schulz_pullback(torch.zeros_like(x), z, eps=eps)
+        assert torch.equal(got[0], torch.copysign(torch.full_like(z[0], math.inf), z[0])) and not got[1:].any()
