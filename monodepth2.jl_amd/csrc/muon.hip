@@ -141,7 +141,7 @@ __device__ inline double block_sum(double v, double* red) {
     return (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-struct MuonArgs { float beta, gscale; int nesterov; };
+struct MuonArgs { float beta, rest, gscale; int nesterov; };      // rest = 1 - beta, rounded once: 1.f - beta loses it as beta nears 1
 enum { SRC_X = 0, SRC_DOUT = 1, SRC_MUON = 2 };
 
 // four neighbouring elements, aligned to their size together
@@ -154,8 +154,8 @@ template <int DT> __device__ inline f32x4 ld_el4(const char* p, int64_t i) {
         return r;
     }
 }
-__device__ inline float momentum_step(float m, float g, const MuonArgs& mu) { return mu.beta * m + (1.f - mu.beta) * (mu.gscale * g); }
-__device__ inline float muon_u(float m, float g, const MuonArgs& mu) { return mu.nesterov ? mu.beta * m + (1.f - mu.beta) * (mu.gscale * g) : m; }
+__device__ inline float momentum_step(float m, float g, const MuonArgs& mu) { return mu.beta * m + mu.rest * (mu.gscale * g); }
+__device__ inline float muon_u(float m, float g, const MuonArgs& mu) { return mu.nesterov ? mu.beta * m + mu.rest * (mu.gscale * g) : m; }
 // One 64 x 128 tile of the source, 8 values of each of the thread's four columns: v[p][e] = element (p * 8 + t / 32, (t % 32) * 4 + e).
 // Rows whose long side is contiguous and aligned are read as vectors; any other source element by element along its contiguous side (neighbouring lanes, neighbouring addresses) and
 // through LDS.  All of a thread's loads are issued before the first is used: what lies outside reads the first row or element instead and is dropped (behind a branch each 16-bit load
@@ -1072,7 +1072,7 @@ template <int DT> static void ns_launch(int kind, NsProblem& p, const Layout& L,
     if (const int mt = ns_small(kind, p.d)) {
         const double a = o.coef[0], b = o.coef[1], c = o.coef[2];
         SmallArgs q{steps, (float)(SA / (SX * SX)), (float)(c * SB / (SA * SA)), (float)(b * SB / SA), (float)(1.0 / SB), (float)a, (float)(1.0 / (SB * SX)), (float)(a / SX), (float)(1.0 - o.lr * o.weight_decay),
-                    o.eps, P.grow, MuonArgs{(float)o.momentum, o.grad_scale, o.nesterov}, DT == NS_F32 ? 4 : 2};
+                    o.eps, P.grow, MuonArgs{(float)o.momentum, (float)(1.0 - o.momentum), o.grad_scale, o.nesterov}, DT == NS_F32 ? 4 : 2};
         if (mt == 1) small_launch<1, DT>(kind, p, q, s); else small_launch<2, DT>(kind, p, q, s);
         return;
     }
@@ -1087,7 +1087,7 @@ template <int DT> static void ns_launch(int kind, NsProblem& p, const Layout& L,
         if (p.cuts.sym[a.kind].tile == 128) hipLaunchKernelGGL((ns_reduce_kernel<128>), dim3((unsigned)L.n_red[a.kind] * 8), blk, 0, s, ws, a);
         else hipLaunchKernelGGL((ns_reduce_kernel<64>), dim3((unsigned)L.n_red[a.kind] * 2), blk, 0, s, ws, a);
     };
-    const MuonArgs mu{(float)o.momentum, o.grad_scale, o.nesterov};
+    const MuonArgs mu{(float)o.momentum, (float)(1.0 - o.momentum), o.grad_scale, o.nesterov};
     const double a = o.coef[0], b = o.coef[1], c = o.coef[2];
     const bool back = kind == NS_BACKWARD;
     double *xpart = ws.part, *dpart = ws.part + L.n_pk, *dots = ws.part + 2 * L.n_pk;

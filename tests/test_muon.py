@@ -608,3 +608,15 @@ def test_pullback_of_the_smallest_and_largest_gradients(shape, dtype):
     for eps in (1e-12, 1e-320):                                  # a^5 / eps dout, past 3.4e38 everywhere but where dout is 0
         z = d * 1e30; z[1:] = 0; got = m.newton_schulz_pullback(torch.zeros_like(x), z, eps=eps)
         assert torch.equal(got[0], torch.copysign(torch.full_like(z[0], math.inf), z[0])) and not got[1:].any()
+
+
+@gpu
+@pytest.mark.parametrize("momentum", [0.9999, 1 - 1e-7, 1 - 1e-8])
+@pytest.mark.parametrize("shape", [(24, 40), (70, 90)])
+def test_a_momentum_next_to_one(shape, momentum):
+    """From zero, m = (1 - momentum) g: three roundings (1 - momentum, grad_scale g, their product), however near 1 the momentum is.  The direction does not depend on the size of u."""
+    p, g, mo = torch.zeros(shape, device="cuda"), gradient_like(shape, 61, noise=1.0, scale=1.0).float().cuda(), torch.zeros(shape, device="cuda")
+    md().muon_raw([p], [g], [mo], lr=1.0, momentum=momentum, nesterov=False, grad_scale=0.75, eps=1e-30)
+    want = (1 - momentum) * 0.75 * g.double()
+    assert float(((mo.double() - want).abs() / want.abs()).max()) <= 4 * 2.0 ** -24
+    check(-p, want.float(), eps=1e-30)
