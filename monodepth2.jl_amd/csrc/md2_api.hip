@@ -1536,6 +1536,7 @@ static const char* muon_check(const MuonHyper& y) {
     if (!(y.weight_decay >= 0) || !std::isfinite(y.weight_decay)) return "weight_decay must be finite and not negative";
     if (y.adjust != 0 && y.adjust != 1) return "adjust must be 0 (spectral) or 1 (rms)";
     if (!std::isfinite(y.grad_scale)) return "grad_scale must be finite";
+    if (!std::isfinite((float)(1.0 - y.lr * y.weight_decay))) return "lr times weight_decay leaves fp32's range";
     return nullptr;
 }
 static NsMatrices muon_matrix(float* p, const float* g, float* m, int64_t rows, int64_t cols, const MuonHyper& y) {
@@ -1545,9 +1546,14 @@ static NsMatrices muon_matrix(float* p, const float* g, float* m, int64_t rows, 
     q.alpha = (float)(y.lr * s);
     return q;
 }
+static const char* muon_alphas(const std::vector<NsMatrices>& q) {
+    for (const NsMatrices& m : q) if (!std::isfinite(m.alpha)) return "lr times a weight's shape factor leaves fp32's range";
+    return nullptr;
+}
 static int muon_run(const char* what, const std::vector<NsMatrices>& q, const MuonHyper& y, void* ws, int64_t ws_bytes, hipStream_t s, const char** why) {
     if ((*why = muon_check(y))) return 2;
     NsOptions o; if (ns_options(o, y.steps, y.co, y.eps, what)) { *why = "null coefficients"; return 2; }
+    if ((*why = muon_alphas(q))) return 2;
     o.lr = y.lr; o.momentum = y.momentum; o.nesterov = y.nesterov != 0; o.weight_decay = y.weight_decay; o.grad_scale = y.grad_scale;
     return ns_run(NS_MUON, NS_F32, q.data(), (int)q.size(), o, ws, ws_bytes, s, why);
 }
@@ -1614,9 +1620,11 @@ int32_t md2_muon_step(md2_handle* h, double lr, double momentum, int32_t nestero
         hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
         if (hipStreamIsCapturing(h->stream, &capturing) != hipSuccess) (void)hipGetLastError();
         if (capturing != hipStreamCaptureStatusNone) { h->err = "md2_muon_step cannot be captured into a graph: the ADAM part's bias corrections change with every step (md2_muon_raw can)"; return 2; }
-        if (!h->MU) if (int r = muon_alloc(h)) return r;
         std::vector<NsMatrices> q;
-        for (const ConvL* c : muon_convs(h)) q.push_back(muon_matrix(h->P + c->w, h->G + c->w, h->MU + c->w, c->coutP, (int64_t)c->taps * c->cinP, y));
+        for (const ConvL* c : muon_convs(h)) q.push_back(muon_matrix(h->P + c->w, h->G + c->w, nullptr, c->coutP, (int64_t)c->taps * c->cinP, y));
+        if ((why = muon_alphas(q))) { h->err = std::string("md2_muon_step: ") + why; return 2; }      // (before the handle becomes Muon's)
+        if (!h->MU) if (int r = muon_alloc(h)) return r;
+        size_t i = 0; for (const ConvL* c : muon_convs(h)) q[i++].x = h->MU + c->w;
         if (int r = muon_run("md2_muon_step", q, y, h->mu_ws, INT64_MAX, h->stream, &why)) { h->err = std::string("md2_muon_step: ") + why; return r; }
         h->beta1p *= 0.9; h->beta2p *= 0.999;
         launch_adam_ranges(h->P, h->G, h->M, h->V, h->mu_ranges, h->mu_nranges, h->mu_n4, (float)(1.0 - h->beta1p), (float)(1.0 - h->beta2p), (float)h->cfg.lr, grad_scale, h->stream);

@@ -620,3 +620,20 @@ def test_a_momentum_next_to_one(shape, momentum):
     want = (1 - momentum) * 0.75 * g.double()
     assert float(((mo.double() - want).abs() / want.abs()).max()) <= 4 * 2.0 ** -24
     check(-p, want.float(), eps=1e-30)
+
+
+@pytest.mark.parametrize("kw,word", [(dict(lr=1e39), "shape factor"), (dict(lr=2e38, rows=(64,), cols=(1,), p=(4096,), g=(8192,), m=(16384,)), "shape factor"), (dict(lr=1e20, decay=1e19), "weight_decay"),
+                                     (dict(lr=3e38), "workspace"), (dict(lr=1e19, decay=1e19), "workspace")])
+def test_a_learning_rate_that_no_float_holds_is_refused(kw, word):
+    """(as infinite factors they would make NaN of weights whose update is zero)"""
+    assert muon_c(**kw) == 2 and word in last_error(), last_error()
+
+
+@gpu
+def test_a_model_step_refuses_such_a_learning_rate_and_stays_adams():
+    m = md(); model, params, cache, x = make_model(); m.train_step(model, x, None, cache, params); p = model.params()
+    for kw in (dict(eta=1e38, adjust="rms"), dict(eta=1e20, weight_decay=1e19)):
+        with pytest.raises(RuntimeError, match="range"):
+            m.update(m.Muon(**kw), model)
+    assert model.muon_state() is None and np.array_equal(model.params(), p)
+    m.train_step(model, x, None, cache, params); assert not np.array_equal(model.params(), p)
