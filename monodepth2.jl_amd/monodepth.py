@@ -315,9 +315,10 @@ class Model:
 
     @lr.setter
     def lr(self, value):
-        self._lr = float(value)
+        value = float(value)
         if getattr(self, "_h", None) is not None:
-            _check(_lib.lib().md2_set_lr(self._h, self._lr), self._h, "set_lr")
+            _check(_lib.lib().md2_set_lr(self._h, value), self._h, "set_lr")
+        self._lr = value
 
     # -- handle management --------------------------------------------------------------------
     def _ensure(self, x, parameters: Optional[Params] = None, cache: Optional[TrainCache] = None, frames=None):
@@ -675,22 +676,33 @@ class Muon:
     adam_eta: float = 1e-4
 
 
+@contextlib.contextmanager
+def _step_size(model, eta):
+    """ADAM's step size for the step inside, and from then on (the property setter calls md2_set_lr); a step that is refused leaves the model its own."""
+    was = model.lr
+    if eta != was:
+        model.lr = eta
+    try:
+        yield
+    except BaseException:
+        if eta != was:
+            model.lr = was
+        raise
+
+
 def update(optimizer, model: Model, grad_scale=1.0):
     """Flux.Optimise.update!(optimizer, theta, grads) — the step size is the optimiser's eta (ADAM or Muon)."""
     if isinstance(optimizer, Muon):
         o = optimizer; h = _need_handle(model, "update"); st, co, ep = _ns_args(o.steps, o.coefficients, o.eps)
         if o.adjust not in _MUON_ADJUST:
             raise ValueError("Muon: adjust must be 'spectral' or 'rms'")
-        if o.adam_eta != model.lr:
-            model.lr = o.adam_eta
-        with torch.cuda.device(model._shape[-1] or 0):
+        with torch.cuda.device(model._shape[-1] or 0), _step_size(model, o.adam_eta):
             _lib.lib().md2_set_stream(h, _stream())
             _check(_lib.lib().md2_muon_step(h, float(o.eta), float(o.momentum), int(bool(o.nesterov)), float(o.weight_decay), _MUON_ADJUST[o.adjust], st, co, ep, float(grad_scale)), h, "muon_step")
         return
     _lib.lib().md2_set_stream(model._h, _stream())
-    if optimizer is not None and optimizer.eta != model.lr:
-        model.lr = optimizer.eta                      # (the property setter calls md2_set_lr)
-    _check(_lib.lib().md2_adam_step(model._h, float(grad_scale)), model._h, "adam_step")
+    with _step_size(model, model.lr if optimizer is None else optimizer.eta):
+        _check(_lib.lib().md2_adam_step(model._h, float(grad_scale)), model._h, "adam_step")
 
 
 def train_step(model: Model, x, auto_loss, cache: TrainCache, parameters: Params, do_update=True):

@@ -637,3 +637,50 @@ def test_a_model_step_refuses_such_a_learning_rate_and_stays_adams():
             m.update(m.Muon(**kw), model)
     assert model.muon_state() is None and np.array_equal(model.params(), p)
     m.train_step(model, x, None, cache, params); assert not np.array_equal(model.params(), p)
+
+
+# ---- a refused update changes nothing ------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("which", ["muon", "adam"])
+def test_a_refused_update_keeps_the_models_step_size(monkeypatch, which):
+    """The library's part is a stand-in that refuses the step, or the step size itself: model.lr and the handle's step size are what they were; an accepted step keeps the new one."""
+    import contextlib
+    m = md(); calls = []; answer = {"step": 2, "lr": 0}
+    class Lib:
+        def md2_set_lr(self, h, v): calls.append(v); return answer["lr"] if v < 0 else 0
+        def md2_set_stream(self, h, s): return 0
+        def md2_muon_step(self, *a): return answer["step"]
+        def md2_adam_step(self, *a): return answer["step"]
+        def md2_last_error(self, h): return b"refused"
+    monkeypatch.setattr(m._lib, "lib", lambda: Lib()); monkeypatch.setattr(m, "_stream", lambda: None); monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    model = m.Model.__new__(m.Model); model._lr, model._h, model._shape = 1e-4, 1, (0,)
+    step = (lambda eta: m.update(m.Muon(adam_eta=eta), model)) if which == "muon" else (lambda eta: m.update(m.ADAM(eta), model))
+    try:
+        with pytest.raises(RuntimeError, match="refused"):
+            step(3e-3)
+        assert model.lr == 1e-4 and (not calls or calls[-1] == 1e-4)
+        answer["lr"] = 2
+        with pytest.raises(RuntimeError, match="refused"):
+            step(-1.0)
+        assert model.lr == 1e-4
+        answer["step"] = 0; step(2e-3); assert model.lr == 2e-3 and calls[-1] == 2e-3
+    finally:
+        model._h = None
+
+
+@gpu
+def test_a_refused_step_keeps_the_handles_step_size():
+    m = md(); model, params, cache, x = make_model(); other = make_model()[0]
+    for mm in (model, other):
+        m.train_step(mm, x, None, cache, params, do_update=False)
+    for bad in (dict(eta=-1.0), dict(momentum=1.0), dict(steps=0), dict(coefficients=(9.0, 0.0, 0.0)), dict(adam_eta=-1.0)):
+        with pytest.raises(RuntimeError):
+            m.update(m.Muon(**{"adam_eta": 0.5, **bad}), model)
+    assert model.lr == 1e-4 and model.muon_state() is None
+    other.grad_buffer().copy_(model.grad_buffer()); other.param_buffer().copy_(model.param_buffer())
+    for mm in (model, other):
+        m.update(None, mm)
+    assert np.array_equal(model.params(), other.params())
+    m.update(m.Muon(adam_eta=2e-4), model)
+    with pytest.raises(RuntimeError, match="stepped by Muon"):
+        m.update(m.ADAM(0.5), model)
+    assert model.lr == 2e-4
