@@ -221,8 +221,8 @@ backward!(h) = check(h, md2_backward(h.ptr), "backward")
 adam_step!(h, grad_scale=1f0) = check(h, md2_adam_step(h.ptr, Float32(grad_scale)), "adam_step")
 # Muon for the hidden convolutions, ADAM for the rest (not in the reference)
 function muon_step!(h; eta=0.02, momentum=0.95, nesterov=true, weight_decay=0.0, adjust=:spectral, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7, grad_scale=1f0)
-    co = collect(Float64, coefficients)
-    GC.@preserve co check(h, md2_muon_step(h.ptr, Float64(eta), Float64(momentum), Int32(nesterov), Float64(weight_decay), Int32(adjust === :rms), Int32(steps), pointer(co), Float64(eps), Float32(grad_scale)), "muon_step")
+    co = ns_coefficients(coefficients); ad = muon_adjust(adjust)
+    GC.@preserve co check(h, md2_muon_step(h.ptr, Float64(eta), Float64(momentum), Int32(nesterov), Float64(weight_decay), ad, Int32(steps), pointer(co), Float64(eps), Float32(grad_scale)), "muon_step")
 end
 function muon_state(h)
     n = md2_muon_state_count(h.ptr); n == 0 && return nothing
@@ -449,23 +449,32 @@ adam_raw!(p, g, m, v, step; lr=1e-4, grad_scale=1f0) = ok(md2_adam_raw(dptr(p), 
 
 # Muon: a Julia matrix (cols, rows) is the library's row-major rows x cols; orthogonalisation does not depend on which side is called rows
 const NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
-ns_dtype(::Type{Float32}) = Int32(0); ns_dtype(::Type{Float16}) = Int32(2)
+# (Core.BFloat16 or the BFloat16s package's: by name, so that neither has to be there)
+ns_dtype(T::Type) = T === Float32 ? Int32(0) : T === Float16 ? Int32(2) : nameof(T) === :BFloat16 ? Int32(1) : throw(ArgumentError("newton_schulz: Float32, BFloat16 or Float16, not $T"))
 ns_strides(x) = Int64[size(x, 1) * size(x, 2), size(x, 1), 1]
+rawptr(x::ROCArray) = Ptr{Cvoid}(UInt(pointer(x)))                     # of any element type (dptr: Float32 only)
+ns_coefficients(c) = length(c) == 3 ? collect(Float64, c) : throw(ArgumentError("coefficients: expected (a, b, c), got $(length(c))"))
+muon_adjust(a) = a === :spectral ? Int32(0) : a === :rms ? Int32(1) : throw(ArgumentError("adjust must be :spectral or :rms, not $a"))
 function newton_schulz(x::ROCArray{T,3}; steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7) where {T}
-    K, R, B = size(x); y = similar(x); n = md2_newton_schulz_workspace(Int64(B), Int64(R), Int64(K), Int32(steps), Int32(0)); ws = ROCArray{UInt8}(undef, max(n, 0)); co = collect(Float64, coefficients); st = ns_strides(x)
-    GC.@preserve co st ok(md2_newton_schulz(dptr(x), dptr(y), Int64(B), Int64(R), Int64(K), pointer(st), ns_dtype(T), Int32(steps), pointer(co), Float64(eps), dptr(ws), n, NOSTREAM), "newton_schulz"); y
+    dt = ns_dtype(T); K, R, B = size(x); y = similar(x); n = md2_newton_schulz_workspace(Int64(B), Int64(R), Int64(K), Int32(steps), Int32(0)); ws = ROCArray{UInt8}(undef, max(n, 0)); co = ns_coefficients(coefficients); st = ns_strides(x)
+    GC.@preserve co st ws ok(md2_newton_schulz(rawptr(x), rawptr(y), Int64(B), Int64(R), Int64(K), pointer(st), dt, Int32(steps), pointer(co), Float64(eps), rawptr(ws), n, NOSTREAM), "newton_schulz"); y
 end
-function ∇newton_schulz(x::ROCArray{T,3}, Δ; steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7) where {T}
-    K, R, B = size(x); dx = similar(x); n = md2_newton_schulz_workspace(Int64(B), Int64(R), Int64(K), Int32(steps), Int32(1)); ws = ROCArray{UInt8}(undef, max(n, 0)); co = collect(Float64, coefficients); st = ns_strides(x)
-    GC.@preserve co st ok(md2_newton_schulz_bwd(dptr(x), dptr(Δ), dptr(dx), Int64(B), Int64(R), Int64(K), pointer(st), pointer(st), ns_dtype(T), Int32(steps), pointer(co), Float64(eps), dptr(ws), n, NOSTREAM), "newton_schulz_bwd"); dx
+function ∇newton_schulz(x::ROCArray{T,3}, Δ::ROCArray{T,3}; steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7) where {T}
+    size(Δ) == size(x) || throw(DimensionMismatch("∇newton_schulz: Δ is $(size(Δ)), x is $(size(x))"))
+    dt = ns_dtype(T); K, R, B = size(x); dx = similar(x); n = md2_newton_schulz_workspace(Int64(B), Int64(R), Int64(K), Int32(steps), Int32(1)); ws = ROCArray{UInt8}(undef, max(n, 0)); co = ns_coefficients(coefficients); st = ns_strides(x)
+    GC.@preserve co st ws ok(md2_newton_schulz_bwd(rawptr(x), rawptr(Δ), rawptr(dx), Int64(B), Int64(R), Int64(K), pointer(st), pointer(st), dt, Int32(steps), pointer(co), Float64(eps), rawptr(ws), n, NOSTREAM), "newton_schulz_bwd"); dx
 end
-# ps, gs, ms: vectors of Float32 arrays whose LAST dimension is the output channels (Flux conv weights (kW,kH,Cin,Cout): rows = Cout)
+# ps, gs, ms: vectors of Float32 arrays (dptr takes no others) whose LAST dimension is the output channels (Flux conv weights (kW,kH,Cin,Cout): rows = Cout)
 function muon_raw!(ps, gs, ms; lr=0.02, momentum=0.95, nesterov=true, weight_decay=0.0, adjust=:spectral, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, grad_scale=1f0)
-    rows = Int64[size(p, ndims(p)) for p in ps]; cols = Int64[length(p) ÷ size(p, ndims(p)) for p in ps]; co = collect(Float64, coefficients); P = dptr.(ps); G = dptr.(gs); M = dptr.(ms)
-    GC.@preserve rows cols co P G M begin
+    length(ps) == length(gs) == length(ms) || throw(DimensionMismatch("muon_raw!: $(length(ps)) weights, $(length(gs)) gradients, $(length(ms)) momenta"))
+    for (p, g, m) in zip(ps, gs, ms)
+        ndims(p) >= 2 && size(p) == size(g) == size(m) || throw(DimensionMismatch("muon_raw!: a weight needs two or more dimensions, and a gradient and a momentum of its size: $(size(p)), $(size(g)), $(size(m))"))
+    end
+    rows = Int64[size(p, ndims(p)) for p in ps]; cols = Int64[length(p) ÷ size(p, ndims(p)) for p in ps]; co = ns_coefficients(coefficients); P = dptr.(ps); G = dptr.(gs); M = dptr.(ms); ad = muon_adjust(adjust)
+    GC.@preserve rows cols co P G M ps gs ms begin
         n = md2_muon_workspace(pointer(rows), pointer(cols), Int32(length(ps)), Int32(steps)); ws = ROCArray{UInt8}(undef, max(n, 0))
-        ok(md2_muon_raw(pointer(P), pointer(G), pointer(M), pointer(rows), pointer(cols), Int32(length(ps)), Float64(lr), Float64(momentum), Int32(nesterov), Float64(weight_decay), Int32(adjust === :rms),
-                        Float32(grad_scale), Int32(steps), pointer(co), Float64(eps), dptr(ws), n, NOSTREAM), "muon_raw")
+        GC.@preserve ws ok(md2_muon_raw(pointer(P), pointer(G), pointer(M), pointer(rows), pointer(cols), Int32(length(ps)), Float64(lr), Float64(momentum), Int32(nesterov), Float64(weight_decay), ad,
+                                        Float32(grad_scale), Int32(steps), pointer(co), Float64(eps), rawptr(ws), n, NOSTREAM), "muon_raw")
     end
 end
 

@@ -56,3 +56,24 @@ def test_julia_param_table_matches_the_shared_layout():
     # Flux's BatchNorm yields (beta, gamma); the table holds (gamma, beta): the Julia walk must swap them
     mod = open(os.path.join(JL, "Monodepth2HIP.jl")).read()
     assert "β, γ = enc[ei], enc[ei + 1]" in mod and "out[i] = γ; out[i + 1] = β" in mod
+
+
+def test_julia_muon_functions_compare_sizes_and_types_before_the_library_reads():
+    """No pointer that the shim passes on may be shorter, or of another type, than the sizes beside it say (a size-0 `size(p, end)` fails before the call as an integer division by zero)."""
+    mod = open(os.path.join(JL, "Monodepth2HIP.jl")).read()
+    def body(name):
+        i = mod.index("\nfunction " + name); return mod[i:mod.index("\nend\n", i)]
+    back, raw, fwd, step = body("∇newton_schulz("), body("muon_raw!("), body("newton_schulz("), body("muon_step!(")
+    assert "Δ::ROCArray{T,3}" in back and back.index("size(Δ) == size(x) || throw(DimensionMismatch") < back.index("md2_newton_schulz_bwd(")
+    assert raw.index("length(ps) == length(gs) == length(ms) || throw(DimensionMismatch") < raw.index("size(p) == size(g) == size(m) || throw(DimensionMismatch") < raw.index("dptr.(ps)") < raw.index("md2_muon_raw(")
+    assert "dptr(x::ROCArray{Float32})" in mod and len(re.findall(r"^dptr\(", mod, re.M)) == 2        # Float32 arrays and nothing: bytes, Float16 and BFloat16 go through rawptr
+    for f in (fwd, back, raw):
+        assert "ROCArray{UInt8}(undef" in f and "dptr(ws)" not in f and "rawptr(ws)" in f
+    for f in (fwd, back):
+        assert "dptr(x)" not in f.replace("rawptr(x)", "") and f.index("ns_dtype(T)") < f.index("ROCArray{UInt8}")
+    for f in (raw, step):                                              # a mistyped symbol is refused, not taken for :spectral
+        assert "muon_adjust(adjust)" in f and "adjust === :rms" not in f
+    assert re.search(r"ns_dtype.*:BFloat16 \? Int32\(1\) : throw", mod) and re.search(r"muon_adjust\(a\).*throw\(ArgumentError", mod)
+    assert re.search(r"ns_coefficients\(c\) = length\(c\) == 3 \? .*throw\(ArgumentError", mod)
+    for f in (fwd, back, raw, step):                                   # the library reads three coefficients
+        assert "co = ns_coefficients(coefficients)" in f and "GC.@preserve" in f
