@@ -1843,10 +1843,19 @@ int32_t md2_broadcast_state(md2_handle* h, int32_t root) {
     NCCLCHK(g_rccl.Broadcast(dbp, dbp, 3, ncclDouble, root, c, h->stream));
     NCCLCHK(g_rccl.GroupEnd());
     HIPCHK(hipStreamSynchronize(h->stream));
-    HIPCHK(hipMemcpy(bp, dbp, sizeof(bp), hipMemcpyDeviceToHost)); (void)hipFree(dbp);
+    HIPCHK(hipMemcpy(bp, dbp, sizeof(bp), hipMemcpyDeviceToHost));
     h->beta1p = bp[0]; h->beta2p = bp[1];
-    if (bp[2] == 0.0) { muon_free(h); return 0; }                       // (every rank has the root's answer, so all of them take the same branch)
-    if (!h->MU) if (int r = muon_alloc(h)) return r;
+    if (bp[2] == 0.0) { (void)hipFree(dbp); muon_free(h); return 0; }   // (every rank has the root's answer, so all of them take the same branch)
+    // A rank that cannot hold the momentum would leave the others waiting in its broadcast: all of them learn first whether every one can, and otherwise return an error together
+    const bool had = h->MU != nullptr; const int mine = had ? 0 : muon_alloc(h); const double can = mine == 0; double all = 0;
+    HIPCHK(hipMemcpy(dbp, &can, sizeof(can), hipMemcpyHostToDevice));
+    NCCLCHK(g_rccl.AllReduce(dbp, dbp, 1, ncclDouble, ncclMin, c, h->stream));
+    HIPCHK(hipStreamSynchronize(h->stream));
+    HIPCHK(hipMemcpy(&all, dbp, sizeof(all), hipMemcpyDeviceToHost)); (void)hipFree(dbp);
+    if (all != 1.0) {
+        if (!had) muon_free(h);
+        h->err = mine ? "md2_broadcast_state: no device memory for Muon's momentum and workspace" : "md2_broadcast_state: another rank has no device memory for Muon's momentum"; return 3;
+    }
     NCCLCHK(g_rccl.Broadcast(h->MU, h->MU, (size_t)h->n_int, ncclFloat, root, c, h->stream));
     HIPCHK(hipStreamSynchronize(h->stream));
     return 0;

@@ -684,3 +684,41 @@ def test_a_refused_step_keeps_the_handles_step_size():
     with pytest.raises(RuntimeError, match="stepped by Muon"):
         m.update(m.ADAM(0.5), model)
     assert model.lr == 2e-4
+
+
+# ---- the state's exchange between ranks ------------------------------------------------------------------------------------------------------
+@gpu
+def test_broadcast_state_leaves_no_rank_waiting_for_one_without_memory():
+    """One rank's part of md2_broadcast_state against a stand-in for RCCL: whether every rank can hold the momentum is agreed on (a reduction that each takes part in) before any of them enters
+    its broadcast, and where one cannot, none does, all return an error, and a momentum allocated for it is given back.  The failing allocation is the host's: nothing reaches the device."""
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__)); assert os.path.exists(os.path.join(here, "native", "libfake_rccl.so")), "run __graft_entry__.build()"
+    r = subprocess.run([sys.executable, "-u", os.path.join(here, "fake_rccl_child.py")], capture_output=True, text=True, timeout=100); assert r.returncode == 0, r.stdout + r.stderr
+    got = {l.split()[0]: l.split(maxsplit=6)[1:] for l in r.stdout.splitlines() if l.split() and l.split()[0] in ("nobody", "dropped", "given", "kept", "other_cannot", "other_cannot_kept", "cannot")}
+    #                            status, broadcasts (parameters, two moments, statistics, the three numbers; the momentum), reductions, this rank's answer, has Muon state
+    assert {k: tuple(float(q) for q in v[:5]) for k, v in got.items()} == {
+        "nobody": (0, 5, 0, -1, 0), "dropped": (0, 5, 0, -1, 0), "given": (0, 6, 1, 1, 1), "kept": (0, 6, 1, 1, 1),
+        "other_cannot": (3, 5, 1, 1, 0), "other_cannot_kept": (3, 5, 1, 1, 1), "cannot": (3, 5, 1, 0, 0)}, r.stdout
+    assert "another rank" in got["other_cannot"][5] and "no device memory" in got["cannot"][5]
+
+
+@gpu
+def test_muon_through_the_librarys_own_communicator():
+    """A handle with Muon state joins a communicator (of one rank: RCCL takes no two on a card): its momentum comes through md2_broadcast_state unchanged, and steps with the gradients summed by
+    the library equal steps without a communicator, bit for bit."""
+    m = md(); opt = m.Muon(eta=1e-3); m.set_deterministic(True)
+    try:
+        runs = []
+        for comm in ("torch", "rccl"):
+            model, params, cache, x = make_model()
+            for _ in range(2):
+                m.train_step(model, x, None, cache, params, do_update=False); m.update(opt, model)
+            st = model.muon_state(); dp = md2amd.parallel.DataParallel(model, comm=comm, x_like=x, parameters=params, cache=cache)
+            assert np.array_equal(model.muon_state(), st) and st.any()
+            losses = [float(dp.train_step(x, None, cache, params, optimizer=opt)) for _ in range(2)]
+            runs.append((losses, model.params(), model.muon_state(), model._opt_and_bn_state()[:4])); model.close()
+        assert runs[0][0] == runs[1][0] and all(np.array_equal(a, b) for a, b in zip(runs[0][1:3], runs[1][1:3])) and all(np.array_equal(a, b) for a, b in zip(runs[0][3], runs[1][3]))
+    finally:
+        m.set_deterministic(False)
