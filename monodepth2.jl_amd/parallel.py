@@ -32,10 +32,18 @@ def shard_range(global_batch, rank, world):
     return lo, lo + base + (1 if rank < rem else 0)
 
 
+def _exchange(t, group, collective):
+    """collective(t), in place; over gloo a GPU's tensor goes through host memory, by copies that wait (gloo given device tensors of ranks that share a card can stop for good)."""
+    if t.is_cuda and dist.get_backend(group) == "gloo":
+        host = t.cpu(); collective(host); t.copy_(host)
+    else:
+        collective(t)
+
+
 def allreduce_sum_(flat, group=None):
     """In-place all-reduce(sum) of a flat gradient buffer; no-op for a single rank."""
     if dist.is_available() and dist.is_initialized() and dist.get_world_size(group) > 1:
-        dist.all_reduce(flat, op=dist.ReduceOp.SUM, group=group)
+        _exchange(flat, group, lambda t: dist.all_reduce(t, op=dist.ReduceOp.SUM, group=group))
     return flat
 
 
@@ -45,7 +53,7 @@ def world_size(group=None):
 
 def broadcast_params_(flat, src=0, group=None):
     if world_size(group) > 1:
-        dist.broadcast(flat, src=src, group=group)
+        _exchange(flat, group, lambda t: dist.broadcast(t, src=src, group=group))
     return flat
 
 
@@ -140,5 +148,5 @@ def verify_rccl(dp, x_common, cache, parameters, g_local, tol=2e-4):
     err = (g / float(w) - g_local).norm() / (g_local.norm() + 1e-30)
     t = torch.tensor([float(err)], device=g.device)
     if w > 1:
-        dist.all_reduce(t, op=dist.ReduceOp.MAX, group=dp.group)
+        _exchange(t, dp.group, lambda v: dist.all_reduce(v, op=dist.ReduceOp.MAX, group=dp.group))
     return bool(float(t.item()) < tol), float(t.item())

@@ -154,3 +154,34 @@ def test_two_rank_data_parallel_step_on_the_hip_gradient_buffer(tmp_path):
     assert np.linalg.norm(l0 - l1) > 0 and np.abs(r0 - (l0 + l1)).max() <= 1e-6 * np.abs(r0).max()          # == the sum of the two HIP shard gradients (ADAM scales by 1/world)
     assert np.array_equal(ld("p_end0.npy"), ld("p_end1.npy"))                                               # and the replicas stay bit-identical over further steps
     assert np.abs(ld("p_end0.npy") - theta0).max() > 1e-5
+
+
+# ---- gloo gets CPU tensors only --------------------------------------------------------------------------------------------------------------------------
+class _CardTensor:
+    """Stands for a GPU's tensor where there is none: what the exchange may do with one is copy it to the host and back."""
+    is_cuda = True
+
+    def __init__(self, t): self.t = t; self.device = t.device
+    def cpu(self): return self.t.clone()
+    def copy_(self, other): self.t.copy_(other); return self
+    def __float__(self): return float(self.t)
+    def item(self): return self.t.item()
+
+
+def _card_worker(rank, world, port, out_dir):
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port), RANK=str(rank), WORLD_SIZE=str(world), LOCAL_RANK=str(rank))
+    import sys
+    sys.path[:0] = [os.path.dirname(os.path.dirname(os.path.abspath(__file__)))]
+    import md2amd as m
+    par = m.parallel; par.init_from_env("gloo")
+    a, b = _CardTensor(torch.arange(5.0) + rank), _CardTensor(torch.full((3,), float(rank)))
+    assert par.allreduce_sum_(a) is a and par.broadcast_params_(b, 1) is b
+    np.save(os.path.join(out_dir, "card%d.npy" % rank), torch.cat([a.t, b.t]).numpy())
+    dist.barrier(); dist.destroy_process_group()
+
+
+def test_a_gpus_tensors_go_through_host_memory_over_gloo(tmp_path):
+    """(a device tensor handed to gloo itself would be refused here: it is no torch tensor)"""
+    world = 2; mp.spawn(_card_worker, args=(world, _free_port(), str(tmp_path)), nprocs=world, join=True)
+    for r in range(world):
+        assert np.array_equal(np.load(tmp_path / ("card%d.npy" % r)), [1, 3, 5, 7, 9, 1, 1, 1])
