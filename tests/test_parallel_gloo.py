@@ -185,3 +185,69 @@ def test_a_gpus_tensors_go_through_host_memory_over_gloo(tmp_path):
     world = 2; mp.spawn(_card_worker, args=(world, _free_port(), str(tmp_path)), nprocs=world, join=True)
     for r in range(world):
         assert np.array_equal(np.load(tmp_path / ("card%d.npy" % r)), [1, 3, 5, 7, 9, 1, 1, 1])
+
+
+# ---- Muon's momentum travels with the other state when the replicas are made identical -------------------------------------------------------------------
+class _StateModel:
+    """The state that DataParallel exchanges, without a handle: dropping Muon's state clears ADAM's, as in the library, so the order of the two restores shows."""
+    def __init__(self, rank, muon):
+        self.flat = torch.full((6,), float(rank)); self.adam = (np.full(6, 10.0 + rank), np.full(6, 20.0 + rank), 0.9 ** (rank + 1), 0.999 ** (rank + 1), np.full(3, 30.0 + rank)); self.mu = np.full(6, 40.0 + rank) if muon else None
+    def _ensure(self, x, parameters, cache): pass
+    def param_buffer(self): return self.flat
+    def _opt_and_bn_state(self): return self.adam
+    def _restore_opt_and_bn_state(self, st): self.adam = st
+    def muon_state(self): return self.mu
+    def load_muon_state(self, st):
+        if st is None and self.mu is not None:
+            self.adam = (np.zeros(6), np.zeros(6), 1.0, 1.0, self.adam[4])
+        self.mu = st
+
+
+def _muon_state_worker(rank, world, port, out_dir):
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port), RANK=str(rank), WORLD_SIZE=str(world), LOCAL_RANK=str(rank))
+    import sys
+    sys.path[:0] = [os.path.dirname(os.path.dirname(os.path.abspath(__file__)))]
+    import md2amd as m
+    par = m.parallel; par.init_from_env("gloo"); m.monodepth._f32 = lambda x: x
+    for has in ((True, False), (False, True), (True, True), (False, False)):
+        model = _StateModel(rank, has[rank]); par.DataParallel(model, comm="torch", x_like=torch.zeros(1), parameters=None, cache=None)
+        got = np.concatenate([model.flat.numpy(), *model.adam[:2], model.adam[2:4], model.adam[4], [] if model.mu is None else model.mu])
+        np.save(os.path.join(out_dir, "s%d%d_%d.npy" % (*has, rank)), got)
+    dist.barrier(); dist.destroy_process_group()
+
+
+def test_muon_state_of_rank_0_reaches_every_rank(tmp_path):
+    world = 2; mp.spawn(_muon_state_worker, args=(world, _free_port(), str(tmp_path)), nprocs=world, join=True)
+    for has in ((1, 0), (0, 1), (1, 1), (0, 0)):
+        root = _StateModel(0, has[0]); want = np.concatenate([root.flat.numpy(), *root.adam[:2], root.adam[2:4], root.adam[4], root.mu if has[0] else []])
+        for r in range(world):
+            assert np.array_equal(np.load(tmp_path / ("s%d%d_%d.npy" % (*has, r))), want), (has, r)
+
+
+def _gpu_muon_worker(rank, world, port, out_dir):
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port), RANK=str(rank), WORLD_SIZE=str(world), LOCAL_RANK="0")
+    import sys
+    sys.path[:0] = [os.path.dirname(os.path.dirname(os.path.abspath(__file__)))]
+    import md2amd as m
+    par = m.parallel; md = m.monodepth; syn = m.synthetic; par.init_from_env("gloo"); torch.cuda.set_device(0)
+    C, H, W = 1, 64, 96; K, iK = syn.depth10k_intrinsics(W, H); params = md.Params(target_size=(W, H), batch_size=1, automasking=False)
+    cache = md.TrainCache(md.SSIM(), md.Backproject(W, H), md.Project(W, H), K, iK, 2, [1, 3], [0.125, 0.25, 0.5, 1.0]); enc = md.ResidualNetwork(18, in_channels=C)
+    model = md.Model(enc, md.DepthDecoder(list(enc.stages), [2, 3, 4, 5]), md.PoseDecoder(512)); model.load_params(syn.init_params(C, seed=5 + rank, randomize_affine=True))
+    x = torch.from_numpy(syn.synthetic_triplets(world, C, H, W, seed=9)[rank:rank + 1].copy()).cuda(); opt = md.Muon(eta=1e-3)
+    md.train_step(model, x, None, cache, params, do_update=False)
+    if rank == 0:
+        md.update(opt, model)
+    dp = par.DataParallel(model, comm="torch", x_like=x, parameters=params, cache=cache); np.save(os.path.join(out_dir, "m0_%d.npy" % rank), model.muon_state())
+    for _ in range(2):
+        dp.train_step(x, None, cache, params, optimizer=opt)
+    np.save(os.path.join(out_dir, "m1_%d.npy" % rank), model.muon_state()); np.save(os.path.join(out_dir, "p1_%d.npy" % rank), model.params())
+    dist.barrier(); dist.destroy_process_group()
+
+
+@pytest.mark.gpu
+def test_two_ranks_step_with_muon(tmp_path):
+    """Rank 0 has stepped with Muon, rank 1 has not: both start from rank 0's momentum and stay bit-identical over further steps."""
+    world = 2; mp.spawn(_gpu_muon_worker, args=(world, _free_port(), str(tmp_path)), nprocs=world, join=True); ld = lambda n: np.load(tmp_path / n)
+    assert ld("m0_0.npy").any() and not np.array_equal(ld("m0_0.npy"), ld("m1_0.npy"))
+    for n in ("m0_", "m1_", "p1_"):
+        assert np.array_equal(ld(n + "0.npy"), ld(n + "1.npy"))
