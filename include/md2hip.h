@@ -291,6 +291,9 @@ int32_t md2_adam_raw(float* p, const float* g, float* m, float* v, int64_t n, in
  * each.  Nothing synchronises, allocates or copies from the host, so all of these can be captured into a graph.  Results do not depend on timing: no atomics.
  * Errors return 2 before anything is enqueued; md2_last_error(NULL) has the reason. */
 int64_t md2_newton_schulz_workspace(int64_t batch, int64_t rows, int64_t cols, int32_t steps, int32_t pullback);
+/* Which kernels a call takes, from its sizes alone (host only): the tile side, 64 or 128, and the pieces its K axis is cut into, of X X^T, b A + c A A, the pullback's S = G X^T + X G^T and
+ * b S + c (S A + A S), and the products of these with the rows x cols matrices.  Side 0: no launch of that kind (all 0: the call is one launch). */
+int32_t md2_newton_schulz_tiles(int64_t batch, int64_t rows, int64_t cols, int32_t steps, int32_t pullback, int32_t* host_side5, int32_t* host_pieces5);
 int32_t md2_newton_schulz(const void* x, void* y, int64_t batch, int64_t rows, int64_t cols, const int64_t* host_x_strides, int32_t dtype, int32_t steps, const double* host_coefficients,
                           double eps, void* workspace, int64_t workspace_bytes, void* stream);
 /* its pullback: dout (like y, strides as x's) -> dx (contiguous, overlapping neither), through every step and the normalisation.  Steps whose pullback could grow a gradient past 8192

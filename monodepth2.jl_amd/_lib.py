@@ -94,6 +94,7 @@ _SIGS = {
     "md2_maxpool3s2_bwd": (I32, [P, P, P, I32, I32, I32, I32, P]),
     "md2_adam_raw": (I32, [P, P, P, P, I64, I32, F64, C.c_float, P]),
     "md2_newton_schulz_workspace": (I64, [I64, I64, I64, I32, I32]),
+    "md2_newton_schulz_tiles": (I32, [I64, I64, I64, I32, I32, C.POINTER(I32), C.POINTER(I32)]),
     "md2_newton_schulz": (I32, [P, P, I64, I64, I64, C.POINTER(I64), I32, I32, C.POINTER(F64), F64, P, I64, P]),
     "md2_newton_schulz_bwd": (I32, [P, P, P, I64, I64, I64, C.POINTER(I64), C.POINTER(I64), I32, I32, C.POINTER(F64), F64, P, I64, P]),
     "md2_muon_workspace": (I64, [C.POINTER(I64), C.POINTER(I64), I32, I32]),

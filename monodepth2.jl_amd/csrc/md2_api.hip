@@ -1501,6 +1501,13 @@ static int ns_options(NsOptions& o, int32_t steps, const double* co, double eps,
 int64_t md2_newton_schulz_workspace(int64_t batch, int64_t rows, int64_t cols, int32_t steps, int32_t pullback) {
     try { NsMatrices q; q.batch = batch; q.rows = rows; q.cols = cols; return ns_workspace(pullback ? NS_BACKWARD : NS_FORWARD, steps, &q, 1); } catch (const std::exception&) { return -1; }
 }
+int32_t md2_newton_schulz_tiles(int64_t batch, int64_t rows, int64_t cols, int32_t steps, int32_t pullback, int32_t* side, int32_t* pieces) {
+    NS_ENTRY(
+        if (!side || !pieces) return ns_fail("newton_schulz_tiles", "null pointer");
+        NsMatrices q; q.batch = batch; q.rows = rows; q.cols = cols;
+        return ns_tiles(pullback ? NS_BACKWARD : NS_FORWARD, steps, &q, 1, side, pieces) ? ns_fail("newton_schulz_tiles", "sizes or steps out of range") : 0;
+    )
+}
 static int ns_call(const char* what, int kind, const void* x, const void* d, void* y, int64_t batch, int64_t rows, int64_t cols, const int64_t* xs, const int64_t* ds, int32_t dtype, int32_t steps,
                    const double* co, double eps, void* ws, int64_t ws_bytes, void* stream) {
     NsOptions o; if (int r = ns_options(o, steps, co, eps, what)) return r;

@@ -24,6 +24,9 @@ struct NsOptions {
 const char* ns_check(int steps, const double* coefficients, double eps);
 // bytes of workspace, -1 for sizes that are refused
 int64_t ns_workspace(int kind, int steps, const NsMatrices* q, int count);
+// which kernels a call takes: tile side and pieces of the K axis of X X^T, b A + c A A, S, V and (pieces 1) the products with m x n; sides 0: none such, or the call is one launch.  -1 for sizes
+// that are refused
+int ns_tiles(int kind, int steps, const NsMatrices* q, int count, int32_t side[5], int32_t pieces[5]);
 // enqueues on s; 0, or 2 with the reason in *why (nothing was enqueued)
 int ns_run(int kind, int dtype, const NsMatrices* q, int count, const NsOptions& o, void* ws, int64_t ws_bytes, hipStream_t s, const char** why);
 

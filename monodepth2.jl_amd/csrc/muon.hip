@@ -1066,6 +1066,22 @@ int64_t ns_workspace(int kind, int steps, const NsMatrices* q, int count) {
     return check_total(ns_layout(p));
 }
 
+int ns_tiles(int kind, int steps, const NsMatrices* q, int count, int32_t side[5], int32_t pieces[5]) {
+    for (int k = 0; k < 5; ++k) side[k] = pieces[k] = 0;
+    if (ns_workspace(kind, steps, q, count) < 0) return -1;
+    NsProblem p; slots_of(kind, steps, p);
+    for (int i = 0; i < count; ++i) p.d.push_back(make_desc(q[i]));
+    if (ns_small(kind, p.d)) return 0;
+    std::stable_sort(p.d.begin(), p.d.end(), [](const Desc& a, const Desc& b) { return a.m > b.m; });
+    ns_layout(p);
+    for (int k = 0; k < p.kinds; ++k) {
+        if (p.cuts.fuse && (k == POLY || k == SYM_V)) continue;      // (done by X X^T's and S's workgroups)
+        const int kb = kblocks(k, p.d[0].m, p.d[0].n); side[k] = p.cuts.sym[k].tile; pieces[k] = cdiv(kb, cdiv(kb, cdiv(kb, p.cuts.sym[k].chunk)));
+    }
+    side[4] = p.cuts.nn_tile; pieces[4] = 1;
+    return 0;
+}
+
 template <int DT> static void ns_launch(int kind, NsProblem& p, const Layout& L, char* base, const NsOptions& o, const Plan& P, hipStream_t s) {
     Ws ws; ws.mats = (Mat*)(base + L.mats); for (int k = 0; k < SYMS; ++k) { ws.sym[k] = (Item*)(base + L.sym[k]); ws.red[k] = (Item*)(base + L.red[k]); } ws.nn = (Item*)(base + L.nn); ws.pk = (Item*)(base + L.pk); ws.fac = (Fac*)(base + L.fac); ws.part = (double*)(base + L.part); ws.split = base + L.split; ws.buf = base + L.buf;
     const int steps = o.steps;

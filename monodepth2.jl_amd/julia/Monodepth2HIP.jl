@@ -455,6 +455,9 @@ ns_strides(x) = Int64[size(x, 1) * size(x, 2), size(x, 1), 1]
 rawptr(x::ROCArray) = Ptr{Cvoid}(UInt(pointer(x)))                     # of any element type (dptr: Float32 only)
 ns_coefficients(c) = length(c) == 3 ? collect(Float64, c) : throw(ArgumentError("coefficients: expected (a, b, c), got $(length(c))"))
 muon_adjust(a) = a === :spectral ? Int32(0) : a === :rms ? Int32(1) : throw(ArgumentError("adjust must be :spectral or :rms, not $a"))
+function newton_schulz_tiles(B, R, K; steps=5, pullback=false)         # which kernels a call takes: (tile sides, pieces of the K axis) of its five products
+    side = Vector{Int32}(undef, 5); pieces = Vector{Int32}(undef, 5); GC.@preserve side pieces ok(md2_newton_schulz_tiles(Int64(B), Int64(R), Int64(K), Int32(steps), Int32(pullback), pointer(side), pointer(pieces)), "newton_schulz_tiles"); side, pieces
+end
 function newton_schulz(x::ROCArray{T,3}; steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7) where {T}
     dt = ns_dtype(T); K, R, B = size(x); y = similar(x); n = md2_newton_schulz_workspace(Int64(B), Int64(R), Int64(K), Int32(steps), Int32(0)); ws = ROCArray{UInt8}(undef, max(n, 0)); co = ns_coefficients(coefficients); st = ns_strides(x)
     GC.@preserve co st ws ok(md2_newton_schulz(rawptr(x), rawptr(y), Int64(B), Int64(R), Int64(K), pointer(st), dt, Int32(steps), pointer(co), Float64(eps), rawptr(ws), n, NOSTREAM), "newton_schulz"); y

@@ -722,3 +722,74 @@ def test_muon_through_the_librarys_own_communicator():
         assert runs[0][0] == runs[1][0] and all(np.array_equal(a, b) for a, b in zip(runs[0][1:3], runs[1][1:3])) and all(np.array_equal(a, b) for a, b in zip(runs[0][3], runs[1][3]))
     finally:
         m.set_deterministic(False)
+
+
+# ---- 128-tiles ---------------------------------------------------------------------------------------------------------------------------------
+def tiles(shape, pullback, steps=5):
+    """-> (tile sides, whether the K axis is cut) of X X^T, b A + c A A, S, V and the products with the matrix."""
+    b, r, c = shape; I = ctypes.c_int32 * 5; side, pieces = I(), I()
+    assert md2amd._lib.lib().md2_newton_schulz_tiles(b, r, c, steps, pullback, side, pieces) == 0
+    return tuple(side), tuple(int(p > 1) for p in pieces)
+
+
+def test_which_kernels_a_call_takes():
+    L = md2amd._lib.lib(); I = ctypes.c_int32 * 5
+    assert tiles((1, 64, 576), 0) == ((0,) * 5, (0,) * 5) and tiles((1, 64, 576), 1)[0][1::2] == (0, 0)      # one launch | B and V by the workgroups of A and S
+    assert tiles((3, 4601, 509), 1) == tiles((3, 509, 4601), 1)
+    assert L.md2_newton_schulz_tiles(0, 4, 4, 5, 0, I(), I()) == 2 and L.md2_newton_schulz_tiles(1, 4, 4, 0, 0, I(), I()) == 2 and L.md2_newton_schulz_tiles(1, 4, 4, 5, 0, None, I()) == 2
+
+
+def held(e, ep, dtype, loose, floor):
+    assert e <= HALF[dtype] + loose and e <= HALF[dtype] + max(2 * ep, floor), (e, ep)
+
+
+def on_the_gpu(x, f):
+    """f of every matrix of the batch by itself, in 64 bits and in 32, where x is."""
+    return tuple(torch.stack([f(i, t) for i in range(x.shape[0])]) for t in (torch.float64, torch.float32))
+
+
+# (batch, rows, columns), its tile sides and which K axes are cut: one of the smallest for each combination with a 128-tile in it that sizes of up to 1500 and batches of up to 24 have
+FORWARD_128 = [((6, 129, 903), (64, 64, 0, 0, 128), (0, 0, 0, 0, 0)), ((1, 509, 4601), (64, 64, 0, 0, 128), (1, 0, 0, 0, 0)), ((1, 4608, 512), (64, 64, 0, 0, 128), (1, 0, 0, 0, 0)),
+               ((24, 257, 335), (64, 128, 0, 0, 128), (0, 0, 0, 0, 0)), ((1, 997, 4501), (128, 64, 0, 0, 128), (1, 0, 0, 0, 0)), ((2, 997, 997), (128, 128, 0, 0, 64), (1, 1, 0, 0, 0)),
+               ((24, 257, 257), (128, 128, 0, 0, 128), (0, 0, 0, 0, 0)), ((8, 1283, 641), (128, 128, 0, 0, 128), (1, 0, 0, 0, 0)), ((2, 997, 1297), (128, 128, 0, 0, 128), (1, 1, 0, 0, 0))]
+BACK_128 = [((12, 129, 465), (64, 64, 64, 64, 128), (0, 0, 0, 0, 0)), ((6, 903, 129), (64, 64, 64, 64, 128), (0, 0, 1, 0, 0)), ((1, 512, 4608), (64, 64, 64, 64, 128), (1, 0, 1, 1, 0)),
+            ((12, 197, 1379), (64, 64, 128, 64, 128), (0, 0, 1, 0, 0)), ((1, 997, 1995), (64, 64, 128, 64, 64), (0, 0, 1, 0, 0)), ((4, 641, 641), (64, 64, 128, 128, 64), (0, 0, 1, 1, 0)),
+            ((4, 833, 641), (64, 64, 128, 128, 128), (0, 0, 1, 1, 0)), ((24, 257, 335), (64, 128, 64, 64, 128), (0, 0, 0, 0, 0)), ((1, 1000, 4500), (128, 64, 128, 64, 128), (1, 0, 1, 0, 0)),
+            ((4, 641, 1283), (128, 64, 128, 128, 64), (1, 0, 1, 1, 0)), ((3, 1539, 769), (128, 64, 128, 128, 128), (1, 0, 1, 1, 0)), ((24, 257, 257), (128, 128, 64, 64, 128), (0, 0, 0, 0, 0)),
+            ((2, 997, 997), (128, 128, 128, 128, 64), (1, 1, 1, 1, 0)), ((24, 385, 385), (128, 128, 128, 128, 128), (0, 0, 0, 0, 0)), ((2, 997, 1297), (128, 128, 128, 128, 128), (1, 1, 1, 1, 0))]
+
+
+def test_the_128_tile_cases_take_128_tiles():
+    for cases, pullback in ((FORWARD_128, 0), (BACK_128, 1)):
+        for shape, side, cut in cases:
+            assert tiles(shape, pullback) == (side, cut), shape
+
+
+@gpu
+@pytest.mark.parametrize("dtype", list(HALF))
+@pytest.mark.parametrize("shape", [c[0] for c in FORWARD_128])
+def test_newton_schulz_in_128_tiles(shape, dtype):
+    x = gradient_like(shape, sum(shape)).to(dtype).cuda(); y = md().newton_schulz(x)
+    exact, plain = on_the_gpu(x, lambda i, t: ns_plain(x[i].to(t)))
+    held(rel(y, exact), rel(plain, exact), dtype, LOOSE, 2e-6)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", list(HALF))
+@pytest.mark.parametrize("shape", [c[0] for c in BACK_128])
+def test_newton_schulz_pullback_in_128_tiles(shape, dtype):
+    x = gradient_like(shape, sum(shape)).to(dtype).cuda(); d = torch.randn(shape, generator=torch.Generator().manual_seed(2), dtype=torch.float64).to(dtype).cuda()
+    dx = md().newton_schulz_pullback(x, d)
+    exact, plain = on_the_gpu(x, lambda i, t: back_plain(x[i], d[i], 5, COEF, 1e-7, t))
+    held(rel(dx, exact), rel(plain, exact), dtype, 4 * LOOSE, 4e-6)
+
+
+@gpu
+@pytest.mark.parametrize("shape,pullback", [((8, 641, 641), 1), ((2, 997, 1297), 1), ((1, 509, 4601), 1), ((24, 257, 335), 0)])
+def test_128_tiles_do_not_depend_on_what_the_workspace_held(shape, pullback):
+    m = md(); x = gradient_like(shape, 3).float().cuda(); d = torch.randn(shape, generator=torch.Generator().manual_seed(4)).cuda(); got = []
+    assert tiles(shape, pullback)[0][4] == 128
+    for fill in (math.nan, 0.0):
+        torch.cuda.empty_cache(); junk = torch.full((1 << 28,), fill, device="cuda"); torch.cuda.synchronize(); del junk      # 1 GB: the workspace is cut from it
+        got.append(m.newton_schulz_pullback(x, d) if pullback else m.newton_schulz(x))
+    assert torch.equal(*got) and torch.isfinite(got[0]).all()
