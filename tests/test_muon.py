@@ -793,3 +793,23 @@ def test_128_tiles_do_not_depend_on_what_the_workspace_held(shape, pullback):
         torch.cuda.empty_cache(); junk = torch.full((1 << 28,), fill, device="cuda"); torch.cuda.synchronize(); del junk      # 1 GB: the workspace is cut from it
         got.append(m.newton_schulz_pullback(x, d) if pullback else m.newton_schulz(x))
     assert torch.equal(*got) and torch.isfinite(got[0]).all()
+
+
+@gpu
+def test_the_largest_weights_of_the_resnet50_network():
+    """test_model_update_with_muon leaves the values of ResNet-50's weights of more than 2^20 elements unchecked (256 x 18432, 256 x 11520, 2048 x 1024, 512 x 4608, ...: 128-tiles and cut K axes of
+    a list).  Here they are held to the same bounds, against 64 bits where the card multiplies: the momentum element by element, the weight by its step."""
+    m = md(); model, params, cache, x = make_model(50); opt = m.Muon(eta=1e-3, weight_decay=0.1, adjust="rms"); mom = None
+    for _ in range(2):
+        m.train_step(model, x, None, cache, params, do_update=False); p0, g = arrays(model.params(), 50), arrays(model.grads(), 50)
+        m.update(opt, model, grad_scale=0.5); p1, got = arrays(model.params(), 50), arrays(model.muon_state(), 50); count = 0
+        for name, (kind, after) in p1.items():
+            if not hidden(name, kind) or after.size <= 1 << 20:
+                continue
+            count += 1; up = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()
+            t = up(p0[name][1]), up(g[name][1]), up(mom[name][1]) if mom else torch.zeros(after.shape, device="cuda")
+            ep, em, step = muon_plain(*t, 1e-3, 0.95, True, 0.1, "rms", 0.5); a, mu = up(after).double(), up(got[name][1]).double()
+            assert float((mu - em).abs().max()) <= 3 * 2.0 ** -24 * float(t[1].abs().max() + t[2].abs().max()), name
+            assert float((a - ep).norm()) <= float(2 * 2.0 ** -24 * (t[0].double().norm() + step.norm()) + 2e-5 * step.norm()), name
+        assert count == 7
+        mom = got
