@@ -238,3 +238,16 @@ def test_bench_convolution_class_accounting(tmp_path):
     floor_s = 8.0e9 / 157.3e12 + (2.0 * M * co * 9 * ci) * (16.0 / 36.0) * 6.0 / 2500e12 + (2.0 * M * co * ci) / 157.3e12
     assert abs(acct["floor_ms"] - floor_s * 1e3) < 1e-6 * floor_s * 1e3
     assert acct["launches_by_product_form"] == {"fp32": 2.0, "split3": 1.0}
+
+
+def test_every_stream_has_the_default_priority():
+    """Work on streams of different priorities can stop for good on this hardware: no source asks for another one."""
+    bad = []
+    asks = re.compile("Stream" + "CreateWithPriority|is_high_priority" + r"_stream\s*=\s*True|Stream\([^)]*priority" + r"\s*=")
+    for top in ("monodepth2.jl_amd", "tests", "tools", "perf", "include"):
+        for d, _, files in os.walk(os.path.join(ROOT, top)):
+            for f in files:
+                if f.endswith((".hip", ".h", ".cpp", ".py", ".jl")):
+                    text = open(os.path.join(d, f), encoding="utf-8").read()
+                    bad += ["%s: %s" % (os.path.join(d, f), m.group(0)) for m in asks.finditer(text)]
+    text = open(os.path.join(ROOT, "bench.py")).read(); assert not asks.search(text) and not bad, bad
