@@ -338,17 +338,23 @@ void launch_pose_compose_bwd(const float* rvec, const float* tvec, const double*
 #define GRID1D(total) dim3((int)std::max<long>(1, std::min<long>(((total) + 255) / 256, 4096))), dim3(256)
 #define FOR1D(i, total) for (long i = blockIdx.x * (long)blockDim.x + threadIdx.x; i < (total); i += (long)gridDim.x * blockDim.x)
 
+// the reflected 3 x 3 window's sums of x, y, x x, y y and x y; every product and sum is rounded by itself, so that all kernels that take an SSIM (or its minimum over predictions) agree in
+// every bit
+__device__ __forceinline__ void window_sums(const float* __restrict__ xp, const float* __restrict__ yp, int h, int w, int H, int W, float& sx, float& sy, float& sxx, float& syy, float& sxy) {
+#pragma clang fp contract(off)
+    sx = sy = sxx = syy = sxy = 0.f;
+    for (int dy = -1; dy <= 1; ++dy)
+        for (int dx = -1; dx <= 1; ++dx) {
+            const int o = refl_idx(h + dy, H) * W + refl_idx(w + dx, W);
+            const float xv = xp[o], yv = yp[o];
+            sx += xv; sy += yv; sxx += xv * xv; syy += yv * yv; sxy += xv * yv;
+        }
+}
 __global__ void op_ssim_kernel(const float* __restrict__ x, const float* __restrict__ y, float* __restrict__ out, int planes, int H, int W) {
     FOR1D(i, (long)planes * H * W) {
         const int w = i % W; const long t = i / W; const int h = t % H; const long p = t / H;
         const float* xp = x + p * H * W; const float* yp = y + p * H * W;
-        float sx = 0.f, sy = 0.f, sxx = 0.f, syy = 0.f, sxy = 0.f;
-        for (int dy = -1; dy <= 1; ++dy)
-            for (int dx = -1; dx <= 1; ++dx) {
-                const int o = refl_idx(h + dy, H) * W + refl_idx(w + dx, W);
-                const float xv = xp[o], yv = yp[o];
-                sx += xv; sy += yv; sxx += xv * xv; syy += yv * yv; sxy += xv * yv;
-            }
+        float sx, sy, sxx, syy, sxy; window_sums(xp, yp, h, w, H, W, sx, sy, sxx, syy, sxy);
         SsimOut so; ssim_from_sums(sx, sy, sxx, syy, sxy, false, so);
         out[i] = so.val;
     }
@@ -364,13 +370,7 @@ __global__ void op_prediction_kernel(const float* __restrict__ preds, int k, con
             float ss = 0.f, l1 = 0.f;
             for (int c = 0; c < C; ++c) {
                 const float* xp = preds + (long)j * pj + (long)n * pn + (long)c * P; const float* yp = tgt + (long)n * tn + (long)c * P;
-                float sx = 0.f, sy = 0.f, sxx = 0.f, syy = 0.f, sxy = 0.f;
-                for (int dy = -1; dy <= 1; ++dy)
-                    for (int dx = -1; dx <= 1; ++dx) {
-                        const int o = refl_idx(h + dy, H) * W + refl_idx(w + dx, W);
-                        const float xv = xp[o], yv = yp[o];
-                        sx += xv; sy += yv; sxx += xv * xv; syy += yv * yv; sxy += xv * yv;
-                    }
+                float sx, sy, sxx, syy, sxy; window_sums(xp, yp, h, w, H, W, sx, sy, sxx, syy, sxy);
                 SsimOut so; ssim_from_sums(sx, sy, sxx, syy, sxy, false, so);
                 ss += so.val; l1 += fabsf(yp[(long)h * W + w] - xp[(long)h * W + w]);
             }
@@ -490,13 +490,7 @@ __global__ void op_ssim_bwd_kernel(const float* __restrict__ x, const float* __r
                         float d = dout[dbase + qo];
                         if (win && win[dbase + qo] != wj) d = 0.f;
                         if (d == 0.f) continue;
-                        float sx = 0.f, sy = 0.f, sxx = 0.f, syy = 0.f, sxy = 0.f;
-                        for (int a = -1; a <= 1; ++a)
-                            for (int b = -1; b <= 1; ++b) {
-                                const int o = refl_idx(qy + a, H) * W + refl_idx(qx + b, W);
-                                const float xa = xp[o], ya = yp[o];
-                                sx += xa; sy += ya; sxx += xa * xa; syy += ya * ya; sxy += xa * ya;
-                            }
+                        float sx, sy, sxx, syy, sxy; window_sums(xp, yp, qy, qx, H, W, sx, sy, sxx, syy, sxy);
                         SsimOut so; ssim_from_sums(sx, sy, sxx, syy, sxy, true, so);
                         g += d * (1.f / 9.f) * (so.g_mx + 2.f * xv * so.g_pxx + yv * so.g_pxy);
                     }
@@ -521,13 +515,7 @@ __global__ void op_prediction_argmin_kernel(const float* __restrict__ preds, int
             float ss = 0.f, l1 = 0.f;
             for (int c = 0; c < C; ++c) {
                 const float* xp = preds + (long)j * pj + (long)n * pn + (long)c * P; const float* yp = tgt + (long)n * tn + (long)c * P;
-                float sx = 0.f, sy = 0.f, sxx = 0.f, syy = 0.f, sxy = 0.f;
-                for (int dy = -1; dy <= 1; ++dy)
-                    for (int dx = -1; dx <= 1; ++dx) {
-                        const int o = refl_idx(h + dy, H) * W + refl_idx(w + dx, W);
-                        const float xv = xp[o], yv = yp[o];
-                        sx += xv; sy += yv; sxx += xv * xv; syy += yv * yv; sxy += xv * yv;
-                    }
+                float sx, sy, sxx, syy, sxy; window_sums(xp, yp, h, w, H, W, sx, sy, sxx, syy, sxy);
                 SsimOut so; ssim_from_sums(sx, sy, sxx, syy, sxy, false, so);
                 ss += so.val; l1 += fabsf(yp[(long)h * W + w] - xp[(long)h * W + w]);
             }

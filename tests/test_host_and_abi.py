@@ -251,3 +251,19 @@ def test_every_stream_has_the_default_priority():
                     text = open(os.path.join(d, f), encoding="utf-8").read()
                     bad += ["%s: %s" % (os.path.join(d, f), m.group(0)) for m in asks.finditer(text)]
     text = open(os.path.join(ROOT, "bench.py")).read(); assert not asks.search(text) and not bad, bad
+
+
+def test_no_kernel_is_compiled_with_packed_fp32_arithmetic():
+    """Some forms of v_pk_add_f32, v_pk_mul_f32 and v_pk_fma_f32 have given wrong results on this hardware, which hipcc makes of ordinary float code: every compilation of kernels turns the
+    feature off, and none is written by hand."""
+    import subprocess
+    src = os.path.join(ROOT, "monodepth2.jl_amd", "csrc")
+    lines = [l for l in subprocess.run(["make", "-C", src, "-n", "-B"], capture_output=True, text=True, check=True).stdout.splitlines() if " -c " in l]
+    assert len(lines) == len([f for f in os.listdir(src) if f.endswith(".hip")]) >= 8
+    entry = [l for l in open(os.path.join(ROOT, "__graft_entry__.py")).read().splitlines() if "hipcc" in l and "check_call" in l]
+    for l in lines:
+        assert "-Xclang -target-feature -Xclang -packed-fp32-ops" in l, l
+    assert entry and all('"-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"' in l for l in entry)
+    for f in os.listdir(src):
+        if f.endswith((".hip", ".h")):
+            assert not re.search(r"v_pk_(add|mul|fma)" + "_f32", open(os.path.join(src, f)).read()), f
