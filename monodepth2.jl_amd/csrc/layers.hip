@@ -928,25 +928,23 @@ void launch_pose_mean_bwd(const float* drvec, const float* dtvec, const View& dy
 }
 
 // ---- Flux ADAM (beta 0.9/0.999, eps 1e-8): one fused pass over the flat parameter buffer ------------------------------------------
+// (one element; shared by every kernel below, so that a parameter's bits do not depend on which of them stepped it)
+__device__ __forceinline__ void adam_element(float& p, float g, float& m, float& v, float c1, float c2, float lr, float gs) {
+    const float ge = g * gs;
+    m = 0.9f * m + (1.f - 0.9f) * ge;
+    v = 0.999f * v + (1.f - 0.999f) * ge * ge;
+    p -= m / c1 / (sqrtf(v / c2) + 1e-8f) * lr;
+}
 __global__ __launch_bounds__(256) void adam_kernel(float* __restrict__ p, const float* __restrict__ g, float* __restrict__ m, float* __restrict__ v, long n4, float c1, float c2, float lr, float gs) {
     for (long i = blockIdx.x * (long)blockDim.x + threadIdx.x; i < n4; i += (long)gridDim.x * blockDim.x) {
         float4 P = ld4(p + i * 4), G = ld4(g + i * 4), M = ld4(m + i * 4), V = ld4(v + i * 4);
-        float* pp = &P.x; float* gg = &G.x; float* mm = &M.x; float* vv = &V.x;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float ge = gg[e] * gs;
-            mm[e] = 0.9f * mm[e] + (1.f - 0.9f) * ge;
-            vv[e] = 0.999f * vv[e] + (1.f - 0.999f) * ge * ge;
-            pp[e] -= mm[e] / c1 / (sqrtf(vv[e] / c2) + 1e-8f) * lr;
-        }
+        adam_element(P.x, G.x, M.x, V.x, c1, c2, lr, gs); adam_element(P.y, G.y, M.y, V.y, c1, c2, lr, gs); adam_element(P.z, G.z, M.z, V.z, c1, c2, lr, gs); adam_element(P.w, G.w, M.w, V.w, c1, c2, lr, gs);
         st4(p + i * 4, P); st4(m + i * 4, M); st4(v + i * 4, V);
     }
 }
 __global__ void adam_tail_kernel(float* __restrict__ p, const float* __restrict__ g, float* __restrict__ m, float* __restrict__ v, long n, float c1, float c2, float lr, float gs) {
     const long i = blockIdx.x * (long)blockDim.x + threadIdx.x; if (i >= n) return;
-    const float ge = g[i] * gs;
-    m[i] = 0.9f * m[i] + (1.f - 0.9f) * ge; v[i] = 0.999f * v[i] + (1.f - 0.999f) * ge * ge;
-    p[i] -= m[i] / c1 / (sqrtf(v[i] / c2) + 1e-8f) * lr;
+    adam_element(p[i], g[i], m[i], v[i], c1, c2, lr, gs);
 }
 // the same for the listed ranges of the flat buffers only (what Muon leaves to ADAM): r[i] = {first float4, float4s before this range}, r[n] = {-, all of them}
 __global__ __launch_bounds__(256) void adam_ranges_kernel(float* __restrict__ p, const float* __restrict__ g, float* __restrict__ m, float* __restrict__ v, const long2* __restrict__ r, int n, float c1, float c2,
@@ -957,14 +955,7 @@ __global__ __launch_bounds__(256) void adam_ranges_kernel(float* __restrict__ p,
         while (lo < hi) { const int q = (lo + hi + 1) / 2; if (r[q].y <= i) lo = q; else hi = q - 1; }
         const long at = (r[lo].x + (i - r[lo].y)) * 4;
         float4 P = ld4(p + at), G = ld4(g + at), M = ld4(m + at), V = ld4(v + at);
-        float* pp = &P.x; float* gg = &G.x; float* mm = &M.x; float* vv = &V.x;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float ge = gg[e] * gs;
-            mm[e] = 0.9f * mm[e] + (1.f - 0.9f) * ge;
-            vv[e] = 0.999f * vv[e] + (1.f - 0.999f) * ge * ge;
-            pp[e] -= mm[e] / c1 / (sqrtf(vv[e] / c2) + 1e-8f) * lr;
-        }
+        adam_element(P.x, G.x, M.x, V.x, c1, c2, lr, gs); adam_element(P.y, G.y, M.y, V.y, c1, c2, lr, gs); adam_element(P.z, G.z, M.z, V.z, c1, c2, lr, gs); adam_element(P.w, G.w, M.w, V.w, c1, c2, lr, gs);
         st4(p + at, P); st4(m + at, M); st4(v + at, V);
     }
 }

@@ -813,3 +813,18 @@ def test_the_largest_weights_of_the_resnet50_network():
             assert float((a - ep).norm()) <= float(2 * 2.0 ** -24 * (t[0].double().norm() + step.norm()) + 2e-5 * step.norm()), name
         assert count == 7
         mom = got
+
+
+@gpu
+def test_adams_bits_do_not_depend_on_which_kernel_steps_a_parameter():
+    """adam_raw on an aligned buffer (four parameters a thread, the last ones singly) and on one that begins 4 bytes later (all singly); the listed ranges that Muon leaves to ADAM are held to the
+    plain ADAM step, bit for bit, in test_model_update_with_muon."""
+    m = md(); n = 4099; g = torch.Generator().manual_seed(71); start = [torch.randn(n, generator=g) * s for s in (0.1, 1e-3, 1e-3)] + [torch.rand(n, generator=g) * 1e-6]; got = []
+    for off in (0, 1):
+        t = [torch.zeros(n + 4, device="cuda")[off:off + n] for _ in range(4)]
+        for a, b in zip(t, start):
+            a.copy_(b)
+        for step in (1, 2, 3):
+            m.adam_raw(*t, step, lr=1e-3, grad_scale=0.5)
+        got.append([a.clone() for a in t])
+    assert all(torch.equal(a, b) for a, b in zip(*got)) and not torch.equal(got[0][0].cpu(), start[0])
