@@ -943,8 +943,7 @@ __global__ __launch_bounds__(256) void adam_kernel(float* __restrict__ p, const 
     }
 }
 __global__ void adam_tail_kernel(float* __restrict__ p, const float* __restrict__ g, float* __restrict__ m, float* __restrict__ v, long n, float c1, float c2, float lr, float gs) {
-    const long i = blockIdx.x * (long)blockDim.x + threadIdx.x; if (i >= n) return;
-    adam_element(p[i], g[i], m[i], v[i], c1, c2, lr, gs);
+    for (long i = blockIdx.x * (long)blockDim.x + threadIdx.x; i < n; i += (long)gridDim.x * blockDim.x) adam_element(p[i], g[i], m[i], v[i], c1, c2, lr, gs);
 }
 // the same for the listed ranges of the flat buffers only (what Muon leaves to ADAM): r[i] = {first float4, float4s before this range}, r[n] = {-, all of them}
 __global__ __launch_bounds__(256) void adam_ranges_kernel(float* __restrict__ p, const float* __restrict__ g, float* __restrict__ m, float* __restrict__ v, const long2* __restrict__ r, int n, float c1, float c2,

@@ -208,3 +208,10 @@ def test_adam_raw_matches_oracle():
         net.set_grads(gg); net.adam_step(1e-3)
         md().adam_raw(pd, dev(g), m, v, step, lr=1e-3)
     assert rel(host(pd), net.get_params()[:n]) < 1e-6
+
+
+def test_adam_raw_steps_every_element_of_a_large_unaligned_buffer():
+    """4096 workgroups of 256 (2^20 elements) are the most a launch has: a buffer that does not begin at a multiple of 16 bytes is stepped one element a thread, all of it."""
+    n = (1 << 20) + 5000; t = [torch.zeros(n + 4, device="cuda")[1:n + 1] for _ in range(4)]; t[1].fill_(1.0)
+    md().adam_raw(*t, 1, lr=1e-3)
+    assert float(t[0].max()) < -0.9e-3 and float(t[2].min()) > 0.09 and float(t[3].min()) > 0.9e-3
