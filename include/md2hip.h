@@ -287,7 +287,7 @@ int32_t md2_adam_raw(float* p, const float* g, float* m, float* v, int64_t n, in
  * drives every singular value towards 1 and keeps the singular vectors.  host_coefficients: a, b, c (3.4445, -4.7750, 2.0315); coefficients that let a singular value grow past 4
  * are refused, as is an eps above 3.4e38.  x: any non-negative strides, host_x_strides = {batch, row, column} in elements; y: contiguous.  dtype: 0 fp32, 1 bf16, 2 fp16 (x and y); inside, fp32 accuracy in
  * every product.  y must not overlap x (refused).  A matrix of zeros gives zeros; a matrix with a NaN or an infinity gives NaNs and leaves the others of its batch alone.
- * workspace: device memory of at least md2_newton_schulz_workspace() bytes (-1 = refused sizes), aligned to 256; calls that can run at the same time, captured ones too, need one
+ * workspace: device memory of at least md2_newton_schulz_workspace() bytes (-1 = refused sizes), aligned to 256, overlapping nothing else of the call (refused); calls that can run at the same time, captured ones too, need one
  * each.  Nothing synchronises, allocates or copies from the host, so all of these can be captured into a graph.  Results do not depend on timing: no atomics.
  * Errors return 2 before anything is enqueued; md2_last_error(NULL) has the reason. */
 int64_t md2_newton_schulz_workspace(int64_t batch, int64_t rows, int64_t cols, int32_t steps, int32_t pullback);

@@ -1168,12 +1168,13 @@ const char* ns_check(int steps, const double* co, double eps) {
     const Plan P = ns_bounds(steps, co, false);
     return P.ok ? nullptr : P.why;
 }
-// does the contiguous result share memory with what `st` reaches from p?
-static bool overlaps(const NsMatrices& q, const void* p, const int64_t st[3], int el) {
-    const __int128 y0 = (__int128)(uintptr_t)q.y, y1 = y0 + (__int128)q.batch * q.rows * q.cols * el, p0 = (__int128)(uintptr_t)p;
+// does memory of so many bytes share any with what `st` reaches from p? | the contiguous result?
+static bool overlaps(const void* a, __int128 bytes, const NsMatrices& q, const void* p, const int64_t st[3], int el) {
+    const __int128 a0 = (__int128)(uintptr_t)a, p0 = (__int128)(uintptr_t)p;
     const __int128 p1 = p0 + ((__int128)(q.batch - 1) * st[0] + (__int128)(q.rows - 1) * st[1] + (__int128)(q.cols - 1) * st[2] + 1) * el;
-    return y0 < p1 && p0 < y1;
+    return a0 < p1 && p0 < a0 + bytes;
 }
+static bool overlaps(const NsMatrices& q, const void* p, const int64_t st[3], int el) { return overlaps(q.y, (__int128)q.batch * q.rows * q.cols * el, q, p, st, el); }
 int ns_run(int kind, int dtype, const NsMatrices* q, int count, const NsOptions& o, void* wsp, int64_t ws_bytes, hipStream_t s, const char** why) {
     if (!eps_ok(o.eps)) { *why = kEps; return 2; }
     const Plan P = ns_bounds(o.steps, o.coef, kind == NS_BACKWARD);
@@ -1195,6 +1196,11 @@ int ns_run(int kind, int dtype, const NsMatrices* q, int count, const NsOptions&
     Layout L{}; L.total = 256;
     if (!ns_small(kind, p.d)) { L = ns_layout(p); if (check_total(L) < 0) { *why = "too many matrices"; return 2; } }
     if (!wsp || (uintptr_t)wsp % 256 || ws_bytes < L.total) { *why = "the workspace is missing, too small or not aligned to 256 bytes"; return 2; }
+    if (!ns_small(kind, p.d))                                    // (which uses none)
+        for (int i = 0; i < count; ++i) {
+            const NsMatrices& m = q[i]; const int64_t ys[3] = {m.rows * m.cols, m.cols, 1};
+            if (overlaps(wsp, L.total, m, m.x, m.xs, el) || overlaps(wsp, L.total, m, m.y, ys, el) || (m.d && overlaps(wsp, L.total, m, m.d, m.ds, el))) { *why = "the workspace overlaps an input or a result"; return 2; }
+        }
     if (dtype == NS_F32) ns_launch<NS_F32>(kind, p, L, (char*)wsp, o, P, s);
     else if (dtype == NS_BF16) ns_launch<NS_BF16>(kind, p, L, (char*)wsp, o, P, s);
     else ns_launch<NS_F16>(kind, p, L, (char*)wsp, o, P, s);

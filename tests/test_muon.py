@@ -828,3 +828,17 @@ def test_adams_bits_do_not_depend_on_which_kernel_steps_a_parameter():
             m.adam_raw(*t, step, lr=1e-3, grad_scale=0.5)
         got.append([a.clone() for a in t])
     assert all(torch.equal(a, b) for a, b in zip(*got)) and not torch.equal(got[0][0].cpu(), start[0])
+
+
+@pytest.mark.parametrize("which", ["x", "y", "dout", "p", "g", "m"])
+def test_a_workspace_that_overlaps_the_calls_tensors_is_refused(which):
+    """200 x 300 fp32 matrices (240000 bytes, more than a workgroup keeps in LDS), the workspace over the last 256 bytes of one of them."""
+    L = md2amd._lib.lib(); size = 240000; at = {k: (i + 1) << 30 for i, k in enumerate(("x", "y", "dout", "p", "g", "m"))}; ws = (at[which] + size - 1) // 256 * 256
+    st, co = (ctypes.c_int64 * 3)(60000, 300, 1), (ctypes.c_double * 3)(*COEF); V, I = ctypes.c_void_p, ctypes.c_int64
+    if which in "pgm":
+        r = L.md2_muon_raw((V * 1)(at["p"]), (V * 1)(at["g"]), (V * 1)(at["m"]), (I * 1)(200), (I * 1)(300), 1, 0.02, 0.95, 1, 0.0, 0, 1.0, 5, co, 1e-7, ws, 1 << 40, None)
+    elif which == "dout":
+        r = L.md2_newton_schulz_bwd(at["x"], at["dout"], at["y"], 1, 200, 300, st, st, 0, 5, co, 1e-7, ws, 1 << 40, None)
+    else:
+        r = L.md2_newton_schulz(at["x"], at["y"], 1, 200, 300, st, 0, 5, co, 1e-7, ws, 1 << 40, None)
+    assert r == 2 and "workspace overlaps" in last_error()
