@@ -863,10 +863,13 @@ _NS_DEFAULT = _F64x3(*NS_COEFFICIENTS)
 
 
 def _ns_args(steps, coefficients, eps):
+    """(numbers of steps outside the library's 1..16 stay outside: what no int32 holds would wrap into it)"""
     co = tuple(coefficients)
     if len(co) != 3:
         raise ValueError("coefficients: expected (a, b, c)")
-    return int(steps), _NS_DEFAULT if co == NS_COEFFICIENTS else _F64x3(*(float(c) for c in co)), float(eps)
+    if int(steps) != steps:
+        raise ValueError("steps: expected a whole number")
+    return min(max(int(steps), 0), 17), _NS_DEFAULT if co == NS_COEFFICIENTS else _F64x3(*(float(c) for c in co)), float(eps)
 
 
 def _on(device):

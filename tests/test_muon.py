@@ -842,3 +842,12 @@ def test_a_workspace_that_overlaps_the_calls_tensors_is_refused(which):
     else:
         r = L.md2_newton_schulz(at["x"], at["y"], 1, 200, 300, st, 0, 5, co, 1e-7, ws, 1 << 40, None)
     assert r == 2 and "workspace overlaps" in last_error()
+
+
+def test_numbers_of_steps_that_no_int32_holds():
+    m = md()
+    for bad, passed in ((1 << 32 | 5, 17), (-(1 << 32) + 5, 0), (-3, 0), (0, 0), (17, 17), (5, 5), (16, 16), (5.0, 5)):
+        assert m._ns_args(bad, COEF, 1e-7)[0] == passed
+    for bad in (2.5, math.nan, math.inf):
+        with pytest.raises((ValueError, OverflowError)):
+            m._ns_args(bad, COEF, 1e-7)
