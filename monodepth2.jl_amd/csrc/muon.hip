@@ -11,11 +11,12 @@
 // Numbers.  A singular value grows by up to a per step, so what is rounded in an early step is amplified by up to a^steps (485 with the default coefficients): operands of 8 or
 // 11 bits leave errors of 1e-3 .. 4e-3 relative to the result.  Every operand is therefore a PAIR of f16, x = hi + lo with 22 significant bits, and a product three
 // v_mfma_f32_32x32x16_f16 (hi hi + hi lo + lo hi) with fp32 sums: 1.0 - 1.2x the error of plain fp32 products against 64 bits, at a third of the f16 rate instead of the fp32 MFMA's
-// sixteenth.  The pairs are scaled by powers of two that come from bounds of the iterates' norms (ns_plan), so that no hi overflows and the lo of a typical entry is a normal number.
+// sixteenth.  The pairs are scaled by powers of two that come from bounds of the iterates' norms (ns_bounds), so that no hi overflows and the lo of a typical entry is a normal number.
 // a X is added in fp32 in the epilogue: inside B (B + a I) its rounding would be the largest error of all.  Norms are sums in 64 bits.
 //
 // Layout.  A pair matrix is row-major in blocks of 16 columns, 64 bytes each: 16 hi, then 16 lo -- what an MFMA K-step reads of a row is contiguous.  Rows are padded to 128,
-// columns of X to 128, with zeros that every step keeps (rows of B beyond m are 0), so the products need no bounds checks.
+// columns of X to 128, with zeros that every step keeps (rows of B beyond m are 0), so the products need no bounds checks.  A thin matrix pays for that in memory: 1 x 2^20 fp32 (4 MB) that
+// does not fit a workgroup takes 1.1 GB of workspace, 3.8 GB for its pullback (every iterate of five steps), 17 x 3 x 9000 (1.8 MB) 164 and 570 MB.
 #include "md2_internal.h"
 #include "muon.h"
 #include <cmath>
@@ -563,18 +564,14 @@ template <int T> __global__ __launch_bounds__(256, T == 128 ? 2 : 1) void ns_sym
 }
 // the shares of a tile, summed in order: 16 rows of a 128-tile or 32 of a 64-tile a workgroup (8 KB of each share)
 template <int T> __device__ inline void reduce_tile(float* tile, const Item& it, const Ws& ws, const SymArgs& a, int r0) {
-    constexpr int R = 2048 / T, N = 1; const float* in = reinterpret_cast<const float*>(ws.split + (int64_t)it.part * PART) + r0 * T + threadIdx.x * 8;
-    f32x4 v[N][2] = {};
+    constexpr int R = 2048 / T; const float* in = reinterpret_cast<const float*>(ws.split + (int64_t)it.part * PART) + r0 * T + threadIdx.x * 8;
+    f32x4 v[2] = {};
 #pragma unroll 8
     for (int k = 0; k < it.k1; ++k)
 #pragma unroll
-        for (int z = 0; z < N; ++z)
+        for (int h = 0; h < 2; ++h) v[h] += *reinterpret_cast<const f32x4*>(in + (int64_t)k * T * T + h * 4);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) v[z][h] += *reinterpret_cast<const f32x4*>(in + (int64_t)k * T * T + z * 2048 + h * 4);
-#pragma unroll
-    for (int z = 0; z < N; ++z)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) *reinterpret_cast<f32x4*>(tile + tile_at<T>((z * 256 + threadIdx.x) / (T / 8), threadIdx.x % (T / 8) * 8 + h * 4)) = v[z][h];
+    for (int h = 0; h < 2; ++h) *reinterpret_cast<f32x4*>(tile + tile_at<T>(threadIdx.x / (T / 8), threadIdx.x % (T / 8) * 8 + h * 4)) = v[h];
     __syncthreads();
     sym_finish<T, R>(it, a, ws.fac, tile, 1, r0);
 }
@@ -963,7 +960,10 @@ struct NsProblem { std::vector<Desc> d; std::vector<Use> u; Strides st{}; int nX
 // 128-tiles share a staged row between two waves (half the loads of 64-tiles, whose four waves split K instead) and are the faster ones where they fill the chip; a call with few tiles is over
 // sooner in 64-tiles, and sooner still with its K axis cut.  Measured: a block of 16 K takes a 128-tile 0.4 us at two workgroups a CU and 0.5 alone, a 64-tile 0.14 (a step of its waves,
 // 0.55, is four blocks) and 0.22 where the chip is full of them (their loads); a workgroup's way in and out is 4 us, which two 128-tiles a CU hide from each other; a cut K axis costs a launch of 5 us and its partial sums' way through memory.
-// (512 x 4608, X X^T: 180 128-tile pieces 13 us and 6 to join them, 36 64-tiles uncut 32; B X: 144 128-tiles 19.5, 576 64-tiles 23.  512 x 2304, B X: 72 128-tiles 20, 288 64-tiles 15.)
+// (512 x 4608, X X^T: 36 64-tiles in five pieces, which it takes, 14.9 us and 4.8 to join them, uncut 45; ten 128-tiles in 18 pieces 13.0 and 5.9.  B X: 144 128-tiles 19.3, 576 64-tiles 23.
+// 512 x 2304, B X: 72 128-tiles 20, 288 64-tiles 15.)
+// Of lists, whose items are of many lengths, it only ranks the choices: it gives the ResNet-18 and -50 networks' b A + c A A 9.5 and 25.8 us, where 64-tiles take 16.5 and 41.3 (an item that
+// follows another on its CU costs more than 0.14 a block) and 128-tiles 28.2 and 44.4; their B X 44 and 98, measured 59.6 and 127; ResNet-50's X X^T 77 with the join, measured 86 + 12.7.
 static constexpr int CUS = 256, MIN128 = 16, MIN64 = 16;
 static constexpr double LAUNCH = 5.0, PART_US = 64.0 * 1024 * 2 / 5.0e6;
 static double launch_us(int tile, int64_t items, int64_t work, int64_t longest, bool equal) {      // items, their K blocks in all, the longest one's; equal: they come in whole rounds
@@ -1022,7 +1022,7 @@ static Layout ns_layout(NsProblem& p) {
     L.part = take((2 * L.n_pk + L.n_nn) * sizeof(double)); L.split = take(split_max * PART); L.buf = take(buf); L.total = at;
     return L;
 }
-static bool fits(int64_t batch, int64_t rows, int64_t cols) {      // sizes whose work items and element counts stay far inside 31 bits
+static bool fits(int64_t batch, int64_t rows, int64_t cols) {      // (a matrix may have 2^31 elements: offsets of elements are 64-bit; the work items are counted in check_total)
     return rows > 0 && cols > 0 && batch > 0 && rows <= (1 << 20) && cols <= (1 << 20) && rows * cols <= (1ll << 31) && batch <= (1 << 20);
 }
 static int64_t check_total(const Layout& L) {      // (a launch has fewer than 2^32 threads: 2^24 workgroups of 256)
