@@ -147,7 +147,7 @@ int32_t md2_opt_state_set(md2_handle* h, const float* host_m, const float* host_
  * momentum and a workspace (no call can be captured into a graph: ADAM's bias corrections change with every step) and makes the handle Muon's: md2_adam_step and md2_train_step's update then return an error, because the
  * hidden convolutions' ADAM moments are no longer kept, until md2_muon_state_set(h, NULL, 0). */
 int32_t md2_muon_step(md2_handle* h, double lr, double momentum, int32_t nesterov, double weight_decay, int32_t adjust, int32_t steps, const double* host_coefficients, double eps, float grad_scale);
-/* Muon's momentum (Flux parameter layout, host; 0 where ADAM steps): count = md2_params_count(h) once the handle has it, 0 before.  set gives the handle Muon state (a resumed run);
+/* Muon's momentum (Flux parameter layout, host; 0 where ADAM steps): count = md2_params_count(h) once the handle has it, 0 before.  set gives the handle Muon state (a resumed run; a loss-only handle keeps it, as it does ADAM's);
  * set(h, NULL, 0) drops it and starts ADAM anew (moments zero, beta powers 1); md2_params_set does both, too. */
 int64_t md2_muon_state_count(md2_handle* h);
 int32_t md2_muon_state_get(md2_handle* h, float* host_momentum, int64_t n);

@@ -1650,7 +1650,6 @@ int32_t md2_muon_state_set(md2_handle* h, const float* host, int64_t n) {
             KCHK(); return 0;
         }
         if (!host || n != h->n_flux) { h->err = "md2_muon_state_set: wrong parameter count"; return 2; }
-        if (!h->net_ok) { h->err = "md2_muon_state_set: this handle is loss-only"; return 2; }
         if (!h->MU) if (int r = muon_alloc(h)) return r;
         std::vector<float> in((size_t)h->n_int), only((size_t)h->n_int, 0.f);
         convert_params(h, in.data(), const_cast<float*>(host), true);

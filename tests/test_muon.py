@@ -851,3 +851,19 @@ def test_numbers_of_steps_that_no_int32_holds():
     for bad in (2.5, math.nan, math.inf):
         with pytest.raises((ValueError, OverflowError)):
             m._ns_args(bad, COEF, 1e-7)
+
+
+@gpu
+def test_muon_state_survives_a_shape_that_only_the_loss_takes():
+    """An image too small for the network gives the model a loss-only handle for that call: the momentum passes through it, as ADAM's moments do."""
+    m = md(); model, params, cache, x = make_model(); opt = m.Muon(eta=1e-3)
+    m.train_step(model, x, None, cache, params, do_update=False); m.update(opt, model); st, adam, p = model.muon_state(), model._opt_and_bn_state(), model.params()
+    H = W = 48; K, iK = md2amd.synthetic.depth10k_intrinsics(W, H); small = torch.from_numpy(md2amd.synthetic.synthetic_triplets(2, 1, H, W, seed=6)).cuda(); g = torch.Generator().manual_seed(5)
+    cs = m.TrainCache(m.SSIM(), m.Backproject(W, H), m.Project(W, H), K, iK, 2, [1, 3], [0.125, 0.25, 0.5, 1.0]); model._ensure(small, m.Params(target_size=(W, H), batch_size=2, automasking=False), cs)
+    disps = [(0.2 + 0.6 * torch.rand(2, 1, H >> k, W >> k, generator=g)).cuda() for k in (3, 2, 1, 0)]; r, t = [(0.01 * torch.randn(2, 2, 3, generator=g)).cuda() for _ in range(2)]
+    assert np.isfinite(float(m.loss_fwd_bwd(model, small, disps, r, t)[0]))
+    with pytest.raises(RuntimeError, match="loss-only"):
+        m.update(opt, model)
+    m.train_step(model, x, None, cache, params, do_update=False)
+    assert np.array_equal(model.muon_state(), st) and np.array_equal(model.params(), p) and all(np.array_equal(a, b) for a, b in zip(model._opt_and_bn_state()[:4], adam[:4]))
+    m.update(opt, model); assert not np.array_equal(model.muon_state(), st)
