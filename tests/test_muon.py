@@ -867,3 +867,18 @@ def test_muon_state_survives_a_shape_that_only_the_loss_takes():
     m.train_step(model, x, None, cache, params, do_update=False)
     assert np.array_equal(model.muon_state(), st) and np.array_equal(model.params(), p) and all(np.array_equal(a, b) for a, b in zip(model._opt_and_bn_state()[:4], adam[:4]))
     m.update(opt, model); assert not np.array_equal(model.muon_state(), st)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape,pullback", [((5, 97, 211), 0), ((1, 512, 4608), 0), ((1, 512, 2304), 1), ((3, 385, 130), 1)])
+def test_16_bit_results_are_roundings_of_results_as_accurate_as_fp32(shape, pullback, dtype):
+    """Element by element: what is further from 64 bits than half a step of its type (fp16: of its subnormals, 2^-25) is so by no more than fp32's own error, whose root mean square the tests
+    above bound by twice plain fp32's; the largest of 10^6 elements is held to eight times that.  Where two such results lie on both sides of a tie they differ by one step, and neither is the
+    better one.  The same call gives the same bits."""
+    m = md(); x = gradient_like(shape, sum(shape)).to(dtype).cuda(); d = torch.randn(shape, generator=torch.Generator().manual_seed(2), dtype=torch.float64).to(dtype).cuda()
+    call = (lambda: m.newton_schulz_pullback(x, d)) if pullback else (lambda: m.newton_schulz(x))
+    exact, plain = on_the_gpu(x, (lambda i, t: back_plain(x[i], d[i], 5, COEF, 1e-7, t)) if pullback else (lambda i, t: ns_plain(x[i].to(t))))
+    y = call(); off = 8 * max(2 * rel(plain, exact), 4e-6 if pullback else 2e-6) * exact.square().mean().sqrt()
+    assert ((y.double() - exact).abs() <= HALF[dtype] * (exact.abs() + off) + (2.0 ** -25 if dtype == torch.float16 else 0.0) + off).all()
+    assert all(torch.equal(y, call()) for _ in range(5))
