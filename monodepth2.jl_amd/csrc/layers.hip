@@ -930,10 +930,10 @@ void launch_pose_mean_bwd(const float* drvec, const float* dtvec, const View& dy
 // ---- Flux ADAM (beta 0.9/0.999, eps 1e-8): one fused pass over the flat parameter buffer ------------------------------------------
 // (one element; shared by every kernel below, so that a parameter's bits do not depend on which of them stepped it)
 __device__ __forceinline__ void adam_element(float& p, float g, float& m, float& v, float c1, float c2, float lr, float gs) {
-    const float ge = g * gs;
-    m = 0.9f * m + (1.f - 0.9f) * ge;
-    v = 0.999f * v + (1.f - 0.999f) * ge * ge;
-    p -= m / c1 / (sqrtf(v / c2) + 1e-8f) * lr;
+    const float ge = g * gs;                             // (which products are fused is written out: left to the compiler it differed from kernel to kernel)
+    m = fmaf(0.9f, m, (1.f - 0.9f) * ge);
+    v = fmaf(ge, (1.f - 0.999f) * ge, 0.999f * v);
+    p = fmaf(-(m / c1 / (sqrtf(v / c2) + 1e-8f)), lr, p);
 }
 __global__ __launch_bounds__(256) void adam_kernel(float* __restrict__ p, const float* __restrict__ g, float* __restrict__ m, float* __restrict__ v, long n4, float c1, float c2, float lr, float gs) {
     for (long i = blockIdx.x * (long)blockDim.x + threadIdx.x; i < n4; i += (long)gridDim.x * blockDim.x) {

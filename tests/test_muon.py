@@ -828,6 +828,11 @@ def test_adams_bits_do_not_depend_on_which_kernel_steps_a_parameter():
             m.adam_raw(*t, step, lr=1e-3, grad_scale=0.5)
         got.append([a.clone() for a in t])
     assert all(torch.equal(a, b) for a, b in zip(*got)) and not torch.equal(got[0][0].cpu(), start[0])
+    # the moments' roundings: m = fma(0.9, m, 0.1 g), v = fma(g, 0.001 g, 0.999 v) (in 64 bits, which hold the fused product; two roundings of a sum differ from one in 2^-29 of cases)
+    f = np.float32; b1, b2 = f(0.9), f(0.999); m0, v0, ge = start[2].numpy(), start[3].numpy(), start[1].numpy() * f(0.5)
+    for _ in range(3):
+        m0 = (np.float64(b1) * m0 + np.float64((f(1) - b1) * ge)).astype(f); v0 = (np.float64(ge) * ((f(1) - b2) * ge) + np.float64(b2 * v0)).astype(f)
+    assert (got[0][2].cpu().numpy() != m0).sum() <= 2 and (got[0][3].cpu().numpy() != v0).sum() <= 2
 
 
 @pytest.mark.parametrize("which", ["x", "y", "dout", "p", "g", "m"])
