@@ -169,7 +169,7 @@ int32_t md2_comm_world(md2_handle* h, int32_t* rank, int32_t* world);
 int32_t md2_comm_bucket_plan(const md2_config* cfg, int64_t* lo4, int64_t* hi4, int64_t* count);
 int32_t md2_allreduce_grads(md2_handle* h);                 /* sum over ranks of the gradient buffer; no-op when md2_backward already reduced it */
 int32_t md2_comm_allreduce(md2_handle* h, float* dev_buf, int64_t n);   /* in-place sum of any device buffer (loss logging, self-checks) */
-int32_t md2_broadcast_state(md2_handle* h, int32_t root);   /* parameters, ADAM moments + beta powers, Muon's momentum (a rank without any gets it, a root without any takes it away), BatchNorm running statistics of `root` to every rank */
+int32_t md2_broadcast_state(md2_handle* h, int32_t root);   /* parameters, ADAM moments + beta powers, Muon's momentum (a rank without any gets it, a root without any takes it away; where a rank has no device memory for it, every rank returns 3 and no momentum moves), BatchNorm running statistics of `root` to every rank */
 
 /* The loss half alone (src/training.jl:28-77) given disparities and poses; pullbacks may be NULL.
  * ddisp_i like disp_i; drvec/dtvec [2][N][3]. */
